@@ -104,7 +104,9 @@ EXPORTS = ['eg_default_config', 'eg_variable_count', 'eg_variable_info', 'eg_cre
            'eg_last_error', 'eg_set_variable', 'eg_get_variable', 'eg_upload_batch', 'eg_substep',
            'eg_train_step', 'eg_train_batch', 'eg_losses_wait', 'eg_read_losses', 'eg_eval_losses', 'eg_infer', 'eg_infer_upload', 'eg_infer_run', 'eg_infer_download', 'eg_sync', 'eg_comm_unique_id', 'eg_comm_init',
            'eg_comm_reduce_scalars', 'eg_comm_info', 'eg_comm_timing', 'eg_comm_timing_read',
-           'eg_profile_begin', 'eg_profile_end', 'eg_profile_layers', 'eg_memory_stats', 'eg_mfma_probe', 'eg_test_op', 'eg_net_forward', 'eg_crc32c']
+           'eg_profile_begin', 'eg_profile_end', 'eg_profile_layers', 'eg_memory_stats', 'eg_mfma_probe', 'eg_test_op', 'eg_net_forward', 'eg_crc32c',
+           'eg_layer_norm', 'eg_layer_norm_workspace', 'eg_layer_norm_backward', 'eg_quantize_rows', 'eg_int8_matmul_workspace',
+           'eg_int8_matmul', 'eg_distill_loss_workspace', 'eg_distill_loss']
 
 _lib = None
 
@@ -157,6 +159,18 @@ def load_library() -> C.CDLL:
                                    C.c_longlong]
     lib.eg_crc32c.restype = C.c_uint
     lib.eg_crc32c.argtypes = [C.c_uint, C.c_void_p, C.c_ulonglong]
+    # operators over rows in device memory: pointers as plain addresses
+    p, i, n, f = C.c_void_p, C.c_int, C.c_longlong, C.c_float
+    lib.eg_layer_norm.argtypes = [i, p, i, p, n, i, p, p, n, n, f, i, p, n, p, p]
+    lib.eg_layer_norm_workspace.argtypes = [n, n]
+    lib.eg_layer_norm_backward.argtypes = [i, p, i, p, n, p, n, p, p, i, p, p, n, n, i, p, n, p, p, p, n]
+    lib.eg_quantize_rows.argtypes = [i, p, i, p, n, i, p, p, f, n, n, p, n, p]
+    lib.eg_int8_matmul_workspace.argtypes = [n, n, n]
+    lib.eg_int8_matmul.argtypes = [i, p, p, n, p, p, n, p, p, n, n, n, i, p, n, p, n]
+    lib.eg_distill_loss_workspace.argtypes = [n, n]
+    lib.eg_distill_loss.argtypes = [i, p, i, p, n, i, p, n, p, n, p, n, n, n, f, p, p, n, p, n]
+    for name in ('eg_layer_norm_workspace', 'eg_int8_matmul_workspace', 'eg_distill_loss_workspace'):
+        getattr(lib, name).restype = n
     _lib = lib
     return lib
 

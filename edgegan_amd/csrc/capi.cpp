@@ -14,6 +14,7 @@ struct eg_ctx {
 };
 
 static thread_local std::string g_create_error;
+void eg_set_global_error(const char* what) { g_create_error = what; }   // (rowops.cpp: entries without a context)
 
 static Config to_config(const eg_config* k) {
   EG_CHECK(k, "null eg_config");

@@ -1,0 +1,109 @@
+// Operators over rows in device memory (C entries: rowops.cpp; kernels: k_layer_norm.hip, k_int8.hip, k_distill.hip).
+// A row is `cols` consecutive elements; rows are `ld` elements apart (ld >= cols, any alignment).
+#pragma once
+#include <hip/hip_runtime.h>
+
+namespace eg {
+
+enum RowType { ROW_F32 = 0, ROW_BF16 = 1, ROW_F16 = 2 };
+
+struct LayerNormArgs {
+  const void* x;
+  long long ldx;
+  const void *gamma, *beta;   // [cols] or null
+  long long rows;
+  int cols;
+  float eps;
+  int act;                    // ACT_NONE / ACT_RELU / ACT_LRELU
+  void* y;
+  long long ldy;
+  float *mean, *rstd;         // [rows]; null: not stored (forward), required (backward)
+};
+struct LayerNormGradArgs {
+  const void *dy, *x;
+  long long lddy, ldx;
+  const float *mean, *rstd;
+  const void *gamma, *beta;
+  long long rows;
+  int cols;
+  int act;
+  void* dx;                   // null: not wanted
+  long long lddx;
+  int acc_x;                  // dx += (f32 only)
+  void *dgamma, *dbeta;       // null: not wanted
+  int acc_w;                  // dgamma +=, dbeta += (f32 parameters only)
+  float* partial;             // layer_norm_partial_floats()
+};
+// J_v of the layer norm at x and its reverse (f32; the gradient penalty of a critic)
+struct LayerNormTangentArgs {
+  const float *x, *mean, *rstd, *gamma, *beta, *tx;
+  long long rows;
+  int cols;
+  int act;
+  float* ty;                  // forward: act' gamma P tx
+  const float* dty;           // reverse: the gradient of ty ...
+  float* dtx;                 //   ... gives that of tx, x and gamma
+  int acc_t;
+  float* dx;
+  int acc_x;
+  float* dgamma;
+  int acc_w;
+  float* partial;
+};
+struct QuantizeArgs {
+  const void* x;
+  long long ldx;
+  const float *gamma, *beta;  // the fused layer norm's (null: 1, 0)
+  bool norm;
+  float eps;
+  long long rows;
+  int cols;
+  signed char* q;
+  long long ldq;
+  float* scale;
+};
+struct Int8Args {
+  const signed char* a;
+  long long lda;
+  const float* a_scale;
+  const signed char* b;
+  long long ldb;
+  const float* b_scale;
+  const float* bias;          // [n] or null
+  long long m;
+  int n, k;
+  void* out;
+  long long ldo;
+};
+struct DistillArgs {
+  const void* logits;
+  long long ld;
+  const void* index;          // int32 or int64
+  long long ld_index;
+  int index64;
+  const float* teacher;
+  long long ld_teacher;
+  const float* row_weight;    // [rows] or null
+  long long rows;
+  int cols, top;
+  float temperature;
+  float weight;               // a factor of every row
+  float* loss;                // [rows]
+  void* grad;                 // null: not wanted
+  long long ldg;
+  int acc;                    // grad += (f32 only)
+  float* partial;             // distill_partial_floats()
+};
+
+size_t layer_norm_partial_floats(long long rows, int cols);
+void launch_layer_norm(const LayerNormArgs& a, int type, int wtype, hipStream_t s);
+void launch_layer_norm_backward(const LayerNormGradArgs& a, int type, int wtype, hipStream_t s);
+void launch_layer_norm_tangent(const LayerNormTangentArgs& a, hipStream_t s);
+void launch_layer_norm_tangent_backward(const LayerNormTangentArgs& a, hipStream_t s);
+void launch_quantize_rows(const QuantizeArgs& a, int type, hipStream_t s);
+size_t int8_partial_floats(long long m, int n, int k);
+void launch_int8_matmul(const Int8Args& a, int out_type, float* partial, hipStream_t s);
+size_t distill_partial_floats(long long rows, int cols);
+void launch_distill(const DistillArgs& a, int type, hipStream_t s);
+
+}  // namespace eg

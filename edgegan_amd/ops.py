@@ -1,0 +1,241 @@
+"""Operators over rows on torch tensors of the GPU: layer norm and its gradient, 8-bit quantisation and the product of 8-bit
+integer matrices, distillation from a teacher's top logits.
+
+They are for training and inference code beside the engine (a head behind the encoder's features, a recogniser that the classifier learns
+from); the engine runs the same kernels where ``E_norm`` / ``G_norm`` / ``D_norm`` is 'layernorm', in ``EdgeGAN.set_teacher`` and in 8-bit inference.
+A call works on the current stream of its tensors' device, allocates its results there with torch, waits for nothing, and may be
+captured into a graph.  The last dimension is the row; the dimensions before it have to be one stride apart as if they were a single one (a slice of columns is fine, a transposed
+view is not).  Every refusal raises EdgeGANLibError.  There is no autograd: the gradient calls are explicit, as everywhere in this package."""
+from __future__ import annotations
+
+import sys
+from typing import Optional, Tuple
+
+import torch
+
+from ._lib import EdgeGANLibError, load_library
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_ACTS = {None: 0, 'none': 0, 'relu': 1, 'lrelu': 2}
+_lib = None
+
+
+def _library():
+    """The library, on the HIP runtime that torch uses (two runtimes in a process share neither streams nor memory)."""
+    global _lib
+    if _lib is None:
+        lib = load_library()
+        if sys.platform == 'linux':
+            with open('/proc/self/maps') as f:
+                runtimes = {line.split()[-1] for line in f if 'libamdhip64' in line}
+            if len(runtimes) > 1:
+                raise EdgeGANLibError('the engine was loaded before torch and runs on another HIP runtime '
+                                      f'({", ".join(sorted(runtimes))}): import torch or edgegan_amd.ops first')
+        _lib = lib
+    return _lib
+
+
+def _refuse(what: str):
+    raise EdgeGANLibError(what)
+
+
+def _rows(x: torch.Tensor, name: str, types=_TYPES) -> Tuple[int, int, int]:
+    """(rows, cols, elements between rows) of a GPU tensor of one of `types`."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        _refuse(f'{name}: a tensor on the GPU is required')
+    if x.dtype not in types:
+        _refuse(f'{name}: {x.dtype} is not one of {", ".join(str(t) for t in types)}')
+    shape, stride = x.shape, x.stride()
+    if len(shape) == 0:
+        _refuse(f'{name}: at least one dimension is required')
+    cols = shape[-1]
+    if cols > 1 and stride[-1] != 1:
+        _refuse(f'{name}: the last dimension has to be consecutive (stride {stride[-1]})')
+    if len(shape) == 2:
+        rows = shape[0]
+        ld = stride[0] if rows > 1 else cols
+    elif len(shape) == 1:
+        return 1, cols, cols
+    else:
+        rows, ld = 1, cols
+        for n, s in zip(reversed(shape[:-1]), reversed(stride[:-1])):
+            if n == 1:
+                continue
+            if rows == 1:
+                ld = s
+            elif s != ld * rows:
+                _refuse(f'{name}: dimensions {tuple(shape[:-1])} with strides {tuple(stride[:-1])} are not rows one stride apart')
+            rows *= n
+    if rows > 1 and ld < cols:
+        _refuse(f'{name}: rows {ld} elements apart overlap')
+    return rows, cols, ld
+
+
+def _vector(v: Optional[torch.Tensor], n: int, name: str, x: torch.Tensor, types) -> Optional[int]:
+    """The address of a consecutive vector of n elements beside x (None: null)."""
+    if v is None:
+        return None
+    if not isinstance(v, torch.Tensor) or v.device != x.device:
+        _refuse(f'{name}: a tensor on {x.device} is required')
+    if v.dtype not in types:
+        _refuse(f'{name}: {v.dtype} is not one of {", ".join(str(t) for t in types)}')
+    if v.numel() != n or not v.is_contiguous():
+        _refuse(f'{name}: {n} consecutive elements are required, not {tuple(v.shape)} with strides {tuple(v.stride())}')
+    return v.data_ptr()
+
+
+def _act(act) -> int:
+    if act not in _ACTS:
+        _refuse(f'act: {act!r} is not one of {", ".join(repr(a) for a in _ACTS)}')
+    return _ACTS[act]
+
+
+def _stream(x: torch.Tensor) -> Tuple[int, int]:
+    return x.device.index, torch.cuda.current_stream(x.device).cuda_stream
+
+
+def _check(rc: int):
+    if rc:
+        raise EdgeGANLibError(_lib.eg_last_error(None).decode())
+
+
+def _workspace(size: int, x: torch.Tensor) -> Tuple[Optional[torch.Tensor], Optional[int], int]:
+    if size < 0:
+        _refuse('sizes out of range')
+    if size == 0:
+        return None, None, 0
+    w = torch.empty(size, dtype=torch.uint8, device=x.device)
+    return w, w.data_ptr(), size
+
+
+def _parameter_type(weight, bias, x) -> Tuple[int, Tuple]:
+    """One type for both: that of x or f32."""
+    given = [p.dtype for p in (weight, bias) if isinstance(p, torch.Tensor)]
+    t = given[0] if given else torch.float32
+    if t not in (x.dtype, torch.float32) or any(g != t for g in given):
+        _refuse(f'weight, bias: both {x.dtype} or both torch.float32, not {", ".join(str(g) for g in given)}')
+    return _TYPES[t], (t,)
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5,
+               act: Optional[str] = None, statistics: bool = False):
+    """y = act((x - mean) rstd weight + bias) over the last dimension, in x's type (f32, bf16, f16); act: None, 'relu', 'lrelu' (slope 0.2).
+
+    statistics: also returns mean and rstd (f32, one of each row), which layer_norm_backward needs."""
+    lib = _lib or _library()
+    rows, cols, ld = _rows(x, 'x')
+    wtype, types = _parameter_type(weight, bias, x)
+    w, b = _vector(weight, cols, 'weight', x, types), _vector(bias, cols, 'bias', x, types)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean = rstd = None
+    if statistics:
+        mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        rstd = torch.empty_like(mean)
+    device, stream = _stream(x)
+    _check(lib.eg_layer_norm(device, stream, _TYPES[x.dtype], x.data_ptr(), ld, wtype, w, b, rows, cols, eps, _act(act), y.data_ptr(), cols,
+                             mean.data_ptr() if statistics else None, rstd.data_ptr() if statistics else None))
+    return (y, mean, rstd) if statistics else y
+
+
+def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, weight: Optional[torch.Tensor] = None,
+                        bias: Optional[torch.Tensor] = None, act: Optional[str] = None):
+    """(dx, dweight, dbias) of layer_norm at x, with the statistics that it returned; dweight is None without a weight, dbias without a bias."""
+    lib = _lib or _library()
+    rows, cols, ld = _rows(x, 'x')
+    if not isinstance(dy, torch.Tensor) or dy.device != x.device or dy.dtype != x.dtype or dy.shape != x.shape:
+        _refuse(f'dy: {x.dtype} of shape {tuple(x.shape)} on {x.device} is required')
+    _, _, ldy = _rows(dy, 'dy')
+    f32 = (torch.float32,)
+    m, r = _vector(mean, rows, 'mean', x, f32), _vector(rstd, rows, 'rstd', x, f32)
+    if m is None or r is None:
+        _refuse('mean, rstd: required')
+    wtype, types = _parameter_type(weight, bias, x)
+    w, b = _vector(weight, cols, 'weight', x, types), _vector(bias, cols, 'bias', x, types)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dweight = torch.empty_like(weight) if weight is not None else None
+    dbias = torch.empty_like(bias) if bias is not None else None
+    keep, ws, size = _workspace(lib.eg_layer_norm_workspace(rows, cols) if w or b else 0, x)
+    device, stream = _stream(x)
+    _check(lib.eg_layer_norm_backward(device, stream, _TYPES[x.dtype], dy.data_ptr(), ldy, x.data_ptr(), ld, m, r, wtype, w, b, rows, cols, _act(act),
+                                      dx.data_ptr(), cols, dweight.data_ptr() if w else None, dbias.data_ptr() if b else None, ws, size))
+    return dx, dweight, dbias
+
+
+def _norm_parameters(norm, cols, x):
+    if norm is None:
+        return 0, None, None, 1.0
+    if not isinstance(norm, (tuple, list)) or len(norm) != 3:
+        _refuse('norm: (weight or None, bias or None, eps) is required')
+    f32 = (torch.float32,)
+    return 1, _vector(norm[0], cols, 'norm weight', x, f32), _vector(norm[1], cols, 'norm bias', x, f32), float(norm[2])
+
+
+def quantize_rows(x: torch.Tensor, norm=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(q, scale): q int8 of x's shape, scale f32 of each row = max |x| / 127; q = the whole number nearest to 127 x / max |x|, a tie to the even one.
+
+    A row of zeros has scale 0; one with a NaN or an infinity has scale NaN.  norm = (weight, bias, eps): of layer_norm(x, weight, bias, eps) in the same pass
+    (weight, bias f32 or None).  q's rows are a multiple of 16 bytes apart, the gap zeros: what int8_matmul reads fastest."""
+    lib = _lib or _library()
+    rows, cols, ld = _rows(x, 'x')
+    on, g, b, eps = _norm_parameters(norm, cols, x)
+    pitch = (cols + 15) // 16 * 16
+    q = torch.empty(x.shape[:-1] + (pitch,), dtype=torch.int8, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    device, stream = _stream(x)
+    _check(lib.eg_quantize_rows(device, stream, _TYPES[x.dtype], x.data_ptr(), ld, on, g, b, eps, rows, cols, q.data_ptr(), pitch, scale.data_ptr()))
+    return (q if pitch == cols else q[..., :cols]), scale
+
+
+def int8_matmul(q: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """out[..., j] = (sum_k q[..., k] weight[j, k]) scale[...] weight_scale[j] + bias[j], the sum in 32-bit integers.
+
+    q int8 [..., k] with a scale for each row, weight int8 [n, k] with a scale for each output channel (both as quantize_rows returns them; k <= 131071),
+    bias f32 [n] or None; out in out_dtype (f32, bf16, f16)."""
+    lib = _lib or _library()
+    i8, f32 = (torch.int8,), (torch.float32,)
+    m, k, lda = _rows(q, 'q', i8)
+    n, kw, ldb = _rows(weight, 'weight', i8)
+    if weight.dim() != 2 or weight.device != q.device or kw != k:
+        _refuse(f'weight: [n, {k}] on {q.device} is required, not {tuple(weight.shape)} on {weight.device}')
+    if out_dtype not in _TYPES:
+        _refuse(f'out_dtype: {out_dtype} is not one of {", ".join(str(t) for t in _TYPES)}')
+    s, ws, b = _vector(scale, m, 'scale', q, f32), _vector(weight_scale, n, 'weight_scale', q, f32), _vector(bias, n, 'bias', q, f32)
+    if s is None or ws is None:
+        _refuse('scale, weight_scale: required')
+    out = torch.empty(q.shape[:-1] + (n,), dtype=out_dtype, device=q.device)
+    keep, wp, size = _workspace(lib.eg_int8_matmul_workspace(m, n, k), q)
+    device, stream = _stream(q)
+    _check(lib.eg_int8_matmul(device, stream, q.data_ptr(), lda, s, weight.data_ptr(), ldb, ws, b, m, n, k, _TYPES[out_dtype], out.data_ptr(), n, wp, size))
+    return out
+
+
+def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias: Optional[torch.Tensor] = None, norm=None,
+                out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """A linear layer in 8-bit integers: int8_matmul(*quantize_rows(x, norm), weight, weight_scale, bias), in x's type unless out_dtype says otherwise."""
+    q, scale = quantize_rows(x, norm)
+    return int8_matmul(q, scale, weight, weight_scale, bias, out_dtype or x.dtype)
+
+
+def distill_loss(logits: torch.Tensor, index: torch.Tensor, teacher: torch.Tensor, temperature: float = 1.0,
+                 row_weight: Optional[torch.Tensor] = None, grad: bool = True):
+    """(loss, dlogits): for each row w T^2 KL(softmax(teacher / T) || softmax(logits / T)) over the teacher's kept logits, and the gradient of
+    the losses' sum (None with grad=False).
+
+    logits [..., classes] (f32, bf16, f16; dlogits in the same type), index [..., top] int32 or int64 and teacher [..., top] f32 (top <= 1024), row_weight f32 [...]
+    or None (1).  An index outside [0, classes) is padding; a row of weight 0 or without a kept logit has loss and gradient 0 whatever its logits hold."""
+    lib = _lib or _library()
+    rows, cols, ld = _rows(logits, 'logits')
+    if not isinstance(index, torch.Tensor) or not isinstance(teacher, torch.Tensor) or index.shape != teacher.shape or index.shape[:-1] != logits.shape[:-1] \
+            or index.device != logits.device or teacher.device != logits.device:
+        _refuse(f'index, teacher: both {tuple(logits.shape[:-1])} + (top,) on {logits.device} are required')
+    _, top, ldi = _rows(index, 'index', (torch.int64, torch.int32))
+    _, _, ldt = _rows(teacher, 'teacher', (torch.float32,))
+    w = _vector(row_weight, rows, 'row_weight', logits, (torch.float32,))
+    loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=logits.device)
+    dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if grad else None
+    keep, ws, size = _workspace(lib.eg_distill_loss_workspace(rows, cols), logits)
+    device, stream = _stream(logits)
+    _check(lib.eg_distill_loss(device, stream, _TYPES[logits.dtype], logits.data_ptr(), ld, index.element_size(), index.data_ptr(), ldi, teacher.data_ptr(), ldt,
+                               w, rows, cols, top, temperature, loss.data_ptr(), dlogits.data_ptr() if grad else None, cols, ws, size))
+    return loss, dlogits

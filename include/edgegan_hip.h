@@ -209,6 +209,49 @@ int eg_net_forward(eg_ctx* ctx, const char* net, const float* input, int nb, int
  *      tf.train.Saver writes (models/edgegan.py:635-639); needs no GPU. -------------------------------- */
 unsigned int eg_crc32c(unsigned int crc, const void* data, unsigned long long n);
 
+/* ---- operators over rows in device memory (no reference counterpart) -----------------------------------------------------------
+ * For training and inference code beside the engine (edgegan_amd/ops.py binds them to torch tensors).  They need no eg_ctx: every
+ * operand is a pointer into the memory of `device`, the work is enqueued on `stream` (a hipStream_t of that device, NULL: its default
+ * stream) and nothing is allocated, kept or waited for, so that a call can be captured into a HIP graph and calls on several
+ * streams or threads are independent (each with a workspace of its own).  The caller's current device is left as it was.  A matrix is rows x cols with its columns consecutive and its rows `ld`
+ * elements apart; any alignment of the element type works, 16 bytes is fastest.  Outputs may not overlap inputs (y == x, dx == dy
+ * and grad == logits with the same ld are allowed).  Sizes of zero are allowed where a result is defined.  The message of a failed call: eg_last_error(NULL),
+ * on the calling thread. */
+enum { EG_F32 = 0, EG_BF16 = 1, EG_F16 = 2 };                       /* element types */
+enum { EG_ACT_NONE = 0, EG_ACT_RELU = 1, EG_ACT_LRELU = 2 };        /* LeakyReLU's slope is 0.2, as the discriminators' */
+
+/* y = act((x - mean) rstd gamma + beta) for each row; rstd = (var + eps)^-1/2, var biased.  gamma / beta [cols] of type wtype, or
+ * NULL; mean / rstd [rows] (what the gradient needs), or NULL. */
+int eg_layer_norm(int device, void* stream, int dtype, const void* x, long long ldx, int wtype, const void* gamma, const void* beta,
+                  long long rows, long long cols, float eps, int act, void* y, long long ldy, float* mean, float* rstd);
+/* The gradient: dx [rows x cols], dgamma and dbeta [cols] (type wtype); each may be NULL.  beta matters only to an activation's sign.
+ * The workspace (bytes: eg_layer_norm_workspace, -1 for bad sizes) is needed for dgamma / dbeta. */
+long long eg_layer_norm_workspace(long long rows, long long cols);
+int eg_layer_norm_backward(int device, void* stream, int dtype, const void* dy, long long lddy, const void* x, long long ldx,
+                           const float* mean, const float* rstd, int wtype, const void* gamma, const void* beta, long long rows,
+                           long long cols, int act, void* dx, long long lddx, void* dgamma, void* dbeta, void* workspace,
+                           long long workspace_bytes);
+/* Rows in 8 bits: scale = max |x| / 127, q = the whole number nearest to 127 x / max |x| (a tie to the even one); a row of zeros has scale
+ * 0, a row with a NaN or an infinity scale NaN and q = 0.  norm != 0: of the row's layer norm (gamma / beta f32 or NULL) in the same pass.
+ * Each row of q is filled up with zeros to a multiple of 16 bytes where ldq leaves room (the last row's allocation too). */
+int eg_quantize_rows(int device, void* stream, int dtype, const void* x, long long ldx, int norm, const float* gamma, const float* beta,
+                     float eps, long long rows, long long cols, signed char* q, long long ldq, float* scale);
+/* out[i][j] = (sum_k a[i][k] b[j][k]) a_scale[i] b_scale[j] + bias[j]: a [m x k] a scale for each row (token, position), b [n x k] one for
+ * each output channel; 32-bit integer sums (k <= 131071).  bias f32 or NULL. */
+long long eg_int8_matmul_workspace(long long m, long long n, long long k);
+int eg_int8_matmul(int device, void* stream, const signed char* a, long long lda, const float* a_scale, const signed char* b,
+                   long long ldb, const float* b_scale, const float* bias, long long m, long long n, long long k, int out_type,
+                   void* out, long long ldo, void* workspace, long long workspace_bytes);
+/* Distillation from a teacher's top logits: p = softmax(teacher / T) over the `top` (<= 1024) kept logits of a row, q = softmax(logits / T);
+ * loss[r] = w_r T^2 sum_k p_k (log p_k - log q_index[k]); grad (or NULL) = d(sum of loss) / d(logits).  index: 4- or 8-byte integers;
+ * one outside [0, cols) is padding, one given twice counts twice.  row_weight f32 [rows] or NULL (1): a row of weight 0 or without a kept
+ * logit has loss 0 and gradient 0 whatever its logits hold. */
+long long eg_distill_loss_workspace(long long rows, long long cols);
+int eg_distill_loss(int device, void* stream, int dtype, const void* logits, long long ld, int index_bytes, const void* index,
+                    long long ld_index, const float* teacher, long long ld_teacher, const float* row_weight, long long rows,
+                    long long cols, long long top, float temperature, float* loss, void* grad, long long ldg, void* workspace,
+                    long long workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,84 @@
+"""The row operators' C entries on the host: every refusal is an error code and a message, before any device is touched."""
+import ctypes as C
+import os
+import subprocess
+import sys
+
+import numpy as np
+import pytest
+
+from edgegan_amd import _lib
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+P = 1 << 20      # an address that is never read
+
+
+def norm(lib, device=0, dtype=0, x=P, ldx=8, wtype=0, rows=2, cols=8, eps=1e-5, act=0, y=P, ldy=8, mean=None, rstd=None):
+    return lib.eg_layer_norm(device, None, dtype, x, ldx, wtype, None, None, rows, cols, eps, act, y, ldy, mean, rstd)
+
+
+def backward(lib, rows=2, cols=8, ws=P, size=1 << 20, mean=P, dgamma=P, x=P, lddx=8):
+    return lib.eg_layer_norm_backward(0, None, 0, P, 8, x, 8, mean, P, 0, P, P, rows, cols, 0, P, lddx, dgamma, P, ws, size)
+
+
+def quantize(lib, rows=2, cols=8, q=P, ldq=16, scale=P, norm=0, gamma=None, eps=1e-5):
+    return lib.eg_quantize_rows(0, None, 0, P, 8, norm, gamma, None, eps, rows, cols, q, ldq, scale)
+
+
+def product(lib, a=P, lda=64, sa=P, m=4, n=4, k=64, out_type=0, ldo=4):
+    return lib.eg_int8_matmul(0, None, a, lda, sa, P, 64, P, None, m, n, k, out_type, P, ldo, None, 0)
+
+
+def distill(lib, rows=2, cols=8, top=3, t=1.0, loss=P, index_bytes=8, index=P, ldi=3, ldg=8):
+    return lib.eg_distill_loss(0, None, 0, P, 8, index_bytes, index, ldi, P, 3, None, rows, cols, top, t, loss, P, ldg, P, 1 << 20)
+
+
+CASES = [
+    (norm, dict(dtype=3), 'type'), (norm, dict(wtype=-1), 'type'), (norm, dict(x=None), 'null'), (norm, dict(y=None), 'null'), (norm, dict(ldx=7), 'elements apart'),
+    (norm, dict(ldy=-8), 'elements apart'), (norm, dict(rows=-1), 'rows'), (norm, dict(cols=(1 << 24) + 1), 'columns'), (norm, dict(cols=0), 'without columns'),
+    (norm, dict(eps=0.0), 'eps'), (norm, dict(eps=float('inf')), 'eps'), (norm, dict(act=3), 'activation'), (norm, dict(mean=P), 'together'), (norm, dict(x=P + 2), 'misaligned'),
+    (norm, dict(ldx=1 << 62), 'too large'),
+    (backward, dict(ws=None), 'workspace'), (backward, dict(size=4), 'workspace'), (backward, dict(ws=P + 4), 'workspace'), (backward, dict(mean=None), 'statistics'),
+    (backward, dict(x=None), 'null'), (backward, dict(lddx=3), 'elements apart'), (backward, dict(cols=0), 'without columns'),
+    (quantize, dict(q=None), 'null'), (quantize, dict(ldq=7), 'elements apart'), (quantize, dict(scale=None), 'scale'), (quantize, dict(gamma=P), 'norm'),
+    (quantize, dict(norm=1, eps=-1.0), 'eps'), (quantize, dict(cols=0), 'without columns'),
+    (product, dict(k=131072, lda=131072), 'overflow'), (product, dict(m=-1), 'sizes'), (product, dict(n=1 << 30), 'sizes'), (product, dict(a=None), 'null'), (product, dict(lda=63), 'elements apart'),
+    (product, dict(sa=None), 'scale'), (product, dict(out_type=7), 'type'), (product, dict(ldo=3), 'elements apart'),
+    (distill, dict(top=1025, ldi=1025), 'teacher logits'), (distill, dict(t=0.0), 'temperature'), (distill, dict(t=float('nan')), 'temperature'), (distill, dict(t=1e-45), 'temperature'),
+    (distill, dict(loss=None), 'loss'), (distill, dict(index_bytes=2), 'bytes'), (distill, dict(index=P + 4), 'misaligned'), (distill, dict(ldi=2), 'elements apart'), (distill, dict(ldg=7), 'elements apart'),
+    (distill, dict(cols=0), 'without columns'),
+]
+
+
+@pytest.mark.parametrize('call,args,message', CASES, ids=[f'{c.__name__}-{next(iter(a))}-{i}' for i, (c, a, _) in enumerate(CASES)])
+def test_refusals(built_lib, call, args, message):
+    assert call(built_lib, **args) == 1
+    assert message in built_lib.eg_last_error(None).decode()
+
+
+def test_nothing_to_do_is_no_error(built_lib):
+    """Zero rows: no device is asked for."""
+    assert norm(built_lib, rows=0, x=None, y=None) == 0
+    assert quantize(built_lib, rows=0) == 0
+    assert product(built_lib, m=0, a=None) == 0
+    assert distill(built_lib, rows=0) == 0
+
+
+def test_workspace_sizes(built_lib):
+    assert built_lib.eg_layer_norm_workspace(-1, 8) == -1 and built_lib.eg_layer_norm_workspace(8, (1 << 24) + 1) == -1
+    assert built_lib.eg_layer_norm_workspace(0, 8) == 0
+    assert built_lib.eg_int8_matmul_workspace(1, 1, 131072) == -1 and built_lib.eg_int8_matmul_workspace(1, 4096, 4096) >= 0
+    assert built_lib.eg_distill_loss_workspace(1, -1) == -1 and built_lib.eg_distill_loss_workspace(4, 1000) >= 0
+
+
+def test_two_runtimes_are_refused(built_lib):
+    """The engine loaded before torch runs on another HIP runtime: the operators say so instead of mixing the two."""
+    code = ('import sys; sys.path.insert(0, %r)\n'
+            'from edgegan_amd import _lib\n'
+            '_lib.load_library()\n'
+            'from edgegan_amd import ops\n'
+            'runtimes = {l.split()[-1] for l in open("/proc/self/maps") if "libamdhip64" in l}\n'
+            'try:\n    ops._library()\n    print("taken", len(runtimes))\n'
+            'except _lib.EdgeGANLibError as e:\n    print("refused", len(runtimes))\n' % ROOT)
+    out = subprocess.run([sys.executable, '-c', code], capture_output=True, text=True, timeout=300).stdout.split()
+    assert out in (['refused', '2'], ['taken', '1']), out
