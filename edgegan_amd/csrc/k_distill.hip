@@ -35,7 +35,7 @@ __global__ __launch_bounds__(kDistillThreads) void distill_rows(DistillArgs a) {
       p[k] = idx[k] >= 0 ? a.teacher[r * a.ld_teacher + k] * it : -INFINITY;
       m = (p[k] > m || p[k] != p[k]) ? p[k] : m;
     }
-    m = block_max<kDistillThreads>(m, red);
+    m = team_max<kDistillThreads>(m, red);
     __syncthreads();
     if (w == 0.f || m == -INFINITY) {
       if (g && !a.acc)
@@ -45,7 +45,7 @@ __global__ __launch_bounds__(kDistillThreads) void distill_rows(DistillArgs a) {
     }
     float s[1] = {0.f};
     for (int k = tid; k < a.top; k += kDistillThreads) s[0] += expf(p[k] - m);
-    block_sum<kDistillThreads>(s, red);
+    team_sum<kDistillThreads>(s, red);
     const float lse_t = m + logf(s[0]);
     __syncthreads();
     // the student
@@ -54,11 +54,11 @@ __global__ __launch_bounds__(kDistillThreads) void distill_rows(DistillArgs a) {
       const float v = (float)z[c] * it;
       zm = (v > zm || v != v) ? v : zm;
     }
-    zm = block_max<kDistillThreads>(zm, red);
+    zm = team_max<kDistillThreads>(zm, red);
     __syncthreads();
     float e[1] = {0.f};
     for (int c = tid; c < a.cols; c += kDistillThreads) e[0] += expf((float)z[c] * it - zm);
-    block_sum<kDistillThreads>(e, red);
+    team_sum<kDistillThreads>(e, red);
     const float lse = zm + logf(e[0]);
     __syncthreads();
     // the loss; p becomes a probability
@@ -68,7 +68,7 @@ __global__ __launch_bounds__(kDistillThreads) void distill_rows(DistillArgs a) {
       if (idx[k] >= 0 && pk != 0.f) l[0] += pk * (lp - ((float)z[idx[k]] * it - lse));
       p[k] = pk;
     }
-    block_sum<kDistillThreads>(l, red);
+    team_sum<kDistillThreads>(l, red);
     if (tid == 0) a.loss[r] = w * a.temperature * a.temperature * l[0];
     if (g) {
       // the kept indexes first, from the old gradient where it is added to; then every other column by its own thread

@@ -1,12 +1,15 @@
 // Layer norm over rows: forward, gradient, tangent and its reverse; the row quantisation to 8 bits, with or without a layer
-// norm in front.  Bound by HBM: every pass below reads each row once from memory (further passes over a row hit the caches).
+// norm in front.
 //
 //   xh = (x - m) r,  m = mean x,  r = (mean (x - m)^2 + eps)^-1/2,  y = act(xh gamma + beta)
 //   gradient:  g = dy act'(xh gamma + beta),  dx = r (g gamma - mean(g gamma) - xh mean(g gamma xh)),
 //              dgamma = sum over rows of g xh,  dbeta = sum over rows of g
 //   quantised: q = the whole number nearest to 127 x / max |x| (a tie to the even one), scale = max |x| / 127
 //
-// Sums are in 32 bits.  xh gamma + beta is formed by the same three rounded operations in the forward and the gradient (no
+// All of it is bound by HBM, so a row is read once: it stays in the registers of the team of threads that owns it (8 to 64 lanes of a
+// wave, 256 or 1,024 threads: row_team) between the statistics and the result.  A team of a wave needs no LDS and no barrier; a wider one joins its
+// waves' sums through LDS.  The mean is summed in 64 bits (it decides every x - m, and rows of one value then have xh = 0 exactly), the
+// squares and the gradient's sums in 32.  xh gamma + beta is formed by the same three rounded operations in the forward and the gradient (no
 // contraction into an fma), so the gradient's sign of it is the forward's.
 #include <tuple>
 
@@ -14,62 +17,314 @@
 
 namespace eg {
 
-template <typename T>
-__device__ __forceinline__ float ld1(const T* p) { return (float)*p; }
-
 template <typename W>
 __device__ __forceinline__ float affine(float xh, const W* gamma, const W* beta, int c) {
   const float z = gamma ? __fmul_rn(xh, (float)gamma[c]) : xh;
   return beta ? __fadd_rn(z, (float)beta[c]) : z;
 }
+__device__ __forceinline__ float affine_r(float xh, float gamma, float beta) { return __fadd_rn(__fmul_rn(xh, gamma), beta); }
 
-// mean and 1 / sqrt(var + eps) of a row, by the whole block
-template <typename T, int NT>
-__device__ __forceinline__ void row_statistics(const T* x, int cols, float eps, float* red, float& mean, float& rstd) {
-  float s[1] = {0.f};
-  for (int c = threadIdx.x; c < cols; c += NT) s[0] += ld1(x + c);
-  block_sum<NT>(s, red);
-  const float m0 = s[0] / cols;
-  __syncthreads();
-  // the second pass also sums x - m0: what the first sum lost by rounding
-  float d[2] = {0.f, 0.f};
-  for (int c = threadIdx.x; c < cols; c += NT) {
-    const float u = ld1(x + c) - m0;
-    d[0] += u;
-    d[1] += u * u;
+// ---- rows in registers -------------------------------------------------------------------------------------------------------
+// NT threads own a row, each NV packs of V consecutive elements: pack i of thread t begins at column (i NT + t) V.
+template <typename T, int NT, int NV, int V>
+__device__ __forceinline__ void load_row(const T* p, int cols, int t, float (&v)[NV][V]) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * NT + t) * V;
+    load_pack<T, V>(p + (c < cols ? c : 0), v[i]);   // (no branch, so that all of a thread's loads are in flight at once)
+    if (c >= cols)
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[i][j] = 0.f;
   }
-  block_sum<NT>(d, red);
-  const float e = d[0] / cols;
-  mean = m0 + e;
-  rstd = 1.f / sqrtf(fmaxf(d[1] / cols - e * e, 0.f) + eps);
-  if (d[1] != d[1]) rstd = d[1];   // (fmaxf drops a NaN)
-  __syncthreads();
 }
+template <typename W, int NT, int NV, int V>
+__device__ __forceinline__ void load_parameter(const W* p, int cols, int t, float missing, float (&v)[NV][V]) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int at = (i * NT + t) * V, c = at < cols ? at : 0;
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[i][j] = missing;
+    if (p) {
+      if constexpr (V * sizeof(W) <= 16) load_pack<W, V>(p + c, v[i]);
+      else {   // (16-bit rows with 32-bit parameters: two loads)
+        float lo[V / 2], hi[V / 2];
+        load_pack<W, V / 2>(p + c, lo);
+        load_pack<W, V / 2>(p + c + V / 2, hi);
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) v[i][j] = lo[j], v[i][j + V / 2] = hi[j];
+      }
+    }
+  }
+}
+template <typename T, int NT, int NV, int V>
+__device__ __forceinline__ void store_row(T* p, int cols, int t, const float (&v)[NV][V]) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * NT + t) * V;
+    if (c < cols) store_pack<T, V>(p + c, v[i]);
+  }
+}
+// mean (f64 sum) and rstd of a row in registers; the row becomes x - mean
+template <int NT, int NV, int V>
+__device__ __forceinline__ void centre_row(float (&v)[NV][V], int cols, int t, float eps, double* red, float& mean, float& rstd) {
+  double s[1] = {0.};
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) s[0] += (double)v[i][j];
+  team_sum<NT>(s, red);
+  mean = (float)(s[0] / cols);
+  float d[1] = {0.f};
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      v[i][j] = (i * NT + t) * V < cols ? v[i][j] - mean : 0.f;
+      d[0] += v[i][j] * v[i][j];
+    }
+  team_sum<NT>(d, reinterpret_cast<float*>(red + NT / 64));
+  rstd = 1.f / sqrtf(d[0] / cols + eps);
+}
+constexpr int centre_lds(int nt) { return nt > 64 ? 2 * nt / 64 : 1; }   // doubles
 
-constexpr int kRowThreads = 256;
-
-template <typename T, typename W>
-__global__ __launch_bounds__(kRowThreads) void ln_fwd_rows(LayerNormArgs a) {
-  __shared__ float red[2 * kRowThreads / 64];
-  for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
-    const T* x = (const T*)a.x + r * a.ldx;
-    T* y = (T*)a.y + r * a.ldy;
-    float mean, rstd;
-    row_statistics<T, kRowThreads>(x, a.cols, a.eps, red, mean, rstd);
-    for (int c = threadIdx.x; c < a.cols; c += kRowThreads)
-      y[c] = (T)row_act(affine(__fmul_rn(ld1(x + c) - mean, rstd), (const W*)a.gamma, (const W*)a.beta, c), a.act);
-    if (threadIdx.x == 0 && a.mean) {
+template <typename T, typename W, int NT, int NV, int V>
+__global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_fwd(LayerNormArgs a) {
+  constexpr int NB = NT > 256 ? NT : 256, TEAMS = NB / NT;
+  __shared__ double red[2][centre_lds(NT)];
+  const int t = threadIdx.x % NT, team = threadIdx.x / NT;
+  float g[NV][V], b[NV][V];
+  load_parameter<W, NT, NV, V>((const W*)a.gamma, a.cols, t, 1.f, g);
+  load_parameter<W, NT, NV, V>((const W*)a.beta, a.cols, t, 0.f, b);
+  int turn = 0;
+  for (long long r = (long long)blockIdx.x * TEAMS + team; r < a.rows; r += (long long)gridDim.x * TEAMS, turn ^= 1) {
+    float v[NV][V], mean, rstd;
+    load_row<T, NT, NV, V>((const T*)a.x + r * a.ldx, a.cols, t, v);
+    centre_row<NT, NV, V>(v, a.cols, t, a.eps, red[turn], mean, rstd);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[i][j] = row_act(affine_r(__fmul_rn(v[i][j], rstd), g[i][j], b[i][j]), a.act);
+    store_row<T, NT, NV, V>((T*)a.y + r * a.ldy, a.cols, t, v);
+    if (t == 0 && a.mean) {
       a.mean[r] = mean;
       a.rstd[r] = rstd;
     }
   }
 }
 
+template <typename T, typename W, int NT, int NV, int V>
+__global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_bwd(LayerNormGradArgs a) {
+  constexpr int NB = NT > 256 ? NT : 256, TEAMS = NB / NT;
+  __shared__ float red[2][NT > 64 ? 2 * NT / 64 : 1];
+  const int t = threadIdx.x % NT, team = threadIdx.x / NT;
+  float g[NV][V], sx[NV][V], sg[NV][V];
+  load_parameter<W, NT, NV, V>((const W*)a.gamma, a.cols, t, 1.f, g);
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) sx[i][j] = sg[i][j] = 0.f;
+  const float n = 1.f / a.cols;
+  int turn = 0;
+  for (long long r = (long long)blockIdx.x * TEAMS + team; r < a.rows; r += (long long)gridDim.x * TEAMS, turn ^= 1) {
+    float x[NV][V], d[NV][V];
+    load_row<T, NT, NV, V>((const T*)a.x + r * a.ldx, a.cols, t, x);
+    load_row<T, NT, NV, V>((const T*)a.dy + r * a.lddy, a.cols, t, d);
+    const float mean = a.mean[r], rstd = a.rstd[r];
+    if (a.act != ACT_NONE) {
+      float b[NV][V];
+      load_parameter<W, NT, NV, V>((const W*)a.beta, a.cols, t, 0.f, b);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) d[i][j] *= row_act_grad(affine_r(__fmul_rn(x[i][j] - mean, rstd), g[i][j], b[i][j]), a.act);
+    }
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {   // (columns past the last have d = 0 and reach no sum)
+        x[i][j] = __fmul_rn(x[i][j] - mean, rstd);
+        sg[i][j] += d[i][j];
+        sx[i][j] += d[i][j] * x[i][j];
+        d[i][j] *= g[i][j];
+        s[0] += d[i][j];
+        s[1] += d[i][j] * x[i][j];
+      }
+    if (!a.dx) continue;
+    team_sum<NT>(s, red[turn]);
+    const float m0 = s[0] * n, m1 = s[1] * n;
+    T* dx = (T*)a.dx + r * a.lddx;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) d[i][j] = (d[i][j] - m0 - x[i][j] * m1) * rstd;
+    if (a.acc_x) {
+      load_row<T, NT, NV, V>(dx, a.cols, t, x);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) d[i][j] += x[i][j];
+    }
+    store_row<T, NT, NV, V>(dx, a.cols, t, d);
+  }
+  if (!a.partial) return;
+  float* out = a.partial + (size_t)blockIdx.x * 2 * a.cols;
+  if constexpr (TEAMS > 1) {   // the block's teams add up in their order
+    __shared__ float sum[2][NT * NV * V];
+    for (int k = 0; k < TEAMS; ++k) {
+      if (team == k)
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const int c = (i * NT + t) * V + j;
+            sum[0][c] = (k ? sum[0][c] : 0.f) + sx[i][j];
+            sum[1][c] = (k ? sum[1][c] : 0.f) + sg[i][j];
+          }
+      __syncthreads();
+    }
+    for (int c = threadIdx.x; c < a.cols; c += NB) {
+      out[c] = sum[0][c];
+      out[a.cols + c] = sum[1][c];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * NT + t) * V;
+      if (c < a.cols)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          out[c + j] = sx[i][j];
+          out[a.cols + c + j] = sg[i][j];
+        }
+    }
+  }
+}
+
+// partial [groups][2][cols] -> dgamma, dbeta: a block adds 64 of the 2 cols sums, 16 threads each every 16th group
+template <typename W>
+__global__ __launch_bounds__(1024) void ln_bwd_finish(const float* partial, int groups, int cols, W* dgamma, W* dbeta, int acc) {
+  __shared__ float red[16][64];
+  const int lane = threadIdx.x & 63, part = threadIdx.x >> 6;
+  const int i = blockIdx.x * 64 + lane;
+  float s = 0.f;
+  if (i < 2 * cols) {
+    const float* p = partial + i;
+#pragma unroll 8
+    for (int g = part; g < groups; g += 16) s += p[(size_t)g * 2 * cols];
+  }
+  red[part][lane] = s;
+  __syncthreads();
+  if (part || i >= 2 * cols) return;
+  W* out = i < cols ? dgamma : dbeta;
+  if (!out) return;
+  out += i < cols ? i : i - cols;
+  s = acc ? (float)*out : 0.f;
+#pragma unroll
+  for (int k = 0; k < 16; ++k) s += red[k][lane];
+  *out = (W)s;
+}
+
+// The whole number nearest to 127 v / amax, exactly: inv = 127 / amax in 64 bits; v inv + 98304 is rounded once (fma) to a multiple of
+// 2^-36, where a true tie lands on the tie (the product is off by under 2^-45) and nothing else does (127 v / amax is at least 2^-33 from a
+// border that it is not on: with x's last bit u >= 2^-32 amax, 254 v - odd amax is a multiple of u).  Adding 1.5 2^52 then rounds to whole numbers, ties to even, and the
+// sum's low byte is the signed 8-bit result (98304 = 0x18000).
+__device__ __forceinline__ unsigned quantize1(float v, double inv) {
+  const double t = __builtin_fma((double)v, inv, 98304.0) + 6755399441055744.0;
+  return (unsigned)__double2loint(t) & 0xffu;
+}
+// false for infinity and NaN: such a row's scale is NaN, its values zero
+__device__ __forceinline__ bool quantizable(float amax) { return amax <= 3.4028235e38f; }
+__device__ __forceinline__ double quantize_factor(float amax) { return quantizable(amax) && amax > 0.f ? 127.0 / (double)amax : 0.0; }
+__device__ __forceinline__ float quantize_scale(float amax) { return quantizable(amax) ? amax / 127.f : __builtin_nanf(""); }
+
+template <typename T, int NT, int NV, int V>
+__global__ __launch_bounds__(NT > 256 ? NT : 256) void quantize_rows(QuantizeArgs a) {
+  constexpr int NB = NT > 256 ? NT : 256, TEAMS = NB / NT;
+  __shared__ double red[2][centre_lds(NT)];
+  __shared__ float red_max[2][NT > 64 ? NT / 64 : 1];
+  const int t = threadIdx.x % NT, team = threadIdx.x / NT;
+  const int width = (int)min((long long)((a.cols + 15) & ~15), a.ldq);   // the row's last 16-byte group is filled up with zeros
+  int turn = 0;
+  for (long long r = (long long)blockIdx.x * TEAMS + team; r < a.rows; r += (long long)gridDim.x * TEAMS, turn ^= 1) {
+    float v[NV][V];
+    load_row<T, NT, NV, V>((const T*)a.x + r * a.ldx, a.cols, t, v);
+    if (a.norm) {
+      float mean, rstd, p[NV][V];
+      centre_row<NT, NV, V>(v, a.cols, t, a.eps, red[turn], mean, rstd);
+      load_parameter<float, NT, NV, V>(a.gamma, a.cols, t, 1.f, p);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[i][j] = __fmul_rn(__fmul_rn(v[i][j], rstd), p[i][j]);
+      load_parameter<float, NT, NV, V>(a.beta, a.cols, t, 0.f, p);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[i][j] = __fadd_rn(v[i][j], p[i][j]);
+    }
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) m = max_nan(m, (i * NT + t) * V < a.cols ? fabsf(v[i][j]) : 0.f);
+    m = team_max<NT>(m, red_max[turn]);
+    const double inv = quantize_factor(m);
+    const bool fine = quantizable(m);
+    unsigned char* q = (unsigned char*)a.q + r * a.ldq;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * NT + t) * V;
+      if (c >= width) continue;
+      Pack<unsigned char, V> k;
+#pragma unroll
+      for (int j = 0; j < V; ++j) k.e[j] = (unsigned char)(fine && c < a.cols ? quantize1(v[i][j], inv) : 0u);
+      *reinterpret_cast<Pack<unsigned char, V>*>(q + c) = k;
+    }
+    if (t == 0) a.scale[r] = quantize_scale(m);
+  }
+}
+
+// ---- rows of any length: three passes by 256 threads, element by element -------------------------------------------------------
+constexpr int kRowThreads = 256;
+template <typename T>
+__device__ __forceinline__ void row_statistics(const T* x, int cols, float eps, double* red, float& mean, float& rstd) {
+  double s[1] = {0.};
+  for (int c = threadIdx.x; c < cols; c += kRowThreads) s[0] += (double)(float)x[c];
+  team_sum<kRowThreads>(s, red);
+  mean = (float)(s[0] / cols);
+  float d[1] = {0.f};
+  for (int c = threadIdx.x; c < cols; c += kRowThreads) {
+    const float u = (float)x[c] - mean;
+    d[0] += u * u;
+  }
+  team_sum<kRowThreads>(d, reinterpret_cast<float*>(red + kRowThreads / 64));
+  rstd = 1.f / sqrtf(d[0] / cols + eps);
+}
+
+template <typename T, typename W>
+__global__ __launch_bounds__(kRowThreads) void ln_fwd_rows(LayerNormArgs a) {
+  __shared__ double red[2 * kRowThreads / 64];
+  for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    const T* x = (const T*)a.x + r * a.ldx;
+    T* y = (T*)a.y + r * a.ldy;
+    float mean, rstd;
+    row_statistics<T>(x, a.cols, a.eps, red, mean, rstd);
+    for (int c = threadIdx.x; c < a.cols; c += kRowThreads)
+      y[c] = (T)row_act(affine(__fmul_rn((float)x[c] - mean, rstd), (const W*)a.gamma, (const W*)a.beta, c), a.act);
+    if (threadIdx.x == 0 && a.mean) {
+      a.mean[r] = mean;
+      a.rstd[r] = rstd;
+    }
+    __syncthreads();
+  }
+}
+
 // g = dy act'(z) and xh of one element
 template <typename T, typename W>
 __device__ __forceinline__ void grad_terms(const LayerNormGradArgs& a, const T* x, const T* dy, float mean, float rstd, int c, float& g, float& xh) {
-  xh = __fmul_rn(ld1(x + c) - mean, rstd);
-  g = ld1(dy + c);
+  xh = __fmul_rn((float)x[c] - mean, rstd);
+  g = (float)dy[c];
   if (a.act != ACT_NONE) g *= row_act_grad(affine(xh, (const W*)a.gamma, (const W*)a.beta, c), a.act);
 }
 
@@ -88,7 +343,7 @@ __global__ __launch_bounds__(kRowThreads) void ln_bwd_rows(LayerNormGradArgs a) 
       s[0] += g;
       s[1] += g * xh;
     }
-    block_sum<kRowThreads>(s, red);
+    team_sum<kRowThreads>(s, red);
     const float m0 = s[0] / a.cols, m1 = s[1] / a.cols;
     for (int c = threadIdx.x; c < a.cols; c += kRowThreads) {
       float g, xh;
@@ -123,45 +378,87 @@ __global__ __launch_bounds__(256) void ln_bwd_columns(LayerNormGradArgs a) {
   if (part < 2 && c < a.cols)
     a.partial[((size_t)blockIdx.y * 2 + part) * a.cols + c] = red[part][0][lane] + red[part][1][lane] + red[part][2][lane] + red[part][3][lane];
 }
-// partial [groups][2][cols] -> dgamma, dbeta
-template <typename W>
-__global__ __launch_bounds__(256) void ln_bwd_finish(const float* partial, int groups, int cols, W* dgamma, W* dbeta, int acc) {
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= 2 * cols) return;
-  const int which = i / cols, c = i - which * cols;
-  W* out = which ? dbeta : dgamma;
-  if (!out) return;
-  float s = 0.f;
-  for (int p = 0; p < groups; ++p) s += partial[((size_t)p * 2 + which) * cols + c];
-  if (acc) s += (float)out[c];
-  out[c] = (W)s;
-}
-
 static dim3 row_grid(long long rows) { return dim3((unsigned)std::min<long long>(rows, 1 << 20)); }
 static int part_groups(long long rows) { return (int)std::min<long long>(kPartBlocks, (rows + 3) / 4); }
 
-size_t layer_norm_partial_floats(long long rows, int cols) { return (size_t)part_groups(rows) * 2 * cols; }
+// Calls f(threads of a row, packs of a thread, elements of a pack) for the smallest team whose registers hold a row of `cols`; false: none does.
+// Packs of 16 bytes where every row begins at a multiple of 16 bytes and ends with a whole pack, else single elements.  A thread keeps at most MOST elements.
+template <int MOST, int V, typename F>
+static bool row_team(int cols, F f) {
+#define EG_TEAM(NT, NV) \
+  if constexpr ((NV) * V <= MOST) \
+    if (cols <= (NT) * (NV) * V) return f(std::integral_constant<int, NT>{}, std::integral_constant<int, NV>{}, std::integral_constant<int, V>{}), true;
+  if constexpr (V > 1) {
+    EG_TEAM(8, 1) EG_TEAM(16, 1) EG_TEAM(32, 1) EG_TEAM(64, 1) EG_TEAM(64, 2) EG_TEAM(64, 4) EG_TEAM(256, 2) EG_TEAM(256, 4) EG_TEAM(1024, 2) EG_TEAM(1024, 4)
+  } else {
+    EG_TEAM(32, 1) EG_TEAM(64, 4) EG_TEAM(64, 16) EG_TEAM(256, 8) EG_TEAM(256, 16) EG_TEAM(256, 32) EG_TEAM(1024, 16) EG_TEAM(1024, 32)
+  }
+#undef EG_TEAM
+  return false;
+}
+static bool aligned16(const void* p, long long ld, int elem) { return (uintptr_t)p % 16 == 0 && ld * elem % 16 == 0; }
+template <typename T, int MOST, typename F>
+static bool row_team(bool packs, int cols, F f) {
+  constexpr int V = 16 / sizeof(T);
+  return packs && cols % V == 0 ? row_team<MOST, V>(cols, f) : row_team<MOST, 1>(cols, f);
+}
+static dim3 team_grid(long long rows, int nt, int most) {
+  const int teams = nt > 256 ? 1 : 256 / nt;
+  return dim3((unsigned)std::min<long long>((rows + teams - 1) / teams, most));
+}
+static dim3 team_block(int nt) { return dim3(nt > 256 ? nt : 256); }
+
+constexpr int kGradBlocks = 512;   // blocks of the gradient: each leaves one row of partial parameter gradients
+size_t layer_norm_partial_floats(long long rows, int cols) { return (size_t)std::min<long long>(kGradBlocks, rows) * 2 * cols; }
 
 void launch_layer_norm(const LayerNormArgs& a, int type, int wtype, hipStream_t s) {
   if (a.rows == 0 || a.cols == 0) return;
   by_type(type, [&](auto t) {
-    by_type(wtype, [&](auto w) { row_launch(ln_fwd_rows<decltype(t), decltype(w)>, row_grid(a.rows), dim3(kRowThreads), s, a); });
+    using T = decltype(t);
+    auto go = [&](auto w) {
+      using W = decltype(w);
+      const bool packs = aligned16(a.x, a.ldx, sizeof(T)) && aligned16(a.y, a.ldy, sizeof(T)) && (uintptr_t)a.gamma % 16 == 0 && (uintptr_t)a.beta % 16 == 0;
+      if (!row_team<T, 32>(packs, a.cols, [&](auto nt, auto nv, auto v) {
+            row_launch(ln_fwd<T, W, nt, nv, v>, team_grid(a.rows, nt, 8192), team_block(nt), s, a);
+          }))
+        row_launch(ln_fwd_rows<T, W>, row_grid(a.rows), dim3(kRowThreads), s, a);
+    };
+    if (wtype == type) go(t);
+    else go(float{});
   });
 }
 
-void launch_layer_norm_backward(const LayerNormGradArgs& a, int type, int wtype, hipStream_t s) {
+void launch_layer_norm_backward(const LayerNormGradArgs& given, int type, int wtype, hipStream_t s) {
+  LayerNormGradArgs a = given;
   if (a.cols == 0) return;
+  const bool params = a.dgamma || a.dbeta;
+  if (!params) a.partial = nullptr;
   by_type(type, [&](auto t) {
-    by_type(wtype, [&](auto w) {
-      using T = decltype(t);
+    using T = decltype(t);
+    auto go = [&](auto w) {
       using W = decltype(w);
-      auto rows = [&] { if (a.dx && a.rows) row_launch(ln_bwd_rows<T, W>, row_grid(a.rows), dim3(kRowThreads), s, a); };
-      if (!a.dgamma && !a.dbeta) return rows();
-      const int groups = part_groups(a.rows);
-      if (groups) row_launch(ln_bwd_columns<T, W>, dim3((a.cols + 63) / 64, groups), dim3(256), s, a);
-      row_launch(ln_bwd_finish<W>, dim3((2 * a.cols + 255) / 256), dim3(256), s, a.partial, groups, a.cols, (W*)a.dgamma, (W*)a.dbeta, a.acc_w);
-      rows();   // (last: dx may be dy)
-    });
+      const bool packs = aligned16(a.x, a.ldx, sizeof(T)) && aligned16(a.dy, a.lddy, sizeof(T)) && aligned16(a.dx, a.lddx, sizeof(T)) &&
+                         (uintptr_t)a.gamma % 16 == 0 && (uintptr_t)a.beta % 16 == 0;
+      int groups = 0;
+      if (a.rows) {
+        const bool held = row_team<T, 16>(packs, a.cols, [&](auto nt, auto nv, auto v) {
+          const dim3 grid = team_grid(a.rows, nt, kGradBlocks);
+          groups = (int)grid.x;
+          row_launch(ln_bwd<T, W, nt, nv, v>, grid, team_block(nt), s, a);
+        });
+        if (!held) {
+          if (params) {   // (first: dx may be dy)
+            groups = part_groups(a.rows);
+            row_launch(ln_bwd_columns<T, W>, dim3((a.cols + 63) / 64, groups), dim3(256), s, a);
+          }
+          if (a.dx) row_launch(ln_bwd_rows<T, W>, row_grid(a.rows), dim3(kRowThreads), s, a);
+        }
+      }
+      if (params)
+        row_launch(ln_bwd_finish<W>, dim3((2 * a.cols + 63) / 64), dim3(1024), s, a.partial, groups, a.cols, (W*)a.dgamma, (W*)a.dbeta, a.acc_w);
+    };
+    if (wtype == type) go(t);
+    else go(float{});
   });
 }
 
@@ -181,7 +478,7 @@ __global__ __launch_bounds__(kRowThreads) void ln_tangent_rows(LayerNormTangentA
       s[0] += t;
       s[1] += t * __fmul_rn(a.x[o + c] - mean, rstd);
     }
-    block_sum<kRowThreads>(s, red);
+    team_sum<kRowThreads>(s, red);
     const float mt = s[0] / a.cols, b = s[1] / a.cols;
     for (int c = threadIdx.x; c < a.cols; c += kRowThreads) {
       const float xh = __fmul_rn(a.x[o + c] - mean, rstd);
@@ -206,7 +503,7 @@ __global__ __launch_bounds__(kRowThreads) void ln_tangent_bwd_rows(LayerNormTang
       s[3] += k * xh;
       s[4] += k * t;
     }
-    block_sum<kRowThreads>(s, red);
+    team_sum<kRowThreads>(s, red);
     const float n = 1.f / a.cols;
     const float mt = s[0] * n, b = s[1] * n, mk = s[2] * n, w = s[3] * n, q = s[4] * n - mk * mt;
     for (int c = threadIdx.x; c < a.cols; c += kRowThreads) {
@@ -236,7 +533,7 @@ __global__ __launch_bounds__(256) void ln_tangent_bwd_columns(LayerNormTangentAr
       s[0] += t;
       s[1] += t * __fmul_rn(a.x[o + c] - mean, rstd);
     }
-    block_sum<256>(s, red);
+    team_sum<256>(s, red);
     if (tid < 2) means[tid] = s[tid] / a.cols;
     __syncthreads();
     const float mt = means[0], b = means[1];
@@ -260,50 +557,49 @@ void launch_layer_norm_tangent_backward(const LayerNormTangentArgs& a, hipStream
   if (!a.dgamma) return;
   const int groups = part_groups(a.rows);
   row_launch(ln_tangent_bwd_columns, dim3(groups), dim3(256), s, a);
-  row_launch(ln_bwd_finish<float>, dim3((2 * a.cols + 255) / 256), dim3(256), s, a.partial, groups, a.cols, a.dgamma, nullptr, a.acc_w);
+  row_launch(ln_bwd_finish<float>, dim3((2 * a.cols + 63) / 64), dim3(1024), s, a.partial, groups, a.cols, a.dgamma, nullptr, a.acc_w);
 }
 
-// ---- quantisation ----------------------------------------------------------------------------------------------------------
-// The whole number nearest to 127 v / amax, exactly: inv = 127 / amax in 64 bits; v inv + 98304 is rounded once (fma) to a multiple of
-// 2^-36, where a true tie lands on the tie (the product is off by under 2^-45) and nothing else does (127 v / amax is at least 2^-33 from a
-// border that it is not on: with x's last bit u >= 2^-32 amax, 254 v - odd amax is a multiple of u).  Adding 1.5 2^52 then rounds to whole numbers, ties to even, and the
-// sum's low byte is the signed 8-bit result (98304 = 0x18000).
-__device__ __forceinline__ unsigned quantize1(float v, double inv) {
-  const double t = __builtin_fma((double)v, inv, 98304.0) + 6755399441055744.0;
-  return (unsigned)__double2loint(t) & 0xffu;
-}
-
+// ---- quantisation of rows of any length -----------------------------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(kRowThreads) void quantize_kernel(QuantizeArgs a) {
-  __shared__ float red[2 * kRowThreads / 64];
+  __shared__ double red[2 * kRowThreads / 64];
+  __shared__ float red_max[kRowThreads / 64];
   for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const T* x = (const T*)a.x + r * a.ldx;
     unsigned char* q = (unsigned char*)a.q + r * a.ldq;
     float mean = 0.f, rstd = 1.f;
-    if (a.norm) row_statistics<T, kRowThreads>(x, a.cols, a.eps, red, mean, rstd);
+    if (a.norm) row_statistics<T>(x, a.cols, a.eps, red, mean, rstd);
     auto value = [&](int c) {
-      float v = ld1(x + c);
+      float v = (float)x[c];
       if (a.norm) v = affine(__fmul_rn(v - mean, rstd), a.gamma, a.beta, c);
       return v;
     };
     float m = 0.f;
     for (int c = threadIdx.x; c < a.cols; c += kRowThreads) {
       const float v = fabsf(value(c));
-      m = (v > m || v != v) ? v : m;
+      m = max_nan(m, v);
     }
-    m = block_max<kRowThreads>(m, red);
-    const bool fine = m <= 3.4028235e38f;   // false for infinity and NaN: such a row's scale is NaN, its values zero
-    const double inv = fine && m > 0.f ? 127.0 / (double)m : 0.0;
+    m = team_max<kRowThreads>(m, red_max);
+    const bool fine = quantizable(m);
+    const double inv = quantize_factor(m);
     const int width = (int)min((long long)((a.cols + 15) & ~15), a.ldq);   // the row's last 16-byte group is filled up with zeros
     for (int c = threadIdx.x; c < width; c += kRowThreads) q[c] = (unsigned char)(fine && c < a.cols ? quantize1(value(c), inv) : 0u);
-    if (threadIdx.x == 0) a.scale[r] = fine ? m / 127.f : __builtin_nanf("");
+    if (threadIdx.x == 0) a.scale[r] = quantize_scale(m);
     __syncthreads();
   }
 }
 
 void launch_quantize_rows(const QuantizeArgs& a, int type, hipStream_t s) {
   if (!a.rows) return;
-  by_type(type, [&](auto t) { row_launch(quantize_kernel<decltype(t)>, row_grid(a.rows), dim3(kRowThreads), s, a); });
+  by_type(type, [&](auto t) {
+    using T = decltype(t);
+    const bool packs = aligned16(a.x, a.ldx, sizeof(T)) && aligned16(a.q, a.ldq, 1) && (uintptr_t)a.gamma % 16 == 0 && (uintptr_t)a.beta % 16 == 0;
+    if (!row_team<T, 32>(packs, a.cols, [&](auto nt, auto nv, auto v) {
+          row_launch(quantize_rows<T, nt, nv, v>, team_grid(a.rows, nt, 8192), team_block(nt), s, a);
+        }))
+      row_launch(quantize_kernel<T>, row_grid(a.rows), dim3(kRowThreads), s, a);
+  });
 }
 
 }  // namespace eg

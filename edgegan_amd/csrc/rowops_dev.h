@@ -34,39 +34,78 @@ __device__ __forceinline__ float row_act(float z, int act) {
 // derivative of row_act at the pre-activation z
 __device__ __forceinline__ float row_act_grad(float z, int act) { return act == ACT_NONE || z > 0.f ? 1.f : act == ACT_LRELU ? 0.2f : 0.f; }
 
-// Sums over the LANES (a power of two) neighbouring lanes of a wave.  Every lane gets the result.
-template <int LANES>
-__device__ __forceinline__ float lanes_sum(float v) {
-#pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
-}
-template <int LANES>
-__device__ __forceinline__ float lanes_max(float v) {
-#pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) {
-    const float u = __shfl_xor(v, o, 64);
-    v = (u > v || u != u) ? u : v;   // a NaN stays
+// One step of a butterfly over a wave, by data-parallel primitives (a few cycles; a shuffle goes through LDS): (a, b) are the values of the
+// two lanes whose numbers differ in X, the same pair in the same order or the other way round in both.  For X = 4, 8 the mirrored lane stands in, which holds the
+// same value once the smaller steps are done.
+template <int X>
+__device__ __forceinline__ void lane_pair(int v, int& a, int& b) {
+  a = v;
+  if constexpr (X == 1) b = __builtin_amdgcn_mov_dpp(v, 0xB1, 0xF, 0xF, true);         // quad_perm [1,0,3,2]
+  else if constexpr (X == 2) b = __builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, true);    // quad_perm [2,3,0,1]
+  else if constexpr (X == 4) b = __builtin_amdgcn_mov_dpp(v, 0x141, 0xF, 0xF, true);   // row_half_mirror
+  else if constexpr (X == 8) b = __builtin_amdgcn_mov_dpp(v, 0x140, 0xF, 0xF, true);   // row_mirror
+  else if constexpr (X == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false);
+    a = (int)r[0];
+    b = (int)r[1];
+  } else {
+    static_assert(X == 32, "a wave has 64 lanes");
+    const auto r = __builtin_amdgcn_permlane32_swap((unsigned)v, (unsigned)v, false, false);
+    a = (int)r[0];
+    b = (int)r[1];
   }
-  return v;
+}
+template <int X>
+__device__ __forceinline__ void lane_pair(float v, float& a, float& b) {
+  int x, y;
+  lane_pair<X>(__float_as_int(v), x, y);
+  a = __int_as_float(x);
+  b = __int_as_float(y);
+}
+template <int X>
+__device__ __forceinline__ void lane_pair(double v, double& a, double& b) {
+  int h0, h1, l0, l1;
+  lane_pair<X>(__double2hiint(v), h0, h1);
+  lane_pair<X>(__double2loint(v), l0, l1);
+  a = __hiloint2double(h0, l0);
+  b = __hiloint2double(h1, l1);
+}
+__device__ __forceinline__ float max_nan(float a, float b) { return (b > a || b != b) ? b : a; }   // a NaN stays
+// Sum / maximum over LANES (a power of two) neighbouring lanes; every lane gets the result.
+template <int LANES, int X = 1, typename V>
+__device__ __forceinline__ V lanes_sum(V v) {
+  if constexpr (X < LANES) {
+    V a, b;
+    lane_pair<X>(v, a, b);
+    return lanes_sum<LANES, 2 * X>(a + b);
+  } else
+    return v;
+}
+template <int LANES, int X = 1>
+__device__ __forceinline__ float lanes_max(float v) {
+  if constexpr (X < LANES) {
+    float a, b;
+    lane_pair<X>(v, a, b);
+    return lanes_max<LANES, 2 * X>(max_nan(a, b));
+  } else
+    return v;
 }
 
-// Sums of NV values over the block's NT threads (NT a multiple of 64), in one pass through `red`[NV * NT / 64].  The caller may
-// use the same `red` again only behind a barrier of its own.
-template <int NT, int NV>
-__device__ __forceinline__ void block_sum(float (&v)[NV], float* red) {
+// Sum / maximum over the NT threads that share a row: neighbouring lanes, or (NT > 64) the whole block through red[NT / 64].  Calls that follow one
+// another use other memory, or a barrier lies between them.
+template <int NT, typename V, int N>
+__device__ __forceinline__ void team_sum(V (&v)[N], V* red) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) v[i] = lanes_sum<64>(v[i]);
+  for (int i = 0; i < N; ++i) v[i] = lanes_sum<(NT < 64 ? NT : 64)>(v[i]);
   if constexpr (NT > 64) {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     constexpr int NW = NT / 64;
-    if (lane == 0)
+    if ((threadIdx.x & 63) == 0)
 #pragma unroll
-      for (int i = 0; i < NV; ++i) red[i * NW + wave] = v[i];
+      for (int i = 0; i < N; ++i) red[i * NW + (threadIdx.x >> 6)] = v[i];
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      float t = red[i * NW];
+    for (int i = 0; i < N; ++i) {
+      V t = red[i * NW];
 #pragma unroll
       for (int w = 1; w < NW; ++w) t += red[i * NW + w];
       v[i] = t;
@@ -74,21 +113,36 @@ __device__ __forceinline__ void block_sum(float (&v)[NV], float* red) {
   }
 }
 template <int NT>
-__device__ __forceinline__ float block_max(float v, float* red) {
-  v = lanes_max<64>(v);
+__device__ __forceinline__ float team_max(float v, float* red) {
+  v = lanes_max<(NT < 64 ? NT : 64)>(v);
   if constexpr (NT > 64) {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     constexpr int NW = NT / 64;
-    if (lane == 0) red[wave] = v;
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     v = red[0];
 #pragma unroll
-    for (int w = 1; w < NW; ++w) {
-      const float u = red[w];
-      v = (u > v || u != u) ? u : v;
-    }
+    for (int w = 1; w < NW; ++w) v = max_nan(v, red[w]);
   }
   return v;
+}
+
+// V consecutive elements: one aligned load / store of V sizeof(T) bytes
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Pack {
+  T e[V];
+};
+template <typename T, int V>
+__device__ __forceinline__ void load_pack(const T* p, float (&v)[V]) {
+  const Pack<T, V> k = *reinterpret_cast<const Pack<T, V>*>(p);
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = (float)k.e[i];
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_pack(T* p, const float (&v)[V]) {
+  Pack<T, V> k;
+#pragma unroll
+  for (int i = 0; i < V; ++i) k.e[i] = (T)v[i];
+  *reinterpret_cast<Pack<T, V>*>(p) = k;
 }
 
 }  // namespace eg
