@@ -37,6 +37,22 @@ __device__ __forceinline__ void load_row(const T* p, int cols, int t, float (&v)
       for (int j = 0; j < V; ++j) v[i][j] = 0.f;
   }
 }
+// the same in two halves: the loads (kept in the row's own type, to be issued a row ahead) and the conversion
+template <typename T, int NT, int NV, int V>
+__device__ __forceinline__ void request_row(const T* p, int cols, int t, Pack<T, V> (&k)[NV]) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * NT + t) * V;
+    k[i] = *reinterpret_cast<const Pack<T, V>*>(p + (c < cols ? c : 0));
+  }
+}
+template <typename T, int NT, int NV, int V>
+__device__ __forceinline__ void take_row(const Pack<T, V> (&k)[NV], int cols, int t, float (&v)[NV][V]) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[i][j] = (i * NT + t) * V < cols ? (float)k[i].e[j] : 0.f;
+}
 template <typename W, int NT, int NV, int V>
 __device__ __forceinline__ void load_parameter(const W* p, int cols, int t, float missing, float (&v)[NV][V]) {
 #pragma unroll
@@ -96,9 +112,14 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_fwd(LayerNormArgs a) {
   load_parameter<W, NT, NV, V>((const W*)a.gamma, a.cols, t, 1.f, g);
   load_parameter<W, NT, NV, V>((const W*)a.beta, a.cols, t, 0.f, b);
   int turn = 0;
-  for (long long r = (long long)blockIdx.x * TEAMS + team; r < a.rows; r += (long long)gridDim.x * TEAMS, turn ^= 1) {
+  const long long step = (long long)gridDim.x * TEAMS;
+  long long r = (long long)blockIdx.x * TEAMS + team;
+  Pack<T, V> next[NV];
+  if (r < a.rows) request_row<T, NT, NV, V>((const T*)a.x + r * a.ldx, a.cols, t, next);
+  for (; r < a.rows; r += step, turn ^= 1) {
     float v[NV][V], mean, rstd;
-    load_row<T, NT, NV, V>((const T*)a.x + r * a.ldx, a.cols, t, v);
+    take_row<T, NT, NV, V>(next, a.cols, t, v);
+    if (r + step < a.rows) request_row<T, NT, NV, V>((const T*)a.x + (r + step) * a.ldx, a.cols, t, next);
     centre_row<NT, NV, V>(v, a.cols, t, a.eps, red[turn], mean, rstd);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -125,11 +146,23 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_bwd(LayerNormGradArgs 
     for (int j = 0; j < V; ++j) sx[i][j] = sg[i][j] = 0.f;
   const float n = 1.f / a.cols;
   int turn = 0;
-  for (long long r = (long long)blockIdx.x * TEAMS + team; r < a.rows; r += (long long)gridDim.x * TEAMS, turn ^= 1) {
+  const long long step = (long long)gridDim.x * TEAMS;
+  long long r = (long long)blockIdx.x * TEAMS + team;
+  Pack<T, V> next_x[NV], next_d[NV];
+  float next_mean = 0.f, next_rstd = 0.f;
+  auto request = [&](long long row) {
+    request_row<T, NT, NV, V>((const T*)a.x + row * a.ldx, a.cols, t, next_x);
+    request_row<T, NT, NV, V>((const T*)a.dy + row * a.lddy, a.cols, t, next_d);
+    next_mean = a.mean[row];
+    next_rstd = a.rstd[row];
+  };
+  if (r < a.rows) request(r);
+  for (; r < a.rows; r += step, turn ^= 1) {
     float x[NV][V], d[NV][V];
-    load_row<T, NT, NV, V>((const T*)a.x + r * a.ldx, a.cols, t, x);
-    load_row<T, NT, NV, V>((const T*)a.dy + r * a.lddy, a.cols, t, d);
-    const float mean = a.mean[r], rstd = a.rstd[r];
+    take_row<T, NT, NV, V>(next_x, a.cols, t, x);
+    take_row<T, NT, NV, V>(next_d, a.cols, t, d);
+    const float mean = next_mean, rstd = next_rstd;
+    if (r + step < a.rows) request(r + step);   // (in flight while this row is summed and stored)
     if (a.act != ACT_NONE) {
       float b[NV][V];
       load_parameter<W, NT, NV, V>((const W*)a.beta, a.cols, t, 0.f, b);
@@ -201,21 +234,22 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_bwd(LayerNormGradArgs 
   }
 }
 
-// partial [groups][2][cols] -> dgamma, dbeta: a block adds 64 of the 2 cols sums, 16 threads each every 16th group
+// partial [groups][2][cols] -> dgamma, dbeta: a block adds 32 of the 2 cols sums, 32 threads each every 32nd group
 template <typename W>
 __global__ __launch_bounds__(1024) void ln_bwd_finish(const float* partial, int groups, int cols, W* dgamma, W* dbeta, int acc) {
-  __shared__ float red[16][64];
-  const int lane = threadIdx.x & 63, part = threadIdx.x >> 6;
-  const int i = blockIdx.x * 64 + lane;
+  __shared__ float red[16][32];
+  const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
+  const int i = blockIdx.x * 32 + lane;
   float s = 0.f;
   if (i < 2 * cols) {
     const float* p = partial + i;
 #pragma unroll 8
-    for (int g = part; g < groups; g += 16) s += p[(size_t)g * 2 * cols];
+    for (int g = part; g < groups; g += 32) s += p[(size_t)g * 2 * cols];
   }
-  red[part][lane] = s;
+  s = lanes_sum<64, 32>(s);   // the wave's two groups
+  if ((threadIdx.x & 32) == 0) red[threadIdx.x >> 6][lane] = s;
   __syncthreads();
-  if (part || i >= 2 * cols) return;
+  if (threadIdx.x >= 32 || i >= 2 * cols) return;
   W* out = i < cols ? dgamma : dbeta;
   if (!out) return;
   out += i < cols ? i : i - cols;
@@ -408,7 +442,9 @@ static dim3 team_grid(long long rows, int nt, int most) {
 }
 static dim3 team_block(int nt) { return dim3(nt > 256 ? nt : 256); }
 
-constexpr int kGradBlocks = 512;   // blocks of the gradient: each leaves one row of partial parameter gradients
+// Blocks of the gradient: each leaves one row of partial parameter gradients.  With a row ahead in flight, 16,384 x 4,096 bf16 (a row a block): 512
+// blocks 80 + 5 us (gradient + join), 256 83 + 5, 1,024 98 + 7; 65,536 x 128 f32 (8 rows a block): 1,024 blocks 19 + 5 us, 512 22 + 4, 256 31 + 4.
+constexpr int kGradBlocks = 1024;   // half of them where the block is one row's team
 size_t layer_norm_partial_floats(long long rows, int cols) { return (size_t)std::min<long long>(kGradBlocks, rows) * 2 * cols; }
 
 void launch_layer_norm(const LayerNormArgs& a, int type, int wtype, hipStream_t s) {
@@ -442,7 +478,7 @@ void launch_layer_norm_backward(const LayerNormGradArgs& given, int type, int wt
       int groups = 0;
       if (a.rows) {
         const bool held = row_team<T, 16>(packs, a.cols, [&](auto nt, auto nv, auto v) {
-          const dim3 grid = team_grid(a.rows, nt, kGradBlocks);
+          const dim3 grid = team_grid(a.rows, nt, nt > 64 ? kGradBlocks / 2 : kGradBlocks);
           groups = (int)grid.x;
           row_launch(ln_bwd<T, W, nt, nv, v>, grid, team_block(nt), s, a);
         });
@@ -455,7 +491,7 @@ void launch_layer_norm_backward(const LayerNormGradArgs& given, int type, int wt
         }
       }
       if (params)
-        row_launch(ln_bwd_finish<W>, dim3((2 * a.cols + 63) / 64), dim3(1024), s, a.partial, groups, a.cols, (W*)a.dgamma, (W*)a.dbeta, a.acc_w);
+        row_launch(ln_bwd_finish<W>, dim3((2 * a.cols + 31) / 32), dim3(1024), s, a.partial, groups, a.cols, (W*)a.dgamma, (W*)a.dbeta, a.acc_w);
     };
     if (wtype == type) go(t);
     else go(float{});
@@ -557,7 +593,7 @@ void launch_layer_norm_tangent_backward(const LayerNormTangentArgs& a, hipStream
   if (!a.dgamma) return;
   const int groups = part_groups(a.rows);
   row_launch(ln_tangent_bwd_columns, dim3(groups), dim3(256), s, a);
-  row_launch(ln_bwd_finish<float>, dim3((2 * a.cols + 63) / 64), dim3(1024), s, a.partial, groups, a.cols, a.dgamma, nullptr, a.acc_w);
+  row_launch(ln_bwd_finish<float>, dim3((2 * a.cols + 31) / 32), dim3(1024), s, a.partial, groups, a.cols, a.dgamma, nullptr, a.acc_w);
 }
 
 // ---- quantisation of rows of any length -----------------------------------------------------------------------------------------
