@@ -167,7 +167,7 @@ def load_library() -> C.CDLL:
     lib.eg_quantize_rows.argtypes = [i, p, i, p, n, i, p, p, f, n, n, p, n, p]
     lib.eg_int8_matmul_workspace.argtypes = [n, n, n]
     lib.eg_int8_matmul.argtypes = [i, p, p, n, p, p, n, p, p, n, n, n, i, p, n, p, n]
-    lib.eg_distill_loss_workspace.argtypes = [n, n]
+    lib.eg_distill_loss_workspace.argtypes = [n, n, n]
     lib.eg_distill_loss.argtypes = [i, p, i, p, n, i, p, n, p, n, p, n, n, n, f, p, p, n, p, n]
     for name in ('eg_layer_norm_workspace', 'eg_int8_matmul_workspace', 'eg_distill_loss_workspace'):
         getattr(lib, name).restype = n

@@ -159,9 +159,9 @@ int eg_int8_matmul(int device, void* stream, const signed char* a, long long lda
   });
 }
 
-long long eg_distill_loss_workspace(long long rows, long long cols) {
-  if (rows < 0 || cols < 0 || cols > kMaxCols) return -1;
-  return (long long)distill_partial_floats(rows, (int)cols) * 4;
+long long eg_distill_loss_workspace(long long rows, long long cols, long long top) {
+  if (rows < 0 || cols < 0 || cols > kMaxCols || top < 0 || top > 1024) return -1;
+  return (long long)distill_partial_floats(rows, (int)cols, (int)top) * 4;
 }
 
 int eg_distill_loss(int device, void* stream, int dtype, const void* logits, long long ld, int index_bytes, const void* index, long long ld_index,
@@ -180,7 +180,7 @@ int eg_distill_loss(int device, void* stream, int dtype, const void* logits, lon
     if (rows == 0) return;
     EG_CHECK(loss, "eg_distill_loss: null loss");
     EG_CHECK(cols > 0, "eg_distill_loss: rows without columns");
-    check_workspace("eg_distill_loss", workspace, workspace_bytes, distill_partial_floats(rows, (int)cols));
+    check_workspace("eg_distill_loss", workspace, workspace_bytes, distill_partial_floats(rows, (int)cols, (int)top));
     OnDevice on(device);
     launch_distill({logits, ld, index, ld_index, index_bytes == 8, teacher, ld_teacher, row_weight, rows, (int)cols, (int)top, temperature, 1.f, loss, grad, ldg,
                     0, (float*)workspace},

@@ -103,7 +103,7 @@ void launch_layer_norm_tangent_backward(const LayerNormTangentArgs& a, hipStream
 void launch_quantize_rows(const QuantizeArgs& a, int type, hipStream_t s);
 size_t int8_partial_floats(long long m, int n, int k);
 void launch_int8_matmul(const Int8Args& a, int out_type, float* partial, hipStream_t s);
-size_t distill_partial_floats(long long rows, int cols);
+size_t distill_partial_floats(long long rows, int cols, int top);
 void launch_distill(const DistillArgs& a, int type, hipStream_t s);
 
 }  // namespace eg

@@ -234,7 +234,7 @@ def distill_loss(logits: torch.Tensor, index: torch.Tensor, teacher: torch.Tenso
     w = _vector(row_weight, rows, 'row_weight', logits, (torch.float32,))
     loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=logits.device)
     dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if grad else None
-    keep, ws, size = _workspace(lib.eg_distill_loss_workspace(rows, cols), logits)
+    keep, ws, size = _workspace(lib.eg_distill_loss_workspace(rows, cols, top), logits)
     device, stream = _stream(logits)
     _check(lib.eg_distill_loss(device, stream, _TYPES[logits.dtype], logits.data_ptr(), ld, index.element_size(), index.data_ptr(), ldi, teacher.data_ptr(), ldt,
                                w, rows, cols, top, temperature, loss.data_ptr(), dlogits.data_ptr() if grad else None, cols, ws, size))

@@ -246,7 +246,7 @@ int eg_int8_matmul(int device, void* stream, const signed char* a, long long lda
  * loss[r] = w_r T^2 sum_k p_k (log p_k - log q_index[k]); grad (or NULL) = d(sum of loss) / d(logits).  index: 4- or 8-byte integers;
  * one outside [0, cols) is padding, one given twice counts twice.  row_weight f32 [rows] or NULL (1): a row of weight 0 or without a kept
  * logit has loss 0 and gradient 0 whatever its logits hold. */
-long long eg_distill_loss_workspace(long long rows, long long cols);
+long long eg_distill_loss_workspace(long long rows, long long cols, long long top);
 int eg_distill_loss(int device, void* stream, int dtype, const void* logits, long long ld, int index_bytes, const void* index,
                     long long ld_index, const float* teacher, long long ld_teacher, const float* row_weight, long long rows,
                     long long cols, long long top, float temperature, float* loss, void* grad, long long ldg, void* workspace,

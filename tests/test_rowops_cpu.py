@@ -68,7 +68,8 @@ def test_workspace_sizes(built_lib):
     assert built_lib.eg_layer_norm_workspace(-1, 8) == -1 and built_lib.eg_layer_norm_workspace(8, (1 << 24) + 1) == -1
     assert built_lib.eg_layer_norm_workspace(0, 8) == 0
     assert built_lib.eg_int8_matmul_workspace(1, 1, 131072) == -1 and built_lib.eg_int8_matmul_workspace(1, 4096, 4096) >= 0
-    assert built_lib.eg_distill_loss_workspace(1, -1) == -1 and built_lib.eg_distill_loss_workspace(4, 1000) >= 0
+    assert built_lib.eg_distill_loss_workspace(1, -1, 1) == -1 and built_lib.eg_distill_loss_workspace(1, 8, 1025) == -1
+    assert built_lib.eg_distill_loss_workspace(4, 1000, 8) >= 0
 
 
 def test_two_runtimes_are_refused(built_lib):
