@@ -5,7 +5,8 @@
 // of weight 0 have loss 0 and gradient 0, whatever the student's logits are.
 //
 // Bound by HBM: one read and one write of the logits.  A row stays in the registers of its team (a wave, 256 or 1,024 threads, at most 64 elements each) from
-// the load through maximum, exponential and sum to the store, so each exponential is taken once.  The few columns that the teacher names are corrected
+// the load through maximum and sum to the store: in 16 bits as loaded (half the registers: two rows of 65,536 a compute unit; the exponentials are taken twice), in
+// 32 bits as exponentials.  The few columns that the teacher names are corrected
 // behind the store of the row by the threads that hold the teacher's entries, in the same block.  exp((z - m) / T) is 2^((z - m) c): the difference
 // first, so that rows of the type's lowest value stay finite.
 #include <tuple>
@@ -17,9 +18,9 @@ namespace eg {
 constexpr int kDistillTop = 1024;   // most teacher logits a row
 constexpr int team_top(int nt) { return nt > 64 ? kDistillTop : 128; }   // ... that a team's LDS holds
 
-struct Kept {   // a teacher's entry: its column (-1: padding), (u - max u) / T and then p; the student's logit and the old gradient of the column
+struct Kept {   // a teacher's entry: its column (-1: padding), (u - max u) / T and then p; the student's logit in the column
   int idx;
-  float p, z, old;
+  float p, z;
 };
 
 // A team's threads see each other's LDS and memory writes of before.
@@ -36,10 +37,12 @@ __device__ __forceinline__ void team_sync() {
 template <int NT>
 __device__ __forceinline__ bool load_teacher(const DistillArgs& a, long long r, int t, Kept* kept, float (&red)[2][NT > 64 ? NT / 64 : 1], float it, float& log_norm) {
   float m = -INFINITY;
+#pragma unroll 1
   for (int k = t; k < a.top; k += NT) {
     const long long j = a.index64 ? ((const long long*)a.index)[r * a.ld_index + k] : (long long)((const int*)a.index)[r * a.ld_index + k];
+    const float given = a.teacher[r * a.ld_teacher + k];   // (beside the index, not behind it)
     const bool in = j >= 0 && j < a.cols;
-    const float u = in ? a.teacher[r * a.ld_teacher + k] : -INFINITY;
+    const float u = in ? given : -INFINITY;
     kept[k].idx = in ? (int)j : -1;
     kept[k].p = u;
     m = max_nan(m, u);
@@ -47,6 +50,7 @@ __device__ __forceinline__ bool load_teacher(const DistillArgs& a, long long r, 
   m = team_max<NT>(m, red[0]);
   if (m == -INFINITY) return false;
   float s[1] = {0.f};
+#pragma unroll 1
   for (int k = t; k < a.top; k += NT) {
     const float v = (kept[k].p - m) * it;
     kept[k].p = v;
@@ -58,17 +62,15 @@ __device__ __forceinline__ bool load_teacher(const DistillArgs& a, long long r, 
 }
 // What the row holds in the teacher's columns, before the row is stored (the gradient may lie in the logits' memory).
 template <typename T, int NT>
-__device__ __forceinline__ void read_named(const DistillArgs& a, const T* z, const T* g, int t, Kept* kept) {
-  for (int k = t; k < a.top; k += NT) {
-    const int j = kept[k].idx;
-    kept[k].z = j >= 0 ? (float)z[j] : 0.f;
-    kept[k].old = j >= 0 && a.acc && g ? (float)g[j] : 0.f;
-  }
+__device__ __forceinline__ void read_named(const DistillArgs& a, const T* z, int t, Kept* kept) {
+#pragma unroll 1
+  for (int k = t; k < a.top; k += NT) kept[k].z = kept[k].idx >= 0 ? (float)z[kept[k].idx] : 0.f;
 }
 // sum_k p_k (log p_k - log q_k); the entries' p become probabilities.  m: the student's maximum, log_sum the log of its exponentials' sum.
 template <int NT>
 __device__ __forceinline__ float teacher_loss(const DistillArgs& a, int t, Kept* kept, float (&red)[NT > 64 ? NT / 64 : 1], float it, float log_norm, float m, float log_sum) {
   float l[1] = {0.f};
+#pragma unroll 1
   for (int k = t; k < a.top; k += NT) {
     const float lp = kept[k].p - log_norm;
     const float p = kept[k].idx >= 0 ? expf(lp) : 0.f;
@@ -79,89 +81,152 @@ __device__ __forceinline__ float teacher_loss(const DistillArgs& a, int t, Kept*
   return l[0];
 }
 // The gradient's columns lo .. hi - 1 that the teacher names; an index given several times is written several times, with the same value.
-template <typename T, int NT>
-__device__ __forceinline__ void write_named(const DistillArgs& a, T* g, int t, const Kept* kept, float c, float m, float inv, float f, int lo, int hi) {
+// log_q: of a logit.
+template <typename T, int NT, typename L>
+__device__ __forceinline__ void write_named(const DistillArgs& a, T* g, int t, const Kept* kept, float f, L log_q, int lo, int hi) {
+#pragma unroll 1
   for (int k = t; k < a.top; k += NT) {
     const int j = kept[k].idx;
     if (j < lo || j >= hi) continue;
     float p = 0.f;
+#pragma unroll 4
     for (int l = 0; l < a.top; ++l) p += kept[l].idx == j ? kept[l].p : 0.f;
-    g[j] = (T)(kept[k].old + f * (__builtin_amdgcn_exp2f((kept[k].z - m) * c) * inv - p));
+    g[j] = (T)(f * (expf(log_q(kept[k].z)) - p));
   }
 }
 
 constexpr float kLog2e = 1.44269504088896340736f;
-// A row in a team's registers.
+// Tells the compiler that a pack may have changed: it then forms what follows from the pack again instead of keeping its converted elements and their
+// exponentials in registers from one pass over the row to the next.
+template <typename T, int V>
+__device__ __forceinline__ void opaque(Pack<T, V>& p) {
+  if constexpr (sizeof(p) == 2) {
+    unsigned u = __builtin_bit_cast(unsigned short, p);
+    asm volatile("" : "+v"(u));
+    p = __builtin_bit_cast(Pack<T, V>, (unsigned short)u);
+  } else {
+    struct Words {
+      unsigned w[sizeof(p) / 4];
+    } k = __builtin_bit_cast(Words, p);
+#pragma unroll
+    for (unsigned& w : k.w) asm volatile("" : "+v"(w));
+    p = __builtin_bit_cast(Pack<T, V>, k);
+  }
+}
+
+// The largest of packs.  In 16 bits two elements an instruction: as signed whole numbers non-negative floats keep their order and negative ones lie
+// below them in reversed order, so the row's maximum is the largest whole number if that is a non-negative float, else the smallest.  (A NaN need not be kept: the sum is then NaN.)
+template <typename T>
+struct RowMax {
+  using i16x2 = __attribute__((ext_vector_type(2))) short;
+  float m = -INFINITY;
+  i16x2 hi = {-32768, -32768}, lo = {32767, 32767};
+  template <int V>
+  __device__ __forceinline__ void take(const Pack<T, V>& p) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) m = fmaxf(m, p.e[j]);
+    } else if constexpr (V == 1) {
+      const short k = __builtin_bit_cast(short, p);
+      hi.x = hi.x > k ? hi.x : k;
+      lo.x = lo.x < k ? lo.x : k;
+    } else {
+      struct Words {
+        i16x2 w[V / 2];
+      } k = __builtin_bit_cast(Words, p);
+#pragma unroll
+      for (int j = 0; j < V / 2; ++j) {
+        hi = __builtin_elementwise_max(hi, k.w[j]);
+        lo = __builtin_elementwise_min(lo, k.w[j]);
+      }
+    }
+  }
+  __device__ __forceinline__ float value() const {
+    if constexpr (sizeof(T) == 4) return m;
+    else {
+      const short h = hi.x > hi.y ? hi.x : hi.y, l = lo.x < lo.y ? lo.x : lo.y;
+      return (float)__builtin_bit_cast(T, h >= 0 ? h : l);
+    }
+  }
+};
+// A row in a team's registers.  A long row is alone in its registers: the teacher's part lies before the load and behind the
+// store (with it in between the compiler spilt the row).  The other block of a compute unit fills the waits.
 template <typename T, int NT, int NE, int V>
-__global__ __launch_bounds__(NT > 256 ? NT : 256) void distill_rows(DistillArgs a) {
+__global__ __launch_bounds__(NT > 256 ? NT : 256) __attribute__((amdgpu_waves_per_eu(NT == 1024 && sizeof(T) == 2 && V > 1 ? 8 : 1))) void distill_rows(DistillArgs a) {
   constexpr int NB = NT > 256 ? NT : 256, TEAMS = NB / NT, NV = NE / V;
   __shared__ Kept all_kept[TEAMS][team_top(NT)];
   __shared__ float red_t[2][NT > 64 ? NT / 64 : 1], red[3][NT > 64 ? NT / 64 : 1];   // (one wave needs none)
-  const int t = threadIdx.x % NT, team = threadIdx.x / NT;
+  const int t = TEAMS > 1 ? threadIdx.x % NT : threadIdx.x, team = TEAMS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / NT) : 0;
+  const long long r = (long long)blockIdx.x * TEAMS + team;
+  if (r >= a.rows) return;   // (a whole wave)
   Kept* kept = all_kept[team];
   const float it = 1.f / a.temperature, c = it * kLog2e;
-  for (long long r = (long long)blockIdx.x * TEAMS + team; r < a.rows; r += (long long)gridDim.x * TEAMS) {
-    const T* z = (const T*)a.logits + r * a.ld;
-    T* g = a.grad ? (T*)a.grad + r * a.ldg : nullptr;
-    const float w = (a.row_weight ? a.row_weight[r] : 1.f) * a.weight;
-    float v[NV][V], log_norm = 0.f;
-    bool alive = w != 0.f;
-    if (alive) {
+  const T* z = (const T*)a.logits + r * a.ld;
+  T* g = a.grad ? (T*)a.grad + r * a.ldg : nullptr;
+  const float w = (a.row_weight ? a.row_weight[r] : 1.f) * a.weight;
+  const unsigned row_bytes = (unsigned)a.cols * sizeof(T);
+  const __amdgpu_buffer_rsrc_t zb = row_buffer(z, row_bytes), gb = row_buffer(g, g ? row_bytes : 0);
+  Pack<T, V> v[NV];
+  auto load_row = [&] {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int at = (i * NT + t) * V;
-        load_pack<T, V>(z + (at < a.cols ? at : 0), v[i]);   // (columns past the last repeat the first ones; they are left out of the sum)
-      }
-      alive = load_teacher<NT>(a, r, t, kept, red_t, it, log_norm);
+    for (int i = 0; i < NV; ++i) v[i] = buffer_load<T, V>(zb, min((t + i * NT) * V, a.cols - V) * sizeof(T));   // (past the end: the last pack again, left out of the sum)
+  };
+  constexpr bool EARLY = NE <= 16;   // few registers: the row is on its way while the teacher's part is worked on
+  if constexpr (EARLY) load_row();
+  float log_norm = 0.f;
+  if (w == 0.f || !load_teacher<NT>(a, r, t, kept, red_t, it, log_norm)) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const float zero[V] = {};
+      buffer_store<T, V>(gb, (t + i * NT) * V * sizeof(T), zero);
     }
-    if (!alive) {
-      if (g && !a.acc) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const int at = (i * NT + t) * V;
-          const float zero[V] = {};
-          if (at < a.cols) store_pack<T, V>(g + at, zero);
-        }
-      }
-      if (t == 0) a.loss[r] = 0.f;
-      team_sync<NT>();
-      continue;
-    }
-    read_named<T, NT>(a, z, g, t, kept);
-    float m = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < V; ++j) m = max_nan(m, v[i][j]);
-    m = team_max<NT>(m, red[0]);
-    float s[1] = {0.f};
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        v[i][j] = (i * NT + t) * V < a.cols ? __builtin_amdgcn_exp2f((v[i][j] - m) * c) : 0.f;
-        s[0] += v[i][j];
-      }
-    team_sum<NT>(s, red[1]);
-    const float loss = teacher_loss<NT>(a, t, kept, red[2], it, log_norm, m, logf(s[0]));
-    if (t == 0) a.loss[r] = w * a.temperature * a.temperature * loss;
-    if (g) {
-      const float f = w * a.temperature, inv = 1.f / s[0], fi = f * inv;
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int at = (i * NT + t) * V;
-        if (at >= a.cols) continue;
-        float o[V] = {};
-        if (a.acc) load_pack<T, V>(g + at, o);
-#pragma unroll
-        for (int j = 0; j < V; ++j) o[j] += v[i][j] * fi;
-        store_pack<T, V>(g + at, o);
-      }
-      team_sync<NT>();
-      write_named<T, NT>(a, g, t, kept, c, m, inv, f, 0, a.cols);
-    }
-    team_sync<NT>();
+    if (t == 0) a.loss[r] = 0.f;
+    return;
   }
+  read_named<T, NT>(a, z, t, kept);
+  if constexpr (!EARLY) load_row();
+  RowMax<T> most;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    most.take(v[i]);
+    if constexpr (NE > 16) __builtin_amdgcn_sched_barrier(0);   // (pack by pack: the scheduler would convert the whole row at once)
+  }
+  const float m = team_max<NT>(most.value(), red[0]);
+  float s[1] = {0.f};
+  const int t1 = fresh(t);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    opaque(v[i]);
+    float part = 0.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float e = __builtin_amdgcn_exp2f(((float)v[i].e[j] - m) * c);
+      if constexpr (sizeof(T) == 4) v[i].e[j] = e;
+      part += e;
+    }
+    s[0] += (t1 + i * NT) * V < a.cols ? part : 0.f;
+    opaque(v[i]);
+    if constexpr (NE > 16) __builtin_amdgcn_sched_barrier(0);
+  }
+  team_sum<NT>(s, red[1]);
+  const float f = w * a.temperature;
+  if (g) {
+    const float fi = f / s[0];
+    const int t2 = fresh(t);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float o[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) o[j] = (sizeof(T) == 4 ? (float)v[i].e[j] : __builtin_amdgcn_exp2f(((float)v[i].e[j] - m) * c)) * fi;
+      buffer_store<T, V>(gb, (t2 + i * NT) * V * sizeof(T), o);
+      if constexpr (NE > 16) __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  const float log_sum = logf(s[0]);
+  const float loss = teacher_loss<NT>(a, t, kept, red[2], it, log_norm, m, log_sum);
+  if (t == 0) a.loss[r] = f * a.temperature * loss;
+  team_sync<NT>();
+  if (g) write_named<T, NT>(a, g, t, kept, f, [&](float x) { return it * (x - m) - log_sum; }, 0, a.cols);
 }
 
 // ---- a row over several blocks ----------------------------------------------------------------------------------------------------
@@ -232,17 +297,13 @@ __global__ __launch_bounds__(kChunkThreads) void distill_chunk_grad(DistillArgs 
     const float w = (a.row_weight ? a.row_weight[r] : 1.f) * a.weight;
     float log_norm = 0.f;
     if (w == 0.f || !load_teacher<kChunkThreads>(a, r, t, kept, red_t, it, log_norm)) {
-      if (g && !a.acc)
+      if (g)
         for (int j = lo + t; j < hi; j += kChunkThreads) g[j] = (T)0.f;
       if (t == 0 && chunk == 0) a.loss[r] = 0.f;
       __syncthreads();
       continue;
     }
-    for (int k = t; k < a.top; k += kChunkThreads) {
-      const int j = kept[k].idx;
-      kept[k].z = in[2 * chunks + k];
-      kept[k].old = j >= lo && j < hi && a.acc && g ? (float)g[j] : 0.f;   // (read_named, of this block's columns)
-    }
+    for (int k = t; k < a.top; k += kChunkThreads) kept[k].z = in[2 * chunks + k];
     float m = -INFINITY;
     for (int k = t; k < chunks; k += kChunkThreads) m = max_nan(m, in[2 * k]);
     m = team_max<kChunkThreads>(m, red[0]);
@@ -250,20 +311,20 @@ __global__ __launch_bounds__(kChunkThreads) void distill_chunk_grad(DistillArgs 
     for (int k = t; k < chunks; k += kChunkThreads)
       if (in[2 * k] != -INFINITY) s[0] += in[2 * k + 1] * __builtin_amdgcn_exp2f((in[2 * k] - m) * c);
     team_sum<kChunkThreads>(s, red[1]);
-    const float loss = teacher_loss<kChunkThreads>(a, t, kept, red[2], it, log_norm, m, logf(s[0]));
+    const float log_sum = logf(s[0]);
+    const float loss = teacher_loss<kChunkThreads>(a, t, kept, red[2], it, log_norm, m, log_sum);
     if (t == 0 && chunk == 0) a.loss[r] = w * a.temperature * a.temperature * loss;
     if (g) {
-      const float f = w * a.temperature, inv = 1.f / s[0], fi = f * inv;
+      const float f = w * a.temperature, fi = f / s[0];
       walk<V>(lo, hi, [&](int at) {
-        float v[V], o[V] = {};
+        float v[V], o[V];
         load_pack<T, V>(z + at, v);
-        if (a.acc) load_pack<T, V>(g + at, o);
 #pragma unroll
-        for (int j = 0; j < V; ++j) o[j] += __builtin_amdgcn_exp2f((v[j] - m) * c) * fi;
+        for (int j = 0; j < V; ++j) o[j] = __builtin_amdgcn_exp2f((v[j] - m) * c) * fi;
         store_pack<T, V>(g + at, o);
       });
       __syncthreads();
-      write_named<T, kChunkThreads>(a, g, t, kept, c, m, inv, f, lo, hi);
+      write_named<T, kChunkThreads>(a, g, t, kept, f, [&](float z) { return it * (z - m) - log_sum; }, lo, hi);
     }
     __syncthreads();
   }
@@ -280,7 +341,18 @@ template <typename T, int V>
 static void distill_team(const DistillArgs& a, hipStream_t s) {
   auto go = [&](auto nt, auto ne) {
     constexpr int NT = decltype(nt)::value, NE = decltype(ne)::value, TEAMS = NT > 256 ? 1 : 256 / NT;
-    row_launch(distill_rows<T, NT, NE, V>, dim3((unsigned)std::min<long long>((a.rows + TEAMS - 1) / TEAMS, 1 << 16)), dim3(NT > 256 ? NT : 256), s, a);
+    constexpr long long slab = 1 << 20;   // rows of a launch (a grid has fewer than 2^32 threads)
+    for (long long r = 0; r < a.rows; r += slab) {
+      DistillArgs p = a;
+      p.rows = std::min(slab, a.rows - r);
+      p.logits = (const T*)a.logits + r * a.ld;
+      p.index = (const char*)a.index + r * a.ld_index * (a.index64 ? 8 : 4);
+      p.teacher = a.teacher + r * a.ld_teacher;
+      if (a.row_weight) p.row_weight = a.row_weight + r;
+      p.loss = a.loss + r;
+      if (a.grad) p.grad = (T*)a.grad + r * a.ldg;
+      row_launch(distill_rows<T, NT, NE, V>, dim3((unsigned)((p.rows + TEAMS - 1) / TEAMS)), dim3(NT > 256 ? NT : 256), s, p);
+    }
   };
   using std::integral_constant;
 #define EG_TEAM(NT, NE) if (a.cols <= (NT) * (NE) && a.top <= team_top(NT)) return go(integral_constant<int, NT>{}, integral_constant<int, NE>{})

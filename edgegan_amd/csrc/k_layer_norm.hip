@@ -107,7 +107,7 @@ template <typename T, typename W, int NT, int NV, int V>
 __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_fwd(LayerNormArgs a) {
   constexpr int NB = NT > 256 ? NT : 256, TEAMS = NB / NT;
   __shared__ double red[2][centre_lds(NT)];
-  const int t = threadIdx.x % NT, team = threadIdx.x / NT;
+  const int t = TEAMS > 1 ? threadIdx.x % NT : threadIdx.x, team = TEAMS > 1 ? threadIdx.x / NT : 0;
   float g[NV][V], b[NV][V];
   load_parameter<W, NT, NV, V>((const W*)a.gamma, a.cols, t, 1.f, g);
   load_parameter<W, NT, NV, V>((const W*)a.beta, a.cols, t, 0.f, b);
@@ -137,7 +137,7 @@ template <typename T, typename W, int NT, int NV, int V>
 __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_bwd(LayerNormGradArgs a) {
   constexpr int NB = NT > 256 ? NT : 256, TEAMS = NB / NT;
   __shared__ float red[2][NT > 64 ? 2 * NT / 64 : 1];
-  const int t = threadIdx.x % NT, team = threadIdx.x / NT;
+  const int t = TEAMS > 1 ? threadIdx.x % NT : threadIdx.x, team = TEAMS > 1 ? threadIdx.x / NT : 0;
   float g[NV][V], sx[NV][V], sg[NV][V];
   load_parameter<W, NT, NV, V>((const W*)a.gamma, a.cols, t, 1.f, g);
 #pragma unroll
@@ -277,7 +277,7 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void quantize_rows(QuantizeArg
   constexpr int NB = NT > 256 ? NT : 256, TEAMS = NB / NT;
   __shared__ double red[2][centre_lds(NT)];
   __shared__ float red_max[2][NT > 64 ? NT / 64 : 1];
-  const int t = threadIdx.x % NT, team = threadIdx.x / NT;
+  const int t = TEAMS > 1 ? threadIdx.x % NT : threadIdx.x, team = TEAMS > 1 ? threadIdx.x / NT : 0;
   const int width = (int)min((long long)((a.cols + 15) & ~15), a.ldq);   // the row's last 16-byte group is filled up with zeros
   int turn = 0;
   for (long long r = (long long)blockIdx.x * TEAMS + team; r < a.rows; r += (long long)gridDim.x * TEAMS, turn ^= 1) {

@@ -183,7 +183,7 @@ int eg_distill_loss(int device, void* stream, int dtype, const void* logits, lon
     check_workspace("eg_distill_loss", workspace, workspace_bytes, distill_partial_floats(rows, (int)cols, (int)top));
     OnDevice on(device);
     launch_distill({logits, ld, index, ld_index, index_bytes == 8, teacher, ld_teacher, row_weight, rows, (int)cols, (int)top, temperature, 1.f, loss, grad, ldg,
-                    0, (float*)workspace},
+                    (float*)workspace},
                    dtype, (hipStream_t)stream);
   });
 }

@@ -91,7 +91,6 @@ struct DistillArgs {
   float* loss;                // [rows]
   void* grad;                 // null: not wanted
   long long ldg;
-  int acc;                    // grad += (f32 only)
   float* partial;             // distill_partial_floats()
 };
 

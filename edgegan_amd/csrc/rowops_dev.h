@@ -145,4 +145,32 @@ __device__ __forceinline__ void store_pack(T* p, const float (&v)[V]) {
   *reinterpret_cast<Pack<T, V>*>(p) = k;
 }
 
+// A row as a buffer of its own: a load past its end gives zero and a store there is dropped, and an element's address is one register. The row
+// has to be the same one for the whole wave.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t row_buffer(const void* p, unsigned bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00020000);
+}
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> buffer_load(__amdgpu_buffer_rsrc_t b, unsigned offset) {
+  static_assert(sizeof(Pack<T, V>) == 2 || sizeof(Pack<T, V>) == 4 || sizeof(Pack<T, V>) == 16, "");
+  if constexpr (sizeof(Pack<T, V>) == 2) return __builtin_bit_cast(Pack<T, V>, __builtin_amdgcn_raw_buffer_load_b16(b, offset, 0, 0));
+  else if constexpr (sizeof(Pack<T, V>) == 4) return __builtin_bit_cast(Pack<T, V>, __builtin_amdgcn_raw_buffer_load_b32(b, offset, 0, 0));
+  else return __builtin_bit_cast(Pack<T, V>, __builtin_amdgcn_raw_buffer_load_b128(b, offset, 0, 0));
+}
+template <typename T, int V>
+__device__ __forceinline__ void buffer_store(__amdgpu_buffer_rsrc_t b, unsigned offset, const float (&v)[V]) {
+  Pack<T, V> k;
+#pragma unroll
+  for (int i = 0; i < V; ++i) k.e[i] = (T)v[i];
+  using u32x4 = __attribute__((ext_vector_type(4))) unsigned;
+  if constexpr (sizeof(k) == 2) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, k), b, offset, 0, 0);
+  else if constexpr (sizeof(k) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, k), b, offset, 0, 0);
+  else __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, k), b, offset, 0, 0);
+}
+// A value that the compiler forms anew in each turn of a loop instead of keeping everything that depends on it in registers from turn to turn.
+__device__ __forceinline__ int fresh(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
 }  // namespace eg
