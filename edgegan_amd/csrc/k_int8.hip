@@ -21,12 +21,8 @@ __device__ __forceinline__ i32x4 load16(const signed char* row, int k, int k_end
   return v;
 }
 
-template <typename T>
-__device__ __forceinline__ void store_out(const Int8Args& a, long long i, int j, int sum) {
-  float v = __fmul_rn((float)sum * a.a_scale[i], a.b_scale[j]);
-  if (a.bias) v += a.bias[j];
-  ((T*)a.out)[i * a.ldo + j] = (T)v;
-}
+// the same operations in every kernel, so that a result does not depend on the variant
+__device__ __forceinline__ float int8_result(int sum, float sa, float sb, float bias) { return rounded_mul(rounded_mul((float)sum, sa), sb) + bias; }
 
 // Any sizes, strides and alignment: 64 x 64 outputs a block, a wave 32 x 32 of them, operands straight from memory.
 template <typename T>
@@ -63,19 +59,173 @@ __global__ __launch_bounds__(256) void int8_any(Int8Args a, int tiles_n, int ali
       for (int v = 0; v < 4; ++v) {
         const long long i = i0 + x * 16 + (lane >> 4) * 4 + v;
         const int j = j0 + y * 16 + l15;
-        if (i < a.m && j < a.n) store_out<T>(a, i, j, acc[x][y][v]);
+        if (i < a.m && j < a.n) ((T*)a.out)[i * a.ldo + j] = (T)int8_result(acc[x][y][v], a.a_scale[i], a.b_scale[j], a.bias ? a.bias[j] : 0.f);
       }
+}
+
+// ---- tiles in LDS ------------------------------------------------------------------------------------------------------------------
+// BM x BN outputs a block, WM x WN waves, 128 bytes of k a step, two buffers: while a step's 32x32x32 products run, the next step's tiles are on their way from memory
+// straight to LDS.  A tile row is eight 16-byte groups; group s of row r holds the row's group s ^ (r & 7), so that the 32 rows of a
+// fragment lie in different banks (the write is a wave's 1,024 consecutive bytes: the permutation is in the source addresses).
+// Rows past the end repeat the last one (their results are not stored); groups past k read as zeros; the bytes past k in its last group are cleared
+// in a's fragments, which is enough.
+using i32x16 = __attribute__((ext_vector_type(16))) int;
+constexpr int kStep = 128;
+
+template <int BM, int BN, int WM, int WN>
+struct TileShape {
+  static constexpr int NW = WM * WN, MI = BM / WM / 32, NI = BN / WN / 32, JA = BM / 8 / NW, JB = BN / 8 / NW;
+  static_assert(JA * 8 * NW == BM && JB * 8 * NW == BN, "whole rows of 8 for every wave");
+};
+// A wave's part of a tile: N times 8 rows, straight into LDS
+template <int N>
+__device__ __forceinline__ void request_tile(__amdgpu_buffer_rsrc_t from, const unsigned (&voff)[N], bool in, int k, signed char* to, int waves, int wave) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const unsigned v = in ? voff[j] : 0x80000000u;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void*)(to + (j * waves + wave) * 8 * kStep), 16, v, k, 0, 0);
+  }
+}
+// One step: the next tiles requested (into `na`, `nb`), the current ones multiplied.  The four buffers are different memory and said to be (restrict): the compiler
+// would otherwise wait for the requests before it reads the current tiles.
+template <typename S, bool TAIL>
+__device__ __forceinline__ void int8_step(const signed char* __restrict__ ca, const signed char* __restrict__ cb, signed char* __restrict__ na, signed char* __restrict__ nb,
+                                          __amdgpu_buffer_rsrc_t ab, __amdgpu_buffer_rsrc_t bb, const unsigned (&va)[S::JA], const unsigned (&vb)[S::JB], int koff, int k_all, int k,
+                                          int wave, int lane, int arow, int brow, i32x16 (&acc)[S::MI][S::NI]) {
+  if constexpr (!TAIL) {
+    const bool in = k + kStep + koff < k_all;
+    request_tile<S::JA>(ab, va, in, k + kStep, na, S::NW, wave);
+    request_tile<S::JB>(bb, vb, in, k + kStep, nb, S::NW, wave);
+    __builtin_amdgcn_sched_barrier(0);   // (the requests first: the scheduler would put them behind the products)
+  }
+  const int l31 = lane & 31, lh = lane >> 5;
+#pragma unroll
+  for (int ks = 0; ks < kStep / 32; ++ks) {
+    const int slot = ((ks * 2 + lh) ^ (l31 & 7)) * 16;
+    i32x4 fa[S::MI], fb[S::NI];
+#pragma unroll
+    for (int x = 0; x < S::MI; ++x) fa[x] = *reinterpret_cast<const i32x4*>(ca + (arow + x * 32) * kStep + slot);
+#pragma unroll
+    for (int y = 0; y < S::NI; ++y) fb[y] = *reinterpret_cast<const i32x4*>(cb + (brow + y * 32) * kStep + slot);
+    if constexpr (TAIL) {   // the last step: a's bytes past k
+      const int ends = k_all - k - (ks * 2 + lh) * 16;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        const int keep = min(max(ends - 4 * d, 0), 4), mask = keep == 4 ? -1 : (1 << (8 * keep)) - 1;
+#pragma unroll
+        for (int x = 0; x < S::MI; ++x) fa[x][d] &= mask;
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < S::MI; ++x)
+#pragma unroll
+      for (int y = 0; y < S::NI; ++y) acc[x][y] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[x], fb[y], acc[x][y], 0, 0, 0);
+  }
+}
+
+// every wave's requests have arrived, every wave's reads are done
+__device__ __forceinline__ void tiles_ready() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+
+template <typename T, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(WM * WN * 64) void int8_tiles(Int8Args a, int tiles_m, int tiles_n) {
+  using S = TileShape<BM, BN, WM, WN>;
+  __shared__ __attribute__((aligned(16))) signed char tiles[2][(BM + BN) * kStep];   // a's tile, b's tile
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  const int tile = blockIdx.x;
+  const int tm = __builtin_amdgcn_readfirstlane(tile / tiles_n), tn = tile - tm * tiles_n;
+  const long long i0 = (long long)tm * BM;
+  const int j0 = tn * BN;
+
+  const __amdgpu_buffer_rsrc_t ab = row_buffer(a.a + i0 * a.lda, 0x7ffffff0u), bb = row_buffer(a.b + (long long)j0 * a.ldb, 0x7ffffff0u);
+  const int koff = ((lane & 7) ^ (lane >> 3)) * 16;   // this lane's group of a row in k
+  const int rows_a = (int)min((long long)BM, a.m - i0) - 1, rows_b = min(BN, a.n - j0) - 1;
+  unsigned va[S::JA], vb[S::JB];
+#pragma unroll
+  for (int j = 0; j < S::JA; ++j) va[j] = (unsigned)min((j * S::NW + wave) * 8 + (lane >> 3), rows_a) * (unsigned)a.lda + koff;
+#pragma unroll
+  for (int j = 0; j < S::JB; ++j) vb[j] = (unsigned)min((j * S::NW + wave) * 8 + (lane >> 3), rows_b) * (unsigned)a.ldb + koff;
+  i32x16 acc[S::MI][S::NI];
+#pragma unroll
+  for (int x = 0; x < S::MI; ++x)
+#pragma unroll
+    for (int y = 0; y < S::NI; ++y)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[x][y][v] = 0;
+  const int l31 = lane & 31, lh = lane >> 5;
+  const int arow = wm * (BM / WM) + l31, brow = wn * (BN / WN) + l31;
+  request_tile<S::JA>(ab, va, koff < a.k, 0, tiles[0], S::NW, wave);
+  request_tile<S::JB>(bb, vb, koff < a.k, 0, tiles[0] + BM * kStep, S::NW, wave);
+  int k = 0, cur = 0;
+  for (; k + kStep < a.k; k += kStep, cur ^= 1) {
+    tiles_ready();
+    int8_step<S, false>(tiles[cur], tiles[cur] + BM * kStep, tiles[cur ^ 1], tiles[cur ^ 1] + BM * kStep, ab, bb, va, vb, koff, a.k, k, wave, lane, arow, brow, acc);
+  }
+  tiles_ready();
+  int8_step<S, true>(tiles[cur], tiles[cur] + BM * kStep, nullptr, nullptr, ab, bb, va, vb, koff, a.k, k, wave, lane, arow, brow, acc);
+  // result layout: lane l, register v: row 8 (v / 4) + 4 (l >> 5) + v % 4, column l & 31
+  const int jw = wn * (BN / WN) + l31, iw = wm * (BM / WM) + lh * 4;
+  float* scales = reinterpret_cast<float*>(tiles[0]);   // the rows' scales
+  __syncthreads();
+  for (int i = threadIdx.x; i < BM; i += S::NW * 64) scales[i] = a.a_scale[i0 + min(i, rows_a)];
+  float sb[S::NI], bias[S::NI];
+#pragma unroll
+  for (int y = 0; y < S::NI; ++y) {
+    const int j = j0 + min(jw + y * 32, rows_b);
+    sb[y] = a.b_scale[j];
+    bias[y] = a.bias ? a.bias[j] : 0.f;
+  }
+  __syncthreads();
+  // (a row or column past the end has an offset past the buffer's: its store is dropped)
+  const __amdgpu_buffer_rsrc_t ob = row_buffer((T*)a.out + i0 * a.ldo + j0, 0x7ffffff0u);
+#pragma unroll
+  for (int x = 0; x < S::MI; ++x)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      const int i = iw + x * 32 + (v >> 2) * 8 + (v & 3);
+      const float sa = scales[i];
+      const unsigned at = i <= rows_a ? (unsigned)(i * (int)a.ldo + jw) * (unsigned)sizeof(T) : 0x80000000u;
+#pragma unroll
+      for (int y = 0; y < S::NI; ++y) {
+        const float o[1] = {int8_result(acc[x][y][v], sa, sb[y], bias[y])};
+        buffer_store<T, 1>(ob, jw + y * 32 <= rows_b ? at + y * 32 * (unsigned)sizeof(T) : 0x80000000u, o);
+      }
+      if (v % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+    }
 }
 
 size_t int8_partial_floats(long long m, int n, int k) { return 0; }
 
-void launch_int8_matmul(const Int8Args& a, int out_type, float* partial, hipStream_t s) {
+void launch_int8_matmul(const Int8Args& given, int out_type, float* partial, hipStream_t s) {
+  Int8Args a = given;
   if (a.m == 0 || a.n == 0) return;
+  if (a.m == 1) a.lda = (a.k + 15) & ~15;   // (a single row's distance to the next says nothing)
+  if (a.n == 1) a.ldb = (a.k + 15) & ~15;
   const int al_a = ((uintptr_t)a.a | (uintptr_t)a.lda) % 16 == 0, al_b = ((uintptr_t)a.b | (uintptr_t)a.ldb) % 16 == 0;
-  const long long tiles_m = (a.m + 63) / 64, tiles_n = (a.n + 63) / 64;
-  EG_CHECK(tiles_m * tiles_n < (1ll << 24), "int8 product: too many outputs (%lld x %d)", a.m, a.n);
+  auto grid = [&](int bm, int bn, int& tm, int& tn) {
+    const long long m = (a.m + bm - 1) / bm, n = (a.n + bn - 1) / bn;
+    EG_CHECK(m * n < (1ll << 22), "int8 product: too many outputs (%lld x %d)", a.m, a.n);
+    tm = (int)m;
+    tn = (int)n;
+    return dim3((unsigned)(m * n));
+  };
   by_type(out_type, [&](auto t) {
-    row_launch(int8_any<decltype(t)>, dim3((unsigned)(tiles_m * tiles_n)), dim3(256), s, a, (int)tiles_n, al_a, al_b);
+    using T = decltype(t);
+    int tm, tn;
+    if (al_a && al_b && a.lda <= 1 << 22 && a.ldb <= 1 << 22 && a.ldo <= 1 << 20 && a.k >= 16) {
+      const long long big = ((a.m + 255) / 256) * ((a.n + 255) / 256);
+      if (big >= 200) {
+        const dim3 g = grid(256, 256, tm, tn);
+        return row_launch(int8_tiles<T, 256, 256, 2, 4>, g, dim3(512), s, a, tm, tn);
+      }
+      const dim3 g = grid(128, 128, tm, tn);
+      return row_launch(int8_tiles<T, 128, 128, 2, 2>, g, dim3(256), s, a, tm, tn);
+    }
+    const dim3 g = grid(64, 64, tm, tn);
+    row_launch(int8_any<T>, g, dim3(256), s, a, tn, al_a, al_b);
   });
 }
 

@@ -19,10 +19,10 @@ namespace eg {
 
 template <typename W>
 __device__ __forceinline__ float affine(float xh, const W* gamma, const W* beta, int c) {
-  const float z = gamma ? __fmul_rn(xh, (float)gamma[c]) : xh;
-  return beta ? __fadd_rn(z, (float)beta[c]) : z;
+  const float z = gamma ? rounded_mul(xh, (float)gamma[c]) : xh;
+  return beta ? z + (float)beta[c] : z;
 }
-__device__ __forceinline__ float affine_r(float xh, float gamma, float beta) { return __fadd_rn(__fmul_rn(xh, gamma), beta); }
+__device__ __forceinline__ float affine_r(float xh, float gamma, float beta) { return rounded_mul(xh, gamma) + beta; }
 
 // ---- rows in registers -------------------------------------------------------------------------------------------------------
 // NT threads own a row, each NV packs of V consecutive elements: pack i of thread t begins at column (i NT + t) V.
@@ -124,7 +124,7 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_fwd(LayerNormArgs a) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[i][j] = row_act(affine_r(__fmul_rn(v[i][j], rstd), g[i][j], b[i][j]), a.act);
+      for (int j = 0; j < V; ++j) v[i][j] = row_act(affine_r(rounded_mul(v[i][j], rstd), g[i][j], b[i][j]), a.act);
     store_row<T, NT, NV, V>((T*)a.y + r * a.ldy, a.cols, t, v);
     if (t == 0 && a.mean) {
       a.mean[r] = mean;
@@ -169,14 +169,14 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_bwd(LayerNormGradArgs 
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int j = 0; j < V; ++j) d[i][j] *= row_act_grad(affine_r(__fmul_rn(x[i][j] - mean, rstd), g[i][j], b[i][j]), a.act);
+        for (int j = 0; j < V; ++j) d[i][j] *= row_act_grad(affine_r(rounded_mul(x[i][j] - mean, rstd), g[i][j], b[i][j]), a.act);
     }
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < V; ++j) {   // (columns past the last have d = 0 and reach no sum)
-        x[i][j] = __fmul_rn(x[i][j] - mean, rstd);
+        x[i][j] = rounded_mul(x[i][j] - mean, rstd);
         sg[i][j] += d[i][j];
         sx[i][j] += d[i][j] * x[i][j];
         d[i][j] *= g[i][j];
@@ -290,12 +290,12 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void quantize_rows(QuantizeArg
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[i][j] = __fmul_rn(__fmul_rn(v[i][j], rstd), p[i][j]);
+        for (int j = 0; j < V; ++j) v[i][j] = rounded_mul(rounded_mul(v[i][j], rstd), p[i][j]);
       load_parameter<float, NT, NV, V>(a.beta, a.cols, t, 0.f, p);
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[i][j] = __fadd_rn(v[i][j], p[i][j]);
+        for (int j = 0; j < V; ++j) v[i][j] = v[i][j] + p[i][j];
     }
     float m = 0.f;
 #pragma unroll
@@ -345,7 +345,7 @@ __global__ __launch_bounds__(kRowThreads) void ln_fwd_rows(LayerNormArgs a) {
     float mean, rstd;
     row_statistics<T>(x, a.cols, a.eps, red, mean, rstd);
     for (int c = threadIdx.x; c < a.cols; c += kRowThreads)
-      y[c] = (T)row_act(affine(__fmul_rn((float)x[c] - mean, rstd), (const W*)a.gamma, (const W*)a.beta, c), a.act);
+      y[c] = (T)row_act(affine(rounded_mul((float)x[c] - mean, rstd), (const W*)a.gamma, (const W*)a.beta, c), a.act);
     if (threadIdx.x == 0 && a.mean) {
       a.mean[r] = mean;
       a.rstd[r] = rstd;
@@ -357,7 +357,7 @@ __global__ __launch_bounds__(kRowThreads) void ln_fwd_rows(LayerNormArgs a) {
 // g = dy act'(z) and xh of one element
 template <typename T, typename W>
 __device__ __forceinline__ void grad_terms(const LayerNormGradArgs& a, const T* x, const T* dy, float mean, float rstd, int c, float& g, float& xh) {
-  xh = __fmul_rn((float)x[c] - mean, rstd);
+  xh = rounded_mul((float)x[c] - mean, rstd);
   g = (float)dy[c];
   if (a.act != ACT_NONE) g *= row_act_grad(affine(xh, (const W*)a.gamma, (const W*)a.beta, c), a.act);
 }
@@ -512,12 +512,12 @@ __global__ __launch_bounds__(kRowThreads) void ln_tangent_rows(LayerNormTangentA
     for (int c = threadIdx.x; c < a.cols; c += kRowThreads) {
       const float t = a.tx[o + c];
       s[0] += t;
-      s[1] += t * __fmul_rn(a.x[o + c] - mean, rstd);
+      s[1] += t * rounded_mul(a.x[o + c] - mean, rstd);
     }
     team_sum<kRowThreads>(s, red);
     const float mt = s[0] / a.cols, b = s[1] / a.cols;
     for (int c = threadIdx.x; c < a.cols; c += kRowThreads) {
-      const float xh = __fmul_rn(a.x[o + c] - mean, rstd);
+      const float xh = rounded_mul(a.x[o + c] - mean, rstd);
       const float d = row_act_grad(affine(xh, a.gamma, a.beta, c), a.act);
       a.ty[o + c] = d * a.gamma[c] * (rstd * (a.tx[o + c] - mt - xh * b));
     }
@@ -531,7 +531,7 @@ __global__ __launch_bounds__(kRowThreads) void ln_tangent_bwd_rows(LayerNormTang
     const float mean = a.mean[r], rstd = a.rstd[r];
     float s[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
     for (int c = threadIdx.x; c < a.cols; c += kRowThreads) {
-      const float xh = __fmul_rn(a.x[o + c] - mean, rstd), t = a.tx[o + c];
+      const float xh = rounded_mul(a.x[o + c] - mean, rstd), t = a.tx[o + c];
       const float k = row_act_grad(affine(xh, a.gamma, a.beta, c), a.act) * a.gamma[c] * a.dty[o + c];
       s[0] += t;
       s[1] += t * xh;
@@ -543,7 +543,7 @@ __global__ __launch_bounds__(kRowThreads) void ln_tangent_bwd_rows(LayerNormTang
     const float n = 1.f / a.cols;
     const float mt = s[0] * n, b = s[1] * n, mk = s[2] * n, w = s[3] * n, q = s[4] * n - mk * mt;
     for (int c = threadIdx.x; c < a.cols; c += kRowThreads) {
-      const float xh = __fmul_rn(a.x[o + c] - mean, rstd);
+      const float xh = rounded_mul(a.x[o + c] - mean, rstd);
       const float k = row_act_grad(affine(xh, a.gamma, a.beta, c), a.act) * a.gamma[c] * a.dty[o + c];
       const float pk = rstd * (k - mk - xh * w), pt = rstd * (a.tx[o + c] - mt - xh * b);
       a.dtx[o + c] = (a.acc_t ? a.dtx[o + c] : 0.f) + pk;
@@ -567,14 +567,14 @@ __global__ __launch_bounds__(256) void ln_tangent_bwd_columns(LayerNormTangentAr
     for (int c = tid; c < a.cols; c += 256) {
       const float t = a.tx[o + c];
       s[0] += t;
-      s[1] += t * __fmul_rn(a.x[o + c] - mean, rstd);
+      s[1] += t * rounded_mul(a.x[o + c] - mean, rstd);
     }
     team_sum<256>(s, red);
     if (tid < 2) means[tid] = s[tid] / a.cols;
     __syncthreads();
     const float mt = means[0], b = means[1];
     for (int c = tid; c < a.cols; c += 256) {
-      const float xh = __fmul_rn(a.x[o + c] - mean, rstd);
+      const float xh = rounded_mul(a.x[o + c] - mean, rstd);
       const float v = row_act_grad(affine(xh, a.gamma, a.beta, c), a.act) * a.dty[o + c] * (rstd * (a.tx[o + c] - mt - xh * b));
       out[c] = (first ? 0.f : out[c]) + v;
     }
@@ -608,7 +608,7 @@ __global__ __launch_bounds__(kRowThreads) void quantize_kernel(QuantizeArgs a) {
     if (a.norm) row_statistics<T>(x, a.cols, a.eps, red, mean, rstd);
     auto value = [&](int c) {
       float v = (float)x[c];
-      if (a.norm) v = affine(__fmul_rn(v - mean, rstd), a.gamma, a.beta, c);
+      if (a.norm) v = affine(rounded_mul(v - mean, rstd), a.gamma, a.beta, c);
       return v;
     };
     float m = 0.f;

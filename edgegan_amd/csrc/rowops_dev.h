@@ -28,6 +28,11 @@ void by_type(int type, F f) {
   else f(f16_t{});
 }
 
+// A product that no following sum is contracted with into an fma: it is rounded by itself, wherever it is inlined.
+__device__ __forceinline__ float rounded_mul(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
 __device__ __forceinline__ float row_act(float z, int act) {
   return act == ACT_NONE ? z : z > 0.f ? z : act == ACT_LRELU ? 0.2f * z : (z != z ? z : 0.f);
 }
