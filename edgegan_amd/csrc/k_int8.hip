@@ -197,6 +197,84 @@ __global__ __launch_bounds__(WM * WN * 64) void int8_tiles(Int8Args a, int tiles
     }
 }
 
+// ---- few rows of a ----------------------------------------------------------------------------------------------------------------
+// Up to 16 MT rows: bound by the bytes of b. A block takes 16 NT rows of b, its eight waves k by turns of 128 bytes, eight loads of b a wave and turn of four
+// in flight; a comes from the caches.  The waves' sums are joined through LDS.
+constexpr int kFewWaves = 8;
+template <typename T, int MT, int NT>
+__global__ __launch_bounds__(kFewWaves * 64) void int8_few(Int8Args a) {
+  __shared__ int sums[kFewWaves][MT * NT * 4][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int l15 = lane & 15, lk = (lane >> 4) * 16;
+  const int j0 = blockIdx.x * 16 * NT;
+  const __amdgpu_buffer_rsrc_t ab = row_buffer(a.a, 0x7ffffff0u), bb = row_buffer(a.b + (long long)j0 * a.ldb, 0x7ffffff0u);
+  unsigned va[MT], vb[NT];
+#pragma unroll
+  for (int x = 0; x < MT; ++x) va[x] = (unsigned)min(x * 16 + l15, (int)a.m - 1) * (unsigned)a.lda + lk;
+#pragma unroll
+  for (int y = 0; y < NT; ++y) vb[y] = (unsigned)min(y * 16 + l15, a.n - 1 - j0) * (unsigned)a.ldb + lk;
+  i32x4 acc[MT][NT];
+#pragma unroll
+  for (int x = 0; x < MT; ++x)
+#pragma unroll
+    for (int y = 0; y < NT; ++y) acc[x][y] = i32x4{0, 0, 0, 0};
+  constexpr int U = MT * NT > 2 ? 2 : 4;   // turns at once
+  const int turn = kFewWaves * 128;
+  for (int k0 = wave * 128; k0 < a.k; k0 += U * turn) {
+    i32x4 fa[U][2][MT], fb[U][2][NT];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = k0 + u * turn + h * 64;
+        const unsigned off = k + lk < a.k ? k : 0x80000000u;   // (groups past k read as zeros)
+#pragma unroll
+        for (int y = 0; y < NT; ++y) fb[u][h][y] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(bb, vb[y] + off, 0, 0));
+#pragma unroll
+        for (int x = 0; x < MT; ++x) fa[u][h][x] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(ab, va[x] + off, 0, 0));
+      }
+    if ((a.k & 15) && k0 + (U - 1) * turn + 128 > a.k - 16) {   // this wave may hold the group that k ends in: a's bytes past it
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int ends = a.k - (k0 + u * turn + h * 64 + lk);
+#pragma unroll
+          for (int d = 0; d < 4; ++d) {
+            const int keep = min(max(ends - 4 * d, 0), 4), mask = keep == 4 ? -1 : (1 << (8 * keep)) - 1;
+#pragma unroll
+            for (int x = 0; x < MT; ++x) fa[u][h][x][d] &= mask;
+          }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int x = 0; x < MT; ++x)
+#pragma unroll
+          for (int y = 0; y < NT; ++y) acc[x][y] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fa[u][h][x], fb[u][h][y], acc[x][y], 0, 0, 0);
+  }
+#pragma unroll
+  for (int x = 0; x < MT; ++x)
+#pragma unroll
+    for (int y = 0; y < NT; ++y)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) sums[wave][(x * NT + y) * 4 + v][lane] = acc[x][y][v];
+  __syncthreads();
+  // result layout: lane l, register v: row 4 (l >> 4) + v, column l & 15
+  for (int o = wave; o < MT * NT * 4; o += kFewWaves) {
+    const int x = o / (NT * 4), y = o / 4 % NT, v = o % 4;
+    const int i = x * 16 + (lane >> 4) * 4 + v, j = j0 + y * 16 + l15;
+    if (i >= a.m || j >= a.n) continue;
+    int sum = 0;
+#pragma unroll
+    for (int w = 0; w < kFewWaves; ++w) sum += sums[w][o][lane];
+    ((T*)a.out)[i * a.ldo + j] = (T)int8_result(sum, a.a_scale[i], a.b_scale[j], a.bias ? a.bias[j] : 0.f);
+  }
+}
+
 size_t int8_partial_floats(long long m, int n, int k) { return 0; }
 
 void launch_int8_matmul(const Int8Args& given, int out_type, float* partial, hipStream_t s) {
@@ -216,6 +294,9 @@ void launch_int8_matmul(const Int8Args& given, int out_type, float* partial, hip
     using T = decltype(t);
     int tm, tn;
     if (al_a && al_b && a.lda <= 1 << 22 && a.ldb <= 1 << 22 && a.ldo <= 1 << 20 && a.k >= 16) {
+      if (a.m <= 16) return row_launch(int8_few<T, 1, 1>, dim3((a.n + 15) / 16), dim3(kFewWaves * 64), s, a);
+      if (a.m <= 32) return row_launch(int8_few<T, 2, 1>, dim3((a.n + 15) / 16), dim3(kFewWaves * 64), s, a);
+      if (a.m <= 64) return row_launch(int8_few<T, 4, 2>, dim3((a.n + 31) / 32), dim3(kFewWaves * 64), s, a);
       const long long big = ((a.m + 255) / 256) * ((a.n + 255) / 256);
       if (big >= 200) {
         const dim3 g = grid(256, 256, tm, tn);
