@@ -105,8 +105,8 @@ EXPORTS = ['eg_default_config', 'eg_variable_count', 'eg_variable_info', 'eg_cre
            'eg_train_step', 'eg_train_batch', 'eg_losses_wait', 'eg_read_losses', 'eg_eval_losses', 'eg_infer', 'eg_infer_upload', 'eg_infer_run', 'eg_infer_download', 'eg_sync', 'eg_comm_unique_id', 'eg_comm_init',
            'eg_comm_reduce_scalars', 'eg_comm_info', 'eg_comm_timing', 'eg_comm_timing_read',
            'eg_profile_begin', 'eg_profile_end', 'eg_profile_layers', 'eg_memory_stats', 'eg_mfma_probe', 'eg_test_op', 'eg_net_forward', 'eg_crc32c',
-           'eg_layer_norm', 'eg_layer_norm_workspace', 'eg_layer_norm_backward', 'eg_quantize_rows', 'eg_int8_matmul_workspace',
-           'eg_int8_matmul', 'eg_distill_loss_workspace', 'eg_distill_loss']
+           'eg_layer_norm', 'eg_layer_norm_workspace', 'eg_layer_norm_backward', 'eg_quantize_rows', 'eg_int8_matmul',
+           'eg_int8_linear_workspace', 'eg_int8_linear', 'eg_distill_loss_workspace', 'eg_distill_loss']
 
 _lib = None
 
@@ -165,11 +165,12 @@ def load_library() -> C.CDLL:
     lib.eg_layer_norm_workspace.argtypes = [n, n]
     lib.eg_layer_norm_backward.argtypes = [i, p, i, p, n, p, n, p, p, i, p, p, n, n, i, p, n, p, p, p, n]
     lib.eg_quantize_rows.argtypes = [i, p, i, p, n, i, p, p, f, n, n, p, n, p]
-    lib.eg_int8_matmul_workspace.argtypes = [n, n, n]
-    lib.eg_int8_matmul.argtypes = [i, p, p, n, p, p, n, p, p, n, n, n, i, p, n, p, n]
+    lib.eg_int8_matmul.argtypes = [i, p, p, n, p, p, n, p, p, n, n, n, i, p, n]
+    lib.eg_int8_linear_workspace.argtypes = [n, n]
+    lib.eg_int8_linear.argtypes = [i, p, i, p, n, i, p, p, f, p, n, p, p, n, n, n, i, p, n, p, n]
     lib.eg_distill_loss_workspace.argtypes = [n, n, n]
     lib.eg_distill_loss.argtypes = [i, p, i, p, n, i, p, n, p, n, p, n, n, n, f, p, p, n, p, n]
-    for name in ('eg_layer_norm_workspace', 'eg_int8_matmul_workspace', 'eg_distill_loss_workspace'):
+    for name in ('eg_layer_norm_workspace', 'eg_int8_linear_workspace', 'eg_distill_loss_workspace'):
         getattr(lib, name).restype = n
     _lib = lib
     return lib

@@ -198,12 +198,62 @@ __global__ __launch_bounds__(WM * WN * 64) void int8_tiles(Int8Args a, int tiles
 }
 
 // ---- few rows of a ----------------------------------------------------------------------------------------------------------------
-// Up to 16 MT rows: bound by the bytes of b. A block takes 16 NT rows of b, its eight waves k by turns of 128 bytes, eight loads of b a wave and turn of four
-// in flight; a comes from the caches.  The waves' sums are joined through LDS.
-constexpr int kFewWaves = 8;
+// Up to 16 MT rows: bound by the bytes of b. A block takes 16 NT rows of b, its eight waves k by turns of 128 bytes, eight or four loads of b a lane in
+// flight; a comes from the caches or, where it is quantised in the same launch, from LDS.  The waves' sums are joined through LDS.
+constexpr int kFewWaves = 8, kFewTurn = kFewWaves * 128;
+template <int MT, int NT>
+struct FewShape {
+  static constexpr int U = MT * NT > 2 ? 2 : 4;   // turns at once
+};
+template <int MT, int NT>
+__device__ __forceinline__ void few_request(__amdgpu_buffer_rsrc_t bb, const unsigned (&vb)[NT], int k0, int lk, int k_all, i32x4 (&fb)[FewShape<MT, NT>::U][2][NT]) {
+#pragma unroll
+  for (int u = 0; u < FewShape<MT, NT>::U; ++u)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int k = k0 + u * kFewTurn + h * 64;
+      const unsigned off = k + lk < k_all ? k : 0x80000000u;   // (groups past k read as zeros)
+#pragma unroll
+      for (int y = 0; y < NT; ++y) fb[u][h][y] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(bb, vb[y] + off, 0, 0));
+    }
+}
+template <int MT, int NT>
+__device__ __forceinline__ void few_products(const i32x4 (&fa)[FewShape<MT, NT>::U][2][MT], const i32x4 (&fb)[FewShape<MT, NT>::U][2][NT], i32x4 (&acc)[MT][NT]) {
+#pragma unroll
+  for (int u = 0; u < FewShape<MT, NT>::U; ++u)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int x = 0; x < MT; ++x)
+#pragma unroll
+        for (int y = 0; y < NT; ++y) acc[x][y] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fa[u][h][x], fb[u][h][y], acc[x][y], 0, 0, 0);
+}
+// joins the waves' sums and writes the block's outputs; a_scale of row i
+template <typename T, int MT, int NT, typename S>
+__device__ __forceinline__ void few_finish(const Int8Args& a, int (&sums)[kFewWaves][MT * NT * 4][64], const i32x4 (&acc)[MT][NT], int j0, int lane, int wave, S a_scale) {
+#pragma unroll
+  for (int x = 0; x < MT; ++x)
+#pragma unroll
+    for (int y = 0; y < NT; ++y)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) sums[wave][(x * NT + y) * 4 + v][lane] = acc[x][y][v];
+  __syncthreads();
+  // result layout: lane l, register v: row 4 (l >> 4) + v, column l & 15
+  for (int o = wave; o < MT * NT * 4; o += kFewWaves) {
+    const int x = o / (NT * 4), y = o / 4 % NT, v = o % 4;
+    const int i = x * 16 + (lane >> 4) * 4 + v, j = j0 + y * 16 + (lane & 15);
+    if (i >= a.m || j >= a.n) continue;
+    int sum = 0;
+#pragma unroll
+    for (int w = 0; w < kFewWaves; ++w) sum += sums[w][o][lane];
+    ((T*)a.out)[i * a.ldo + j] = (T)int8_result(sum, a_scale(i), a.b_scale[j], a.bias ? a.bias[j] : 0.f);
+  }
+}
+
 template <typename T, int MT, int NT>
 __global__ __launch_bounds__(kFewWaves * 64) void int8_few(Int8Args a) {
   __shared__ int sums[kFewWaves][MT * NT * 4][64];
+  constexpr int U = FewShape<MT, NT>::U;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l15 = lane & 15, lk = (lane >> 4) * 16;
   const int j0 = blockIdx.x * 16 * NT;
@@ -218,27 +268,24 @@ __global__ __launch_bounds__(kFewWaves * 64) void int8_few(Int8Args a) {
   for (int x = 0; x < MT; ++x)
 #pragma unroll
     for (int y = 0; y < NT; ++y) acc[x][y] = i32x4{0, 0, 0, 0};
-  constexpr int U = MT * NT > 2 ? 2 : 4;   // turns at once
-  const int turn = kFewWaves * 128;
-  for (int k0 = wave * 128; k0 < a.k; k0 += U * turn) {
+  for (int k0 = wave * 128; k0 < a.k; k0 += U * kFewTurn) {
     i32x4 fa[U][2][MT], fb[U][2][NT];
+    few_request<MT, NT>(bb, vb, k0, lk, a.k, fb);
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int k = k0 + u * turn + h * 64;
-        const unsigned off = k + lk < a.k ? k : 0x80000000u;   // (groups past k read as zeros)
-#pragma unroll
-        for (int y = 0; y < NT; ++y) fb[u][h][y] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(bb, vb[y] + off, 0, 0));
+        const int k = k0 + u * kFewTurn + h * 64;
+        const unsigned off = k + lk < a.k ? k : 0x80000000u;
 #pragma unroll
         for (int x = 0; x < MT; ++x) fa[u][h][x] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(ab, va[x] + off, 0, 0));
       }
-    if ((a.k & 15) && k0 + (U - 1) * turn + 128 > a.k - 16) {   // this wave may hold the group that k ends in: a's bytes past it
+    if ((a.k & 15) && k0 + (U - 1) * kFewTurn + 128 > a.k - 16) {   // this wave may hold the group that k ends in: a's bytes past it
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int ends = a.k - (k0 + u * turn + h * 64 + lk);
+          const int ends = a.k - (k0 + u * kFewTurn + h * 64 + lk);
 #pragma unroll
           for (int d = 0; d < 4; ++d) {
             const int keep = min(max(ends - 4 * d, 0), 4), mask = keep == 4 ? -1 : (1 << (8 * keep)) - 1;
@@ -247,37 +294,98 @@ __global__ __launch_bounds__(kFewWaves * 64) void int8_few(Int8Args a) {
           }
         }
     }
+    few_products<MT, NT>(fa, fb, acc);
+  }
+  few_finish<T, MT, NT>(a, sums, acc, j0, lane, wave, [&](int i) { return a.a_scale[i]; });
+}
+
+// The same for up to ROWS rows that are quantised here (behind their layer norm, if there is one): every block forms them for itself while its first loads of b are
+// in flight, which costs less than a launch in front.  A row is two halves of the block's work at a time: 256 threads with NV packs, as in
+// quantize_rows.
+template <typename T, int ROWS, int NV>
+__global__ __launch_bounds__(kFewWaves * 64) void int8_few_linear(Int8Args a, QuantizeArgs q) {
+  constexpr int V = 16 / sizeof(T), NT = 256, TURNS = (ROWS + 1) / 2, PITCH = NT * NV * V + 16, U = FewShape<1, 1>::U;
+  __shared__ int sums[kFewWaves][4][64];
+  __shared__ __attribute__((aligned(16))) unsigned char rows[ROWS][PITCH];
+  __shared__ double red[2][TURNS][centre_lds(NT)];
+  __shared__ float red_max[2][TURNS][NT / 64], scales[ROWS];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int l15 = lane & 15, lk = (lane >> 4) * 16;
+  const int j0 = blockIdx.x * 16;
+  const __amdgpu_buffer_rsrc_t bb = row_buffer(a.b + (long long)j0 * a.ldb, 0x7ffffff0u);
+  const unsigned vb[1] = {(unsigned)min(l15, a.n - 1 - j0) * (unsigned)a.ldb + lk};
+  i32x4 acc[1][1] = {{i32x4{0, 0, 0, 0}}};
+  i32x4 fa[U][2][1], fb[U][2][1];
+  few_request<1, 1>(bb, vb, wave * 128, lk, a.k, fb);
+
+  const int t = threadIdx.x & (NT - 1), side = wave >> 2;
+  float v[TURNS][NV][V];
+#pragma unroll
+  for (int n = 0; n < TURNS; ++n) {
+    const long long r = min((long long)(2 * n + side), a.m - 1);
+    const __amdgpu_buffer_rsrc_t xb = row_buffer((const T*)q.x + r * q.ldx, (unsigned)a.k * sizeof(T));
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const Pack<T, V> k = buffer_load<T, V>(xb, (i * NT + t) * V * sizeof(T));
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[n][i][j] = (float)k.e[j];
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < TURNS; ++n) {
+    if (q.norm) {
+      float mean, rstd, p[NV][V];
+      centre_row<NT, NV, V>(v[n], a.k, t, q.eps, red[side][n], mean, rstd);
+      load_parameter<float, NT, NV, V>(q.gamma, a.k, t, 1.f, p);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[n][i][j] = rounded_mul(rounded_mul(v[n][i][j], rstd), p[i][j]);
+      load_parameter<float, NT, NV, V>(q.beta, a.k, t, 0.f, p);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[n][i][j] = v[n][i][j] + p[i][j];
+    }
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) m = max_nan(m, (i * NT + t) * V < a.k ? fabsf(v[n][i][j]) : 0.f);
+    m = team_max<NT>(m, red_max[side][n]);
+    const double inv = quantize_factor(m);
+    const bool fine = quantizable(m);
+    const int r = 2 * n + side;
+    if (r < ROWS) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i * NT + t) * V;
+        Pack<unsigned char, V> k;
+#pragma unroll
+        for (int j = 0; j < V; ++j) k.e[j] = (unsigned char)(fine && c < a.k ? quantize1(v[n][i][j], inv) : 0u);
+        *reinterpret_cast<Pack<unsigned char, V>*>(&rows[r][c]) = k;
+      }
+      if (t == 0) scales[r] = quantize_scale(m);
+    }
+  }
+  __syncthreads();
+  const unsigned char* mine = rows[min(l15, ROWS - 1)];
+  for (int k0 = wave * 128; k0 < a.k; k0 += U * kFewTurn) {
+    if (k0 != wave * 128) few_request<1, 1>(bb, vb, k0, lk, a.k, fb);
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int x = 0; x < MT; ++x)
-#pragma unroll
-          for (int y = 0; y < NT; ++y) acc[x][y] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fa[u][h][x], fb[u][h][y], acc[x][y], 0, 0, 0);
+      for (int h = 0; h < 2; ++h) {
+        const int k = k0 + u * kFewTurn + h * 64 + lk;
+        fa[u][h][0] = *reinterpret_cast<const i32x4*>(mine + (k < a.k ? k : 0));   // (past k: anything, b's are zeros)
+      }
+    few_products<1, 1>(fa, fb, acc);
   }
-#pragma unroll
-  for (int x = 0; x < MT; ++x)
-#pragma unroll
-    for (int y = 0; y < NT; ++y)
-#pragma unroll
-      for (int v = 0; v < 4; ++v) sums[wave][(x * NT + y) * 4 + v][lane] = acc[x][y][v];
-  __syncthreads();
-  // result layout: lane l, register v: row 4 (l >> 4) + v, column l & 15
-  for (int o = wave; o < MT * NT * 4; o += kFewWaves) {
-    const int x = o / (NT * 4), y = o / 4 % NT, v = o % 4;
-    const int i = x * 16 + (lane >> 4) * 4 + v, j = j0 + y * 16 + l15;
-    if (i >= a.m || j >= a.n) continue;
-    int sum = 0;
-#pragma unroll
-    for (int w = 0; w < kFewWaves; ++w) sum += sums[w][o][lane];
-    ((T*)a.out)[i * a.ldo + j] = (T)int8_result(sum, a.a_scale[i], a.b_scale[j], a.bias ? a.bias[j] : 0.f);
-  }
+  few_finish<T, 1, 1>(a, sums, acc, j0, lane, wave, [&](int i) { return scales[i]; });
 }
 
-size_t int8_partial_floats(long long m, int n, int k) { return 0; }
 
-void launch_int8_matmul(const Int8Args& given, int out_type, float* partial, hipStream_t s) {
+void launch_int8_matmul(const Int8Args& given, int out_type, hipStream_t s) {
   Int8Args a = given;
   if (a.m == 0 || a.n == 0) return;
   if (a.m == 1) a.lda = (a.k + 15) & ~15;   // (a single row's distance to the next says nothing)
@@ -308,6 +416,42 @@ void launch_int8_matmul(const Int8Args& given, int out_type, float* partial, hip
     const dim3 g = grid(64, 64, tm, tn);
     row_launch(int8_any<T>, g, dim3(256), s, a, tn, al_a, al_b);
   });
+}
+
+static long long few_rows(int type, int k) {   // rows that int8_few_linear takes
+  const int packs = (k + 256 * (type == ROW_F32 ? 4 : 8) - 1) / (256 * (type == ROW_F32 ? 4 : 8));
+  return packs <= 2 ? 4 : packs <= 4 ? 2 : 0;
+}
+static long long linear_pitch(int k) { return (k + 15) & ~15; }
+size_t int8_linear_bytes(long long m, int k) { return ((size_t)m * linear_pitch(k) + 15) / 16 * 16 + (size_t)m * 4; }
+
+// quantize_rows and the product, in one launch where the rows are few
+void launch_int8_linear(const QuantizeArgs& given, const Int8Args& product, int type, int out_type, void* workspace, hipStream_t s) {
+  QuantizeArgs q = given;
+  Int8Args a = product;
+  if (a.m == 0 || a.n == 0) return;
+  const int elem = type == ROW_F32 ? 4 : 2;
+  const bool aligned = (uintptr_t)q.x % 16 == 0 && (a.m == 1 || q.ldx * elem % 16 == 0) && a.k % (16 / elem) == 0 && (uintptr_t)q.gamma % 16 == 0 && (uintptr_t)q.beta % 16 == 0 &&
+                       (uintptr_t)a.b % 16 == 0 && (a.n == 1 || a.ldb % 16 == 0) && a.ldb <= 1 << 22;
+  if (aligned && type == out_type && a.m <= few_rows(type, a.k)) {
+    by_type(type, [&](auto t) {
+      using T = decltype(t);
+      constexpr int V = 16 / sizeof(T);
+      const dim3 grid((a.n + 15) / 16), block(kFewWaves * 64);
+      if (a.m == 1 && a.k <= 256 * V * 2) row_launch(int8_few_linear<T, 1, 2>, grid, block, s, a, q);
+      else if (a.m <= 2 && a.k > 256 * V * 2) row_launch(int8_few_linear<T, 2, 4>, grid, block, s, a, q);
+      else row_launch(int8_few_linear<T, 4, 2>, grid, block, s, a, q);
+    });
+    return;
+  }
+  q.q = (signed char*)workspace;
+  q.ldq = linear_pitch(a.k);
+  q.scale = (float*)((char*)workspace + ((size_t)a.m * q.ldq + 15) / 16 * 16);
+  launch_quantize_rows(q, type, s);
+  a.a = q.q;
+  a.lda = q.ldq;
+  a.a_scale = q.scale;
+  launch_int8_matmul(a, out_type, s);
 }
 
 }  // namespace eg

@@ -8,21 +8,14 @@
 //
 // All of it is bound by HBM, so a row is read once: it stays in the registers of the team of threads that owns it (8 to 64 lanes of a
 // wave, 256 or 1,024 threads: row_team) between the statistics and the result.  A team of a wave needs no LDS and no barrier; a wider one joins its
-// waves' sums through LDS.  The mean is summed in 64 bits (it decides every x - m, and rows of one value then have xh = 0 exactly), the
-// squares and the gradient's sums in 32.  xh gamma + beta is formed by the same three rounded operations in the forward and the gradient (no
+// waves' sums through LDS.  The mean and the variance are summed in 64 bits (the mean decides every x - m, and a row of one value
+// then has xh = 0 exactly; and the statistics hardly ever depend on the team), the gradient's sums in 32.  xh gamma + beta is formed by the same three rounded operations in the forward and the gradient (no
 // contraction into an fma), so the gradient's sign of it is the forward's.
 #include <tuple>
 
 #include "rowops_dev.h"
 
 namespace eg {
-
-template <typename W>
-__device__ __forceinline__ float affine(float xh, const W* gamma, const W* beta, int c) {
-  const float z = gamma ? rounded_mul(xh, (float)gamma[c]) : xh;
-  return beta ? z + (float)beta[c] : z;
-}
-__device__ __forceinline__ float affine_r(float xh, float gamma, float beta) { return rounded_mul(xh, gamma) + beta; }
 
 // ---- rows in registers -------------------------------------------------------------------------------------------------------
 // NT threads own a row, each NV packs of V consecutive elements: pack i of thread t begins at column (i NT + t) V.
@@ -53,25 +46,6 @@ __device__ __forceinline__ void take_row(const Pack<T, V> (&k)[NV], int cols, in
 #pragma unroll
     for (int j = 0; j < V; ++j) v[i][j] = (i * NT + t) * V < cols ? (float)k[i].e[j] : 0.f;
 }
-template <typename W, int NT, int NV, int V>
-__device__ __forceinline__ void load_parameter(const W* p, int cols, int t, float missing, float (&v)[NV][V]) {
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int at = (i * NT + t) * V, c = at < cols ? at : 0;
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[i][j] = missing;
-    if (p) {
-      if constexpr (V * sizeof(W) <= 16) load_pack<W, V>(p + c, v[i]);
-      else {   // (16-bit rows with 32-bit parameters: two loads)
-        float lo[V / 2], hi[V / 2];
-        load_pack<W, V / 2>(p + c, lo);
-        load_pack<W, V / 2>(p + c + V / 2, hi);
-#pragma unroll
-        for (int j = 0; j < V / 2; ++j) v[i][j] = lo[j], v[i][j + V / 2] = hi[j];
-      }
-    }
-  }
-}
 template <typename T, int NT, int NV, int V>
 __device__ __forceinline__ void store_row(T* p, int cols, int t, const float (&v)[NV][V]) {
 #pragma unroll
@@ -80,29 +54,6 @@ __device__ __forceinline__ void store_row(T* p, int cols, int t, const float (&v
     if (c < cols) store_pack<T, V>(p + c, v[i]);
   }
 }
-// mean (f64 sum) and rstd of a row in registers; the row becomes x - mean
-template <int NT, int NV, int V>
-__device__ __forceinline__ void centre_row(float (&v)[NV][V], int cols, int t, float eps, double* red, float& mean, float& rstd) {
-  double s[1] = {0.};
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int j = 0; j < V; ++j) s[0] += (double)v[i][j];
-  team_sum<NT>(s, red);
-  mean = (float)(s[0] / cols);
-  float d[1] = {0.f};
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      v[i][j] = (i * NT + t) * V < cols ? v[i][j] - mean : 0.f;
-      d[0] += v[i][j] * v[i][j];
-    }
-  team_sum<NT>(d, reinterpret_cast<float*>(red + NT / 64));
-  rstd = 1.f / sqrtf(d[0] / cols + eps);
-}
-constexpr int centre_lds(int nt) { return nt > 64 ? 2 * nt / 64 : 1; }   // doubles
-
 template <typename T, typename W, int NT, int NV, int V>
 __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_fwd(LayerNormArgs a) {
   constexpr int NB = NT > 256 ? NT : 256, TEAMS = NB / NT;
@@ -259,19 +210,6 @@ __global__ __launch_bounds__(1024) void ln_bwd_finish(const float* partial, int 
   *out = (W)s;
 }
 
-// The whole number nearest to 127 v / amax, exactly: inv = 127 / amax in 64 bits; v inv + 98304 is rounded once (fma) to a multiple of
-// 2^-36, where a true tie lands on the tie (the product is off by under 2^-45) and nothing else does (127 v / amax is at least 2^-33 from a
-// border that it is not on: with x's last bit u >= 2^-32 amax, 254 v - odd amax is a multiple of u).  Adding 1.5 2^52 then rounds to whole numbers, ties to even, and the
-// sum's low byte is the signed 8-bit result (98304 = 0x18000).
-__device__ __forceinline__ unsigned quantize1(float v, double inv) {
-  const double t = __builtin_fma((double)v, inv, 98304.0) + 6755399441055744.0;
-  return (unsigned)__double2loint(t) & 0xffu;
-}
-// false for infinity and NaN: such a row's scale is NaN, its values zero
-__device__ __forceinline__ bool quantizable(float amax) { return amax <= 3.4028235e38f; }
-__device__ __forceinline__ double quantize_factor(float amax) { return quantizable(amax) && amax > 0.f ? 127.0 / (double)amax : 0.0; }
-__device__ __forceinline__ float quantize_scale(float amax) { return quantizable(amax) ? amax / 127.f : __builtin_nanf(""); }
-
 template <typename T, int NT, int NV, int V>
 __global__ __launch_bounds__(NT > 256 ? NT : 256) void quantize_rows(QuantizeArgs a) {
   constexpr int NB = NT > 256 ? NT : 256, TEAMS = NB / NT;
@@ -327,13 +265,13 @@ __device__ __forceinline__ void row_statistics(const T* x, int cols, float eps, 
   for (int c = threadIdx.x; c < cols; c += kRowThreads) s[0] += (double)(float)x[c];
   team_sum<kRowThreads>(s, red);
   mean = (float)(s[0] / cols);
-  float d[1] = {0.f};
+  s[0] = 0.;
   for (int c = threadIdx.x; c < cols; c += kRowThreads) {
     const float u = (float)x[c] - mean;
-    d[0] += u * u;
+    s[0] += (double)u * u;
   }
-  team_sum<kRowThreads>(d, reinterpret_cast<float*>(red + kRowThreads / 64));
-  rstd = 1.f / sqrtf(d[0] / cols + eps);
+  team_sum<kRowThreads>(s, red + kRowThreads / 64);
+  rstd = 1.f / sqrtf((float)(s[0] / cols) + eps);
 }
 
 template <typename T, typename W>

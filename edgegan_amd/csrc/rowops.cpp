@@ -137,14 +137,8 @@ static void check_product(long long m, long long n, long long k) {
   EG_CHECK(k <= 131071, "int8 product: %lld terms can overflow a 32-bit sum (at most 131071)", k);
 }
 
-long long eg_int8_matmul_workspace(long long m, long long n, long long k) {
-  if (m < 0 || n < 0 || k < 0 || n >= (1ll << 30) || k > 131071) return -1;
-  return (long long)int8_partial_floats(m, (int)n, (int)k) * 4;
-}
-
 int eg_int8_matmul(int device, void* stream, const signed char* a, long long lda, const float* a_scale, const signed char* b, long long ldb,
-                   const float* b_scale, const float* bias, long long m, long long n, long long k, int out_type, void* out, long long ldo,
-                   void* workspace, long long workspace_bytes) {
+                   const float* b_scale, const float* bias, long long m, long long n, long long k, int out_type, void* out, long long ldo) {
   return entry([&] {
     type_of(out_type, "eg_int8_matmul");
     check_product(m, n, k);
@@ -153,9 +147,35 @@ int eg_int8_matmul(int device, void* stream, const signed char* a, long long lda
     check_matrix("eg_int8_matmul out", out, ldo, m, n, bytes_of(out_type));
     if (m == 0 || n == 0) return;
     EG_CHECK(a_scale && b_scale, "eg_int8_matmul: null scale");
-    check_workspace("eg_int8_matmul", workspace, workspace_bytes, int8_partial_floats(m, (int)n, (int)k));
     OnDevice on(device);
-    launch_int8_matmul({a, lda, a_scale, b, ldb, b_scale, bias, m, (int)n, (int)k, out, ldo}, out_type, (float*)workspace, (hipStream_t)stream);
+    launch_int8_matmul({a, lda, a_scale, b, ldb, b_scale, bias, m, (int)n, (int)k, out, ldo}, out_type, (hipStream_t)stream);
+  });
+}
+
+long long eg_int8_linear_workspace(long long rows, long long inner) {
+  if (rows < 0 || inner < 0 || inner > 131071) return -1;
+  return (long long)int8_linear_bytes(rows, (int)inner);
+}
+
+int eg_int8_linear(int device, void* stream, int dtype, const void* x, long long ldx, int norm, const float* gamma, const float* beta, float eps,
+                   const signed char* weight, long long ldw, const float* weight_scale, const float* bias, long long rows, long long cols, long long inner,
+                   int out_type, void* out, long long ldo, void* workspace, long long workspace_bytes) {
+  return entry([&] {
+    type_of(dtype, "eg_int8_linear");
+    type_of(out_type, "eg_int8_linear");
+    check_product(rows, cols, inner);
+    check_matrix("eg_int8_linear x", x, ldx, rows, inner, bytes_of(dtype));
+    check_matrix("eg_int8_linear weight", weight, ldw, cols, inner, 1);
+    check_matrix("eg_int8_linear out", out, ldo, rows, cols, bytes_of(out_type));
+    EG_CHECK(norm || (!gamma && !beta), "eg_int8_linear: gamma and beta belong to the norm");
+    if (norm) check_eps(eps);
+    if (rows == 0 || cols == 0) return;
+    EG_CHECK(inner > 0, "eg_int8_linear: rows without columns");
+    EG_CHECK(weight_scale, "eg_int8_linear: null scale");
+    check_workspace("eg_int8_linear", workspace, workspace_bytes, int8_linear_bytes(rows, (int)inner) / 4);
+    OnDevice on(device);
+    launch_int8_linear({x, ldx, gamma, beta, norm != 0, eps, rows, (int)inner, nullptr, 0, nullptr},
+                       {nullptr, 0, nullptr, weight, ldw, weight_scale, bias, rows, (int)cols, (int)inner, out, ldo}, dtype, out_type, workspace, (hipStream_t)stream);
   });
 }
 

@@ -100,8 +100,9 @@ void launch_layer_norm_backward(const LayerNormGradArgs& a, int type, int wtype,
 void launch_layer_norm_tangent(const LayerNormTangentArgs& a, hipStream_t s);
 void launch_layer_norm_tangent_backward(const LayerNormTangentArgs& a, hipStream_t s);
 void launch_quantize_rows(const QuantizeArgs& a, int type, hipStream_t s);
-size_t int8_partial_floats(long long m, int n, int k);
-void launch_int8_matmul(const Int8Args& a, int out_type, float* partial, hipStream_t s);
+void launch_int8_matmul(const Int8Args& a, int out_type, hipStream_t s);
+size_t int8_linear_bytes(long long m, int k);
+void launch_int8_linear(const QuantizeArgs& q, const Int8Args& a, int type, int out_type, void* workspace, hipStream_t s);
 size_t distill_partial_floats(long long rows, int cols, int top);
 void launch_distill(const DistillArgs& a, int type, hipStream_t s);
 

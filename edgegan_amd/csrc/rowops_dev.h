@@ -96,7 +96,8 @@ __device__ __forceinline__ float lanes_max(float v) {
     return v;
 }
 
-// Sum / maximum over the NT threads that share a row: neighbouring lanes, or (NT > 64) the whole block through red[NT / 64].  Calls that follow one
+// Sum / maximum over the NT threads that share a row: neighbouring lanes, or (NT > 64) waves through red[NT / 64]: every
+// thread of the block has to come by, and teams of the same block have a `red` each.  Calls that follow one
 // another use other memory, or a barrier lies between them.
 template <int NT, typename V, int N>
 __device__ __forceinline__ void team_sum(V (&v)[N], V* red) {
@@ -106,7 +107,7 @@ __device__ __forceinline__ void team_sum(V (&v)[N], V* red) {
     constexpr int NW = NT / 64;
     if ((threadIdx.x & 63) == 0)
 #pragma unroll
-      for (int i = 0; i < N; ++i) red[i * NW + (threadIdx.x >> 6)] = v[i];
+      for (int i = 0; i < N; ++i) red[i * NW + (threadIdx.x >> 6) % NW] = v[i];
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -122,7 +123,7 @@ __device__ __forceinline__ float team_max(float v, float* red) {
   v = lanes_max<(NT < 64 ? NT : 64)>(v);
   if constexpr (NT > 64) {
     constexpr int NW = NT / 64;
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0) red[(threadIdx.x >> 6) % NW] = v;
     __syncthreads();
     v = red[0];
 #pragma unroll
@@ -177,5 +178,69 @@ __device__ __forceinline__ int fresh(int v) {
   asm volatile("" : "+v"(v));
   return v;
 }
+
+// ---- what the layer norm, the quantisation and the 8-bit layer for few rows share -----------------------------------------------------
+template <typename W>
+__device__ __forceinline__ float affine(float xh, const W* gamma, const W* beta, int c) {
+  const float z = gamma ? rounded_mul(xh, (float)gamma[c]) : xh;
+  return beta ? z + (float)beta[c] : z;
+}
+__device__ __forceinline__ float affine_r(float xh, float gamma, float beta) { return rounded_mul(xh, gamma) + beta; }
+
+// A vector of parameters in the order of a row: NT threads, each NV packs of V consecutive elements, pack i of thread t beginning at column (i NT + t) V.
+template <typename W, int NT, int NV, int V>
+__device__ __forceinline__ void load_parameter(const W* p, int cols, int t, float missing, float (&v)[NV][V]) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int at = (i * NT + t) * V, c = at < cols ? at : 0;
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[i][j] = missing;
+    if (p) {
+      if constexpr (V * sizeof(W) <= 16) load_pack<W, V>(p + c, v[i]);
+      else {   // (16-bit rows with 32-bit parameters: two loads)
+        float lo[V / 2], hi[V / 2];
+        load_pack<W, V / 2>(p + c, lo);
+        load_pack<W, V / 2>(p + c + V / 2, hi);
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) v[i][j] = lo[j], v[i][j + V / 2] = hi[j];
+      }
+    }
+  }
+}
+// mean (f64 sum) and rstd of a row in registers; the row becomes x - mean
+template <int NT, int NV, int V>
+__device__ __forceinline__ void centre_row(float (&v)[NV][V], int cols, int t, float eps, double* red, float& mean, float& rstd) {
+  double s[1] = {0.};
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) s[0] += (double)v[i][j];
+  team_sum<NT>(s, red);
+  mean = (float)(s[0] / cols);
+  s[0] = 0.;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      v[i][j] = (i * NT + t) * V < cols ? v[i][j] - mean : 0.f;
+      s[0] += (double)v[i][j] * v[i][j];
+    }
+  team_sum<NT>(s, red + NT / 64);
+  rstd = 1.f / sqrtf((float)(s[0] / cols) + eps);
+}
+constexpr int centre_lds(int nt) { return nt > 64 ? 2 * nt / 64 : 1; }   // doubles
+
+// The whole number nearest to 127 v / amax, exactly: inv = 127 / amax in 64 bits; v inv + 98304 is rounded once (fma) to a multiple of
+// 2^-36, where a true tie lands on the tie (the product is off by under 2^-45) and nothing else does (127 v / amax is at least 2^-33 from a
+// border that it is not on: with x's last bit u >= 2^-32 amax, 254 v - odd amax is a multiple of u).  Adding 1.5 2^52 then rounds to whole numbers, ties to even, and the
+// sum's low byte is the signed 8-bit result (98304 = 0x18000).
+__device__ __forceinline__ unsigned quantize1(float v, double inv) {
+  const double t = __builtin_fma((double)v, inv, 98304.0) + 6755399441055744.0;
+  return (unsigned)__double2loint(t) & 0xffu;
+}
+// false for infinity and NaN: such a row's scale is NaN, its values zero
+__device__ __forceinline__ bool quantizable(float amax) { return amax <= 3.4028235e38f; }
+__device__ __forceinline__ double quantize_factor(float amax) { return quantizable(amax) && amax > 0.f ? 127.0 / (double)amax : 0.0; }
+__device__ __forceinline__ float quantize_scale(float amax) { return quantizable(amax) ? amax / 127.f : __builtin_nanf(""); }
 
 }  // namespace eg

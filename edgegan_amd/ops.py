@@ -204,17 +204,35 @@ def int8_matmul(q: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, weig
     if s is None or ws is None:
         _refuse('scale, weight_scale: required')
     out = torch.empty(q.shape[:-1] + (n,), dtype=out_dtype, device=q.device)
-    keep, wp, size = _workspace(lib.eg_int8_matmul_workspace(m, n, k), q)
     device, stream = _stream(q)
-    _check(lib.eg_int8_matmul(device, stream, q.data_ptr(), lda, s, weight.data_ptr(), ldb, ws, b, m, n, k, _TYPES[out_dtype], out.data_ptr(), n, wp, size))
+    _check(lib.eg_int8_matmul(device, stream, q.data_ptr(), lda, s, weight.data_ptr(), ldb, ws, b, m, n, k, _TYPES[out_dtype], out.data_ptr(), n))
     return out
 
 
 def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias: Optional[torch.Tensor] = None, norm=None,
                 out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-    """A linear layer in 8-bit integers: int8_matmul(*quantize_rows(x, norm), weight, weight_scale, bias), in x's type unless out_dtype says otherwise."""
-    q, scale = quantize_rows(x, norm)
-    return int8_matmul(q, scale, weight, weight_scale, bias, out_dtype or x.dtype)
+    """A linear layer in 8-bit integers: int8_matmul(*quantize_rows(x, norm), weight, weight_scale, bias), in x's type unless out_dtype says otherwise; for few rows
+    one launch."""
+    lib = _lib or _library()
+    f32 = (torch.float32,)
+    m, k, ld = _rows(x, 'x')
+    on, g, beta, eps = _norm_parameters(norm, k, x)
+    n, kw, ldw = _rows(weight, 'weight', (torch.int8,))
+    if weight.dim() != 2 or weight.device != x.device or kw != k:
+        _refuse(f'weight: [n, {k}] on {x.device} is required, not {tuple(weight.shape)} on {weight.device}')
+    if out_dtype is None:
+        out_dtype = x.dtype
+    elif out_dtype not in _TYPES:
+        _refuse(f'out_dtype: {out_dtype} is not one of {", ".join(str(t) for t in _TYPES)}')
+    ws, b = _vector(weight_scale, n, 'weight_scale', x, f32), _vector(bias, n, 'bias', x, f32)
+    if ws is None:
+        _refuse('weight_scale: required')
+    out = torch.empty(x.shape[:-1] + (n,), dtype=out_dtype, device=x.device)
+    keep, wp, size = _workspace(lib.eg_int8_linear_workspace(m, k), x)
+    device, stream = _stream(x)
+    _check(lib.eg_int8_linear(device, stream, _TYPES[x.dtype], x.data_ptr(), ld, on, g, beta, eps, weight.data_ptr(), ldw, ws, b, m, n, k, _TYPES[out_dtype],
+                              out.data_ptr(), n, wp, size))
+    return out
 
 
 def distill_loss(logits: torch.Tensor, index: torch.Tensor, teacher: torch.Tensor, temperature: float = 1.0,

@@ -237,11 +237,17 @@ int eg_layer_norm_backward(int device, void* stream, int dtype, const void* dy, 
 int eg_quantize_rows(int device, void* stream, int dtype, const void* x, long long ldx, int norm, const float* gamma, const float* beta,
                      float eps, long long rows, long long cols, signed char* q, long long ldq, float* scale);
 /* out[i][j] = (sum_k a[i][k] b[j][k]) a_scale[i] b_scale[j] + bias[j]: a [m x k] a scale for each row (token, position), b [n x k] one for
- * each output channel; 32-bit integer sums (k <= 131071).  bias f32 or NULL. */
-long long eg_int8_matmul_workspace(long long m, long long n, long long k);
+ * each output channel; 32-bit integer sums (k <= 131071).  bias f32 or NULL.  Where rows begin at multiples of 16 bytes, the
+ * 16-byte group that k ends in is read whole (and what lies past k there ignored). */
 int eg_int8_matmul(int device, void* stream, const signed char* a, long long lda, const float* a_scale, const signed char* b,
                    long long ldb, const float* b_scale, const float* bias, long long m, long long n, long long k, int out_type,
-                   void* out, long long ldo, void* workspace, long long workspace_bytes);
+                   void* out, long long ldo);
+/* A linear layer in 8-bit integers: eg_quantize_rows of x [rows x inner] and eg_int8_matmul with weight [cols x inner], the same numbers,
+ * for few rows in one launch. The workspace holds the quantised rows (bytes: eg_int8_linear_workspace, -1 for bad sizes). */
+long long eg_int8_linear_workspace(long long rows, long long inner);
+int eg_int8_linear(int device, void* stream, int dtype, const void* x, long long ldx, int norm, const float* gamma, const float* beta,
+                   float eps, const signed char* weight, long long ldw, const float* weight_scale, const float* bias, long long rows,
+                   long long cols, long long inner, int out_type, void* out, long long ldo, void* workspace, long long workspace_bytes);
 /* Distillation from a teacher's top logits: p = softmax(teacher / T) over the `top` (<= 1024) kept logits of a row, q = softmax(logits / T);
  * loss[r] = w_r T^2 sum_k p_k (log p_k - log q_index[k]); grad (or NULL) = d(sum of loss) / d(logits).  index: 4- or 8-byte integers;
  * one outside [0, cols) is padding, one given twice counts twice.  row_weight f32 [rows] or NULL (1): a row of weight 0 or without a kept

@@ -26,7 +26,11 @@ def quantize(lib, rows=2, cols=8, q=P, ldq=16, scale=P, norm=0, gamma=None, eps=
 
 
 def product(lib, a=P, lda=64, sa=P, m=4, n=4, k=64, out_type=0, ldo=4):
-    return lib.eg_int8_matmul(0, None, a, lda, sa, P, 64, P, None, m, n, k, out_type, P, ldo, None, 0)
+    return lib.eg_int8_matmul(0, None, a, lda, sa, P, 64, P, None, m, n, k, out_type, P, ldo)
+
+
+def linear(lib, dtype=0, x=P, ldx=64, norm=0, gamma=None, eps=1e-5, w=P, ldw=64, ws=P, rows=2, cols=4, inner=64, out_type=0, out=P, ldo=4, work=P, size=1 << 20):
+    return lib.eg_int8_linear(0, None, dtype, x, ldx, norm, gamma, None, eps, w, ldw, ws, None, rows, cols, inner, out_type, out, ldo, work, size)
 
 
 def distill(lib, rows=2, cols=8, top=3, t=1.0, loss=P, index_bytes=8, index=P, ldi=3, ldg=8):
@@ -44,6 +48,9 @@ CASES = [
     (quantize, dict(norm=1, eps=-1.0), 'eps'), (quantize, dict(cols=0), 'without columns'),
     (product, dict(k=131072, lda=131072), 'overflow'), (product, dict(m=-1), 'sizes'), (product, dict(n=1 << 30), 'sizes'), (product, dict(a=None), 'null'), (product, dict(lda=63), 'elements apart'),
     (product, dict(sa=None), 'scale'), (product, dict(out_type=7), 'type'), (product, dict(ldo=3), 'elements apart'),
+    (linear, dict(dtype=9), 'type'), (linear, dict(x=None), 'null'), (linear, dict(ldx=63), 'elements apart'), (linear, dict(gamma=P), 'norm'), (linear, dict(norm=1, eps=0.0), 'eps'),
+    (linear, dict(w=None), 'null'), (linear, dict(ldw=1), 'elements apart'), (linear, dict(ws=None), 'scale'), (linear, dict(inner=0), 'without columns'), (linear, dict(inner=1 << 17, ldx=1 << 17, ldw=1 << 17), 'overflow'),
+    (linear, dict(work=None), 'workspace'), (linear, dict(size=100), 'workspace'), (linear, dict(out=None), 'null'), (linear, dict(ldo=2), 'elements apart'), (linear, dict(rows=-1), 'sizes'),
     (distill, dict(top=1025, ldi=1025), 'teacher logits'), (distill, dict(t=0.0), 'temperature'), (distill, dict(t=float('nan')), 'temperature'), (distill, dict(t=1e-45), 'temperature'),
     (distill, dict(loss=None), 'loss'), (distill, dict(index_bytes=2), 'bytes'), (distill, dict(index=P + 4), 'misaligned'), (distill, dict(ldi=2), 'elements apart'), (distill, dict(ldg=7), 'elements apart'),
     (distill, dict(cols=0), 'without columns'),
@@ -62,12 +69,13 @@ def test_nothing_to_do_is_no_error(built_lib):
     assert quantize(built_lib, rows=0) == 0
     assert product(built_lib, m=0, a=None) == 0
     assert distill(built_lib, rows=0) == 0
+    assert linear(built_lib, rows=0, x=None) == 0 and linear(built_lib, cols=0, w=None) == 0
 
 
 def test_workspace_sizes(built_lib):
     assert built_lib.eg_layer_norm_workspace(-1, 8) == -1 and built_lib.eg_layer_norm_workspace(8, (1 << 24) + 1) == -1
     assert built_lib.eg_layer_norm_workspace(0, 8) == 0
-    assert built_lib.eg_int8_matmul_workspace(1, 1, 131072) == -1 and built_lib.eg_int8_matmul_workspace(1, 4096, 4096) >= 0
+    assert built_lib.eg_int8_linear_workspace(1, 131072) == -1 and built_lib.eg_int8_linear_workspace(3, 100) >= 3 * 116
     assert built_lib.eg_distill_loss_workspace(1, -1, 1) == -1 and built_lib.eg_distill_loss_workspace(1, 8, 1025) == -1
     assert built_lib.eg_distill_loss_workspace(4, 1000, 8) >= 0
 
