@@ -316,9 +316,14 @@ __global__ __launch_bounds__(kFewWaves * 64) void int8_few_linear(Int8Args a, Qu
   const unsigned vb[1] = {(unsigned)min(l15, a.n - 1 - j0) * (unsigned)a.ldb + lk};
   i32x4 acc[1][1] = {{i32x4{0, 0, 0, 0}}};
   i32x4 fa[U][2][1], fb[U][2][1];
-  few_request<1, 1>(bb, vb, wave * 128, lk, a.k, fb);
 
+  // the rows and the norm's parameters before b: loads arrive in order, and they are what the next lines wait for
   const int t = threadIdx.x & (NT - 1), side = wave >> 2;
+  float gamma[NV][V], beta[NV][V];
+  if (q.norm) {
+    load_parameter<float, NT, NV, V>(q.gamma, a.k, t, 1.f, gamma);
+    load_parameter<float, NT, NV, V>(q.beta, a.k, t, 0.f, beta);
+  }
   float v[TURNS][NV][V];
 #pragma unroll
   for (int n = 0; n < TURNS; ++n) {
@@ -331,21 +336,17 @@ __global__ __launch_bounds__(kFewWaves * 64) void int8_few_linear(Int8Args a, Qu
       for (int j = 0; j < V; ++j) v[n][i][j] = (float)k.e[j];
     }
   }
+  few_request<1, 1>(bb, vb, wave * 128, lk, a.k, fb);
+  __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (int n = 0; n < TURNS; ++n) {
     if (q.norm) {
-      float mean, rstd, p[NV][V];
+      float mean, rstd;
       centre_row<NT, NV, V>(v[n], a.k, t, q.eps, red[side][n], mean, rstd);
-      load_parameter<float, NT, NV, V>(q.gamma, a.k, t, 1.f, p);
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[n][i][j] = rounded_mul(rounded_mul(v[n][i][j], rstd), p[i][j]);
-      load_parameter<float, NT, NV, V>(q.beta, a.k, t, 0.f, p);
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[n][i][j] = v[n][i][j] + p[i][j];
+        for (int j = 0; j < V; ++j) v[n][i][j] = affine_r(rounded_mul(v[n][i][j], rstd), gamma[i][j], beta[i][j]);
     }
     float m = 0.f;
 #pragma unroll

@@ -8,8 +8,8 @@
 //
 // All of it is bound by HBM, so a row is read once: it stays in the registers of the team of threads that owns it (8 to 64 lanes of a
 // wave, 256 or 1,024 threads: row_team) between the statistics and the result.  A team of a wave needs no LDS and no barrier; a wider one joins its
-// waves' sums through LDS.  The mean and the variance are summed in 64 bits (the mean decides every x - m, and a row of one value
-// then has xh = 0 exactly; and the statistics hardly ever depend on the team), the gradient's sums in 32.  xh gamma + beta is formed by the same three rounded operations in the forward and the gradient (no
+// waves' sums through LDS.  The mean and the variance are summed in 64 bits, packs of a thread pairwise in 32 (the
+// mean decides every x - m, and a row of one value has xh = 0 exactly; and the statistics hardly ever depend on the team), the gradient's sums in 32.  xh gamma + beta is formed by the same three rounded operations in the forward and the gradient (no
 // contraction into an fma), so the gradient's sign of it is the forward's.
 #include <tuple>
 

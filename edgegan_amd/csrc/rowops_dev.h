@@ -207,24 +207,36 @@ __device__ __forceinline__ void load_parameter(const W* p, int cols, int t, floa
     }
   }
 }
-// mean (f64 sum) and rstd of a row in registers; the row becomes x - mean
+// pairwise: of equal values exactly
+template <int V>
+__device__ __forceinline__ float tree_sum(const float (&v)[V]) {
+  if constexpr (V == 1) return v[0];
+  else {
+    float h[V / 2];
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) h[i] = v[2 * i] + v[2 * i + 1];
+    return tree_sum(h);
+  }
+}
+// mean and rstd of a row in registers, packs summed in f32 and their sums in f64; the row becomes x - mean
 template <int NT, int NV, int V>
 __device__ __forceinline__ void centre_row(float (&v)[NV][V], int cols, int t, float eps, double* red, float& mean, float& rstd) {
   double s[1] = {0.};
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int j = 0; j < V; ++j) s[0] += (double)v[i][j];
+  for (int i = 0; i < NV; ++i) s[0] += (double)tree_sum(v[i]);
   team_sum<NT>(s, red);
   mean = (float)(s[0] / cols);
   s[0] = 0.;
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV; ++i) {
+    float sq[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       v[i][j] = (i * NT + t) * V < cols ? v[i][j] - mean : 0.f;
-      s[0] += (double)v[i][j] * v[i][j];
+      sq[j] = rounded_mul(v[i][j], v[i][j]);   // (the same wherever it is inlined)
     }
+    s[0] += (double)tree_sum(sq);
+  }
   team_sum<NT>(s, red + NT / 64);
   rstd = 1.f / sqrtf((float)(s[0] / cols) + eps);
 }

@@ -8,10 +8,12 @@ captured into a graph.  The last dimension is the row; the dimensions before it 
 view is not).  Every refusal raises EdgeGANLibError.  There is no autograd: the gradient calls are explicit, as everywhere in this package."""
 from __future__ import annotations
 
+import math
 import sys
 from typing import Optional, Tuple
 
 import torch
+from torch._C import _cuda_getCurrentRawStream as _stream   # torch.cuda.current_stream(device).cuda_stream without the object
 
 from ._lib import EdgeGANLibError, load_library
 
@@ -45,43 +47,45 @@ def _rows(x: torch.Tensor, name: str, types=_TYPES) -> Tuple[int, int, int]:
         _refuse(f'{name}: a tensor on the GPU is required')
     if x.dtype not in types:
         _refuse(f'{name}: {x.dtype} is not one of {", ".join(str(t) for t in types)}')
-    shape, stride = x.shape, x.stride()
-    if len(shape) == 0:
+    shape = x.shape
+    n = len(shape)
+    if n == 0:
         _refuse(f'{name}: at least one dimension is required')
     cols = shape[-1]
+    if x.is_contiguous():
+        return (shape[0] if n == 2 else 1 if n == 1 else math.prod(shape[:-1])), cols, cols
+    stride = x.stride()
     if cols > 1 and stride[-1] != 1:
         _refuse(f'{name}: the last dimension has to be consecutive (stride {stride[-1]})')
-    if len(shape) == 2:
-        rows = shape[0]
-        ld = stride[0] if rows > 1 else cols
-    elif len(shape) == 1:
-        return 1, cols, cols
-    else:
-        rows, ld = 1, cols
-        for n, s in zip(reversed(shape[:-1]), reversed(stride[:-1])):
-            if n == 1:
-                continue
-            if rows == 1:
-                ld = s
-            elif s != ld * rows:
-                _refuse(f'{name}: dimensions {tuple(shape[:-1])} with strides {tuple(stride[:-1])} are not rows one stride apart')
-            rows *= n
+    rows, ld = 1, cols
+    for i in range(n - 2, -1, -1):
+        if shape[i] == 1:
+            continue
+        if rows == 1:
+            ld = stride[i]
+        elif stride[i] != ld * rows:
+            _refuse(f'{name}: dimensions {tuple(shape[:-1])} with strides {tuple(stride[:-1])} are not rows one stride apart')
+        rows *= shape[i]
     if rows > 1 and ld < cols:
         _refuse(f'{name}: rows {ld} elements apart overlap')
     return rows, cols, ld
 
 
-def _vector(v: Optional[torch.Tensor], n: int, name: str, x: torch.Tensor, types) -> Optional[int]:
-    """The address of a consecutive vector of n elements beside x (None: null)."""
+def _vector(v: Optional[torch.Tensor], n: int, name: str, device: int, dtype: torch.dtype) -> Optional[int]:
+    """The address of a consecutive vector of n elements on that GPU (None: null)."""
     if v is None:
         return None
-    if not isinstance(v, torch.Tensor) or v.device != x.device:
-        _refuse(f'{name}: a tensor on {x.device} is required')
-    if v.dtype not in types:
-        _refuse(f'{name}: {v.dtype} is not one of {", ".join(str(t) for t in types)}')
+    if not isinstance(v, torch.Tensor) or v.get_device() != device:
+        _refuse(f'{name}: a tensor on GPU {device} is required')
+    if v.dtype != dtype:
+        _refuse(f'{name}: {dtype} is required, not {v.dtype}')
     if v.numel() != n or not v.is_contiguous():
         _refuse(f'{name}: {n} consecutive elements are required, not {tuple(v.shape)} with strides {tuple(v.stride())}')
     return v.data_ptr()
+
+
+def _like(x: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
 
 
 def _act(act) -> int:
@@ -90,31 +94,30 @@ def _act(act) -> int:
     return _ACTS[act]
 
 
-def _stream(x: torch.Tensor) -> Tuple[int, int]:
-    return x.device.index, torch.cuda.current_stream(x.device).cuda_stream
-
-
 def _check(rc: int):
     if rc:
         raise EdgeGANLibError(_lib.eg_last_error(None).decode())
 
 
-def _workspace(size: int, x: torch.Tensor) -> Tuple[Optional[torch.Tensor], Optional[int], int]:
+def _workspace(size: int, x: torch.Tensor) -> Tuple[Optional[torch.Tensor], Optional[int]]:
     if size < 0:
         _refuse('sizes out of range')
     if size == 0:
-        return None, None, 0
-    w = torch.empty(size, dtype=torch.uint8, device=x.device)
-    return w, w.data_ptr(), size
+        return None, None
+    w = x.new_empty(size, dtype=torch.uint8)
+    return w, w.data_ptr()
 
 
-def _parameter_type(weight, bias, x) -> Tuple[int, Tuple]:
+def _parameter_type(weight, bias, x) -> torch.dtype:
     """One type for both: that of x or f32."""
-    given = [p.dtype for p in (weight, bias) if isinstance(p, torch.Tensor)]
-    t = given[0] if given else torch.float32
-    if t not in (x.dtype, torch.float32) or any(g != t for g in given):
-        _refuse(f'weight, bias: both {x.dtype} or both torch.float32, not {", ".join(str(g) for g in given)}')
-    return _TYPES[t], (t,)
+    t = x.dtype
+    for p in (weight, bias):
+        if isinstance(p, torch.Tensor):
+            t = p.dtype
+            break
+    if t != x.dtype and t != torch.float32:
+        _refuse(f'weight, bias: {x.dtype} or torch.float32 is required, not {t}')
+    return t
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5,
@@ -124,16 +127,14 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     statistics: also returns mean and rstd (f32, one of each row), which layer_norm_backward needs."""
     lib = _lib or _library()
     rows, cols, ld = _rows(x, 'x')
-    wtype, types = _parameter_type(weight, bias, x)
-    w, b = _vector(weight, cols, 'weight', x, types), _vector(bias, cols, 'bias', x, types)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean = rstd = None
+    device, wtype = x.get_device(), _parameter_type(weight, bias, x)
+    w, b = _vector(weight, cols, 'weight', device, wtype), _vector(bias, cols, 'bias', device, wtype)
+    y = _like(x)
+    mean = rstd = pm = pr = None
     if statistics:
-        mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-        rstd = torch.empty_like(mean)
-    device, stream = _stream(x)
-    _check(lib.eg_layer_norm(device, stream, _TYPES[x.dtype], x.data_ptr(), ld, wtype, w, b, rows, cols, eps, _act(act), y.data_ptr(), cols,
-                             mean.data_ptr() if statistics else None, rstd.data_ptr() if statistics else None))
+        mean, rstd = x.new_empty(x.shape[:-1], dtype=torch.float32), x.new_empty(x.shape[:-1], dtype=torch.float32)
+        pm, pr = mean.data_ptr(), rstd.data_ptr()
+    _check(lib.eg_layer_norm(device, _stream(device), _TYPES[x.dtype], x.data_ptr(), ld, _TYPES[wtype], w, b, rows, cols, eps, _act(act), y.data_ptr(), cols, pm, pr))
     return (y, mean, rstd) if statistics else y
 
 
@@ -142,32 +143,38 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, r
     """(dx, dweight, dbias) of layer_norm at x, with the statistics that it returned; dweight is None without a weight, dbias without a bias."""
     lib = _lib or _library()
     rows, cols, ld = _rows(x, 'x')
-    if not isinstance(dy, torch.Tensor) or dy.device != x.device or dy.dtype != x.dtype or dy.shape != x.shape:
+    device = x.get_device()
+    if not isinstance(dy, torch.Tensor) or dy.get_device() != device or dy.dtype != x.dtype or dy.shape != x.shape:
         _refuse(f'dy: {x.dtype} of shape {tuple(x.shape)} on {x.device} is required')
-    _, _, ldy = _rows(dy, 'dy')
-    f32 = (torch.float32,)
-    m, r = _vector(mean, rows, 'mean', x, f32), _vector(rstd, rows, 'rstd', x, f32)
+    ldy = _rows(dy, 'dy')[2]
+    m, r = _vector(mean, rows, 'mean', device, torch.float32), _vector(rstd, rows, 'rstd', device, torch.float32)
     if m is None or r is None:
         _refuse('mean, rstd: required')
-    wtype, types = _parameter_type(weight, bias, x)
-    w, b = _vector(weight, cols, 'weight', x, types), _vector(bias, cols, 'bias', x, types)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    dweight = torch.empty_like(weight) if weight is not None else None
-    dbias = torch.empty_like(bias) if bias is not None else None
-    keep, ws, size = _workspace(lib.eg_layer_norm_workspace(rows, cols) if w or b else 0, x)
-    device, stream = _stream(x)
-    _check(lib.eg_layer_norm_backward(device, stream, _TYPES[x.dtype], dy.data_ptr(), ldy, x.data_ptr(), ld, m, r, wtype, w, b, rows, cols, _act(act),
-                                      dx.data_ptr(), cols, dweight.data_ptr() if w else None, dbias.data_ptr() if b else None, ws, size))
+    wtype = _parameter_type(weight, bias, x)
+    w, b = _vector(weight, cols, 'weight', device, wtype), _vector(bias, cols, 'bias', device, wtype)
+    dx = _like(x)
+    dweight = dbias = keep = pw = pb = ws = None
+    size = 0
+    if weight is not None:
+        dweight = torch.empty_like(weight)
+        pw = dweight.data_ptr()
+    if bias is not None:
+        dbias = torch.empty_like(bias)
+        pb = dbias.data_ptr()
+    if pw or pb:
+        size = lib.eg_layer_norm_workspace(rows, cols)
+        keep, ws = _workspace(size, x)
+    _check(lib.eg_layer_norm_backward(device, _stream(device), _TYPES[x.dtype], dy.data_ptr(), ldy, x.data_ptr(), ld, m, r, _TYPES[wtype], w, b, rows, cols, _act(act),
+                                      dx.data_ptr(), cols, pw, pb, ws, size))
     return dx, dweight, dbias
 
 
-def _norm_parameters(norm, cols, x):
+def _norm_parameters(norm, cols, device):
     if norm is None:
         return 0, None, None, 1.0
     if not isinstance(norm, (tuple, list)) or len(norm) != 3:
         _refuse('norm: (weight or None, bias or None, eps) is required')
-    f32 = (torch.float32,)
-    return 1, _vector(norm[0], cols, 'norm weight', x, f32), _vector(norm[1], cols, 'norm bias', x, f32), float(norm[2])
+    return 1, _vector(norm[0], cols, 'norm weight', device, torch.float32), _vector(norm[1], cols, 'norm bias', device, torch.float32), norm[2]
 
 
 def quantize_rows(x: torch.Tensor, norm=None) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -177,13 +184,23 @@ def quantize_rows(x: torch.Tensor, norm=None) -> Tuple[torch.Tensor, torch.Tenso
     (weight, bias f32 or None).  q's rows are a multiple of 16 bytes apart, the gap zeros: what int8_matmul reads fastest."""
     lib = _lib or _library()
     rows, cols, ld = _rows(x, 'x')
-    on, g, b, eps = _norm_parameters(norm, cols, x)
+    device = x.get_device()
+    on, g, b, eps = _norm_parameters(norm, cols, device)
     pitch = (cols + 15) // 16 * 16
-    q = torch.empty(x.shape[:-1] + (pitch,), dtype=torch.int8, device=x.device)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    device, stream = _stream(x)
-    _check(lib.eg_quantize_rows(device, stream, _TYPES[x.dtype], x.data_ptr(), ld, on, g, b, eps, rows, cols, q.data_ptr(), pitch, scale.data_ptr()))
+    q = x.new_empty(x.shape[:-1] + (pitch,), dtype=torch.int8)
+    scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    _check(lib.eg_quantize_rows(device, _stream(device), _TYPES[x.dtype], x.data_ptr(), ld, on, g, b, eps, rows, cols, q.data_ptr(), pitch, scale.data_ptr()))
     return (q if pitch == cols else q[..., :cols]), scale
+
+
+_INT8 = (torch.int8,)
+
+
+def _weight(weight, k, device) -> Tuple[int, int]:
+    n, kw, ld = _rows(weight, 'weight', _INT8)
+    if weight.dim() != 2 or weight.get_device() != device or kw != k:
+        _refuse(f'weight: [n, {k}] on GPU {device} is required, not {tuple(weight.shape)} on {weight.device}')
+    return n, ld
 
 
 def int8_matmul(q: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
@@ -193,19 +210,17 @@ def int8_matmul(q: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, weig
     q int8 [..., k] with a scale for each row, weight int8 [n, k] with a scale for each output channel (both as quantize_rows returns them; k <= 131071),
     bias f32 [n] or None; out in out_dtype (f32, bf16, f16)."""
     lib = _lib or _library()
-    i8, f32 = (torch.int8,), (torch.float32,)
-    m, k, lda = _rows(q, 'q', i8)
-    n, kw, ldb = _rows(weight, 'weight', i8)
-    if weight.dim() != 2 or weight.device != q.device or kw != k:
-        _refuse(f'weight: [n, {k}] on {q.device} is required, not {tuple(weight.shape)} on {weight.device}')
+    m, k, lda = _rows(q, 'q', _INT8)
+    device = q.get_device()
+    n, ldb = _weight(weight, k, device)
     if out_dtype not in _TYPES:
         _refuse(f'out_dtype: {out_dtype} is not one of {", ".join(str(t) for t in _TYPES)}')
-    s, ws, b = _vector(scale, m, 'scale', q, f32), _vector(weight_scale, n, 'weight_scale', q, f32), _vector(bias, n, 'bias', q, f32)
+    s, ws = _vector(scale, m, 'scale', device, torch.float32), _vector(weight_scale, n, 'weight_scale', device, torch.float32)
+    b = _vector(bias, n, 'bias', device, torch.float32)
     if s is None or ws is None:
         _refuse('scale, weight_scale: required')
-    out = torch.empty(q.shape[:-1] + (n,), dtype=out_dtype, device=q.device)
-    device, stream = _stream(q)
-    _check(lib.eg_int8_matmul(device, stream, q.data_ptr(), lda, s, weight.data_ptr(), ldb, ws, b, m, n, k, _TYPES[out_dtype], out.data_ptr(), n))
+    out = q.new_empty(q.shape[:-1] + (n,), dtype=out_dtype)
+    _check(lib.eg_int8_matmul(device, _stream(device), q.data_ptr(), lda, s, weight.data_ptr(), ldb, ws, b, m, n, k, _TYPES[out_dtype], out.data_ptr(), n))
     return out
 
 
@@ -214,25 +229,27 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     """A linear layer in 8-bit integers: int8_matmul(*quantize_rows(x, norm), weight, weight_scale, bias), in x's type unless out_dtype says otherwise; for few rows
     one launch."""
     lib = _lib or _library()
-    f32 = (torch.float32,)
     m, k, ld = _rows(x, 'x')
-    on, g, beta, eps = _norm_parameters(norm, k, x)
-    n, kw, ldw = _rows(weight, 'weight', (torch.int8,))
-    if weight.dim() != 2 or weight.device != x.device or kw != k:
-        _refuse(f'weight: [n, {k}] on {x.device} is required, not {tuple(weight.shape)} on {weight.device}')
+    device = x.get_device()
+    on, g, beta, eps = _norm_parameters(norm, k, device)
+    n, ldw = _weight(weight, k, device)
     if out_dtype is None:
         out_dtype = x.dtype
     elif out_dtype not in _TYPES:
         _refuse(f'out_dtype: {out_dtype} is not one of {", ".join(str(t) for t in _TYPES)}')
-    ws, b = _vector(weight_scale, n, 'weight_scale', x, f32), _vector(bias, n, 'bias', x, f32)
+    ws, b = _vector(weight_scale, n, 'weight_scale', device, torch.float32), _vector(bias, n, 'bias', device, torch.float32)
     if ws is None:
         _refuse('weight_scale: required')
-    out = torch.empty(x.shape[:-1] + (n,), dtype=out_dtype, device=x.device)
-    keep, wp, size = _workspace(lib.eg_int8_linear_workspace(m, k), x)
-    device, stream = _stream(x)
-    _check(lib.eg_int8_linear(device, stream, _TYPES[x.dtype], x.data_ptr(), ld, on, g, beta, eps, weight.data_ptr(), ldw, ws, b, m, n, k, _TYPES[out_dtype],
+    out = x.new_empty(x.shape[:-1] + (n,), dtype=out_dtype)
+    size = lib.eg_int8_linear_workspace(m, k)
+    keep, wp = _workspace(size, x)
+    _check(lib.eg_int8_linear(device, _stream(device), _TYPES[x.dtype], x.data_ptr(), ld, on, g, beta, eps, weight.data_ptr(), ldw, ws, b, m, n, k, _TYPES[out_dtype],
                               out.data_ptr(), n, wp, size))
     return out
+
+
+_F32 = (torch.float32,)
+_INDEXES = {torch.int64: 8, torch.int32: 4}   # bytes
 
 
 def distill_loss(logits: torch.Tensor, index: torch.Tensor, teacher: torch.Tensor, temperature: float = 1.0,
@@ -244,16 +261,20 @@ def distill_loss(logits: torch.Tensor, index: torch.Tensor, teacher: torch.Tenso
     or None (1).  An index outside [0, classes) is padding; a row of weight 0 or without a kept logit has loss and gradient 0 whatever its logits hold."""
     lib = _lib or _library()
     rows, cols, ld = _rows(logits, 'logits')
-    if not isinstance(index, torch.Tensor) or not isinstance(teacher, torch.Tensor) or index.shape != teacher.shape or index.shape[:-1] != logits.shape[:-1] \
-            or index.device != logits.device or teacher.device != logits.device:
-        _refuse(f'index, teacher: both {tuple(logits.shape[:-1])} + (top,) on {logits.device} are required')
-    _, top, ldi = _rows(index, 'index', (torch.int64, torch.int32))
-    _, _, ldt = _rows(teacher, 'teacher', (torch.float32,))
-    w = _vector(row_weight, rows, 'row_weight', logits, (torch.float32,))
-    loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=logits.device)
-    dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if grad else None
-    keep, ws, size = _workspace(lib.eg_distill_loss_workspace(rows, cols, top), logits)
-    device, stream = _stream(logits)
-    _check(lib.eg_distill_loss(device, stream, _TYPES[logits.dtype], logits.data_ptr(), ld, index.element_size(), index.data_ptr(), ldi, teacher.data_ptr(), ldt,
-                               w, rows, cols, top, temperature, loss.data_ptr(), dlogits.data_ptr() if grad else None, cols, ws, size))
+    device, shape = logits.get_device(), logits.shape[:-1]
+    if not isinstance(index, torch.Tensor) or not isinstance(teacher, torch.Tensor) or index.shape != teacher.shape or index.shape[:-1] != shape \
+            or index.get_device() != device or teacher.get_device() != device:
+        _refuse(f'index, teacher: both {tuple(shape)} + (top,) on {logits.device} are required')
+    _, top, ldi = _rows(index, 'index', _INDEXES)
+    ldt = _rows(teacher, 'teacher', _F32)[2]
+    w = _vector(row_weight, rows, 'row_weight', device, torch.float32)
+    loss = logits.new_empty(shape, dtype=torch.float32)
+    dlogits = pg = None
+    if grad:
+        dlogits = _like(logits)
+        pg = dlogits.data_ptr()
+    size = lib.eg_distill_loss_workspace(rows, cols, top)
+    keep, ws = _workspace(size, logits)
+    _check(lib.eg_distill_loss(device, _stream(device), _TYPES[logits.dtype], logits.data_ptr(), ld, _INDEXES[index.dtype], index.data_ptr(), ldi, teacher.data_ptr(), ldt,
+                               w, rows, cols, top, temperature, loss.data_ptr(), pg, cols, ws, size))
     return loss, dlogits
