@@ -65,8 +65,8 @@ __global__ __launch_bounds__(256) void int8_any(Int8Args a, int tiles_n, int ali
 
 // ---- tiles in LDS ------------------------------------------------------------------------------------------------------------------
 // BM x BN outputs a block, WM x WN waves, 128 bytes of k a step, two buffers: while a step's 32x32x32 products run, the next step's tiles are on their way from memory
-// straight to LDS.  A tile row is eight 16-byte groups; group s of row r holds the row's group s ^ (r & 7), so that the 32 rows of a
-// fragment lie in different banks (the write is a wave's 1,024 consecutive bytes: the permutation is in the source addresses).
+// straight to LDS.  A tile row is eight 16-byte groups; group s of row r holds the row's group s ^ (r / 2 & 7), so that sixteen rows of a
+// fragment lie in all 64 banks (with r & 7 half of the LDS time was bank conflicts; the write is a wave's 1,024 consecutive bytes: the permutation is in the source addresses).
 // Rows past the end repeat the last one (their results are not stored); groups past k read as zeros; the bytes past k in its last group are cleared
 // in a's fragments, which is enough.
 using i32x16 = __attribute__((ext_vector_type(16))) int;
@@ -101,7 +101,7 @@ __device__ __forceinline__ void int8_step(const signed char* __restrict__ ca, co
   const int l31 = lane & 31, lh = lane >> 5;
 #pragma unroll
   for (int ks = 0; ks < kStep / 32; ++ks) {
-    const int slot = ((ks * 2 + lh) ^ (l31 & 7)) * 16;
+    const int slot = ((ks * 2 + lh) ^ ((l31 >> 1) & 7)) * 16;
     i32x4 fa[S::MI], fb[S::NI];
 #pragma unroll
     for (int x = 0; x < S::MI; ++x) fa[x] = *reinterpret_cast<const i32x4*>(ca + (arow + x * 32) * kStep + slot);
@@ -141,7 +141,8 @@ __global__ __launch_bounds__(WM * WN * 64) void int8_tiles(Int8Args a, int tiles
   const int j0 = tn * BN;
 
   const __amdgpu_buffer_rsrc_t ab = row_buffer(a.a + i0 * a.lda, 0x7ffffff0u), bb = row_buffer(a.b + (long long)j0 * a.ldb, 0x7ffffff0u);
-  const int koff = ((lane & 7) ^ (lane >> 3)) * 16;   // this lane's group of a row in k
+  const int koff = ((lane & 7) ^ ((wave * 4 + (lane >> 4)) & 7)) * 16;   // this lane's group of its rows (8 (j NW + wave) + lane / 8) in k
+  static_assert(S::NW % 2 == 0, "the same group for every j");
   const int rows_a = (int)min((long long)BM, a.m - i0) - 1, rows_b = min(BN, a.n - j0) - 1;
   unsigned va[S::JA], vb[S::JB];
 #pragma unroll
