@@ -320,10 +320,10 @@ __global__ __launch_bounds__(kFewWaves * 64) void int8_few_linear(Int8Args a, Qu
 
   // the rows and the norm's parameters before b: loads arrive in order, and they are what the next lines wait for
   const int t = threadIdx.x & (NT - 1), side = wave >> 2;
-  float gamma[NV][V], beta[NV][V];
+  Parameter<float, NT, NV, V, false> gamma, beta;
   if (q.norm) {
-    load_parameter<float, NT, NV, V>(q.gamma, a.k, t, 1.f, gamma);
-    load_parameter<float, NT, NV, V>(q.beta, a.k, t, 0.f, beta);
+    gamma.load(q.gamma, a.k, t);
+    beta.load(q.beta, a.k, t);
   }
   float v[TURNS][NV][V];
 #pragma unroll
@@ -343,17 +343,21 @@ __global__ __launch_bounds__(kFewWaves * 64) void int8_few_linear(Int8Args a, Qu
   for (int n = 0; n < TURNS; ++n) {
     if (q.norm) {
       float mean, rstd;
-      centre_row<NT, NV, V>(v[n], a.k, t, q.eps, red[side][n], mean, rstd);
+      centre_row<NT, NV, V, false>(v[n], a.k, t, q.eps, red[side][n], mean, rstd);
+      each_pack<NT, NV, V>(a.k, t, [&](int i, int) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[n][i][j] = affine_r(rounded_mul(v[n][i][j], rstd), gamma[i][j], beta[i][j]);
+        for (int j = 0; j < V; ++j) {
+          v[n][i][j] = rounded_mul(v[n][i][j], rstd);
+          if (q.gamma) v[n][i][j] = rounded_mul(v[n][i][j], gamma.k[i].e[j]);
+          if (q.beta) v[n][i][j] += beta.k[i].e[j];
+        }
+      });
     }
     float m = 0.f;
+    each_pack<NT, NV, V>(a.k, t, [&](int i, int) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < V; ++j) m = max_nan(m, (i * NT + t) * V < a.k ? fabsf(v[n][i][j]) : 0.f);
+      for (int j = 0; j < V; ++j) m = max_nan(m, fabsf(v[n][i][j]));
+    });
     m = team_max<NT>(m, red_max[side][n]);
     const double inv = quantize_factor(m);
     const bool fine = quantizable(m);

@@ -18,65 +18,49 @@
 namespace eg {
 
 // ---- rows in registers -------------------------------------------------------------------------------------------------------
-// NT threads own a row, each NV packs of V consecutive elements: pack i of thread t begins at column (i NT + t) V.
-template <typename T, int NT, int NV, int V>
-__device__ __forceinline__ void load_row(const T* p, int cols, int t, float (&v)[NV][V]) {
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (i * NT + t) * V;
-    load_pack<T, V>(p + (c < cols ? c : 0), v[i]);   // (no branch, so that all of a thread's loads are in flight at once)
-    if (c >= cols)
-#pragma unroll
-      for (int j = 0; j < V; ++j) v[i][j] = 0.f;
-  }
-}
-// the same in two halves: the loads (kept in the row's own type, to be issued a row ahead) and the conversion
-template <typename T, int NT, int NV, int V>
-__device__ __forceinline__ void request_row(const T* p, int cols, int t, Pack<T, V> (&k)[NV]) {
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (i * NT + t) * V;
-    k[i] = *reinterpret_cast<const Pack<T, V>*>(p + (c < cols ? c : 0));
-  }
-}
-template <typename T, int NT, int NV, int V>
-__device__ __forceinline__ void take_row(const Pack<T, V> (&k)[NV], int cols, int t, float (&v)[NV][V]) {
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[i][j] = (i * NT + t) * V < cols ? (float)k[i].e[j] : 0.f;
-}
-template <typename T, int NT, int NV, int V>
-__device__ __forceinline__ void store_row(T* p, int cols, int t, const float (&v)[NV][V]) {
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (i * NT + t) * V;
-    if (c < cols) store_pack<T, V>(p + c, v[i]);
-  }
-}
-template <typename T, typename W, int NT, int NV, int V>
+template <typename T, typename W, int NT, int NV, int V, bool TAIL>
 __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_fwd(LayerNormArgs a) {
   constexpr int NB = NT > 256 ? NT : 256, TEAMS = NB / NT;
   __shared__ double red[2][centre_lds(NT)];
   const int t = TEAMS > 1 ? threadIdx.x % NT : threadIdx.x, team = TEAMS > 1 ? threadIdx.x / NT : 0;
-  float g[NV][V], b[NV][V];
-  load_parameter<W, NT, NV, V>((const W*)a.gamma, a.cols, t, 1.f, g);
-  load_parameter<W, NT, NV, V>((const W*)a.beta, a.cols, t, 0.f, b);
+  Parameter<W, NT, NV, V, TAIL> gamma, beta;
+  auto parameters = [&] {
+    gamma.load((const W*)a.gamma, a.cols, t);
+    beta.load((const W*)a.beta, a.cols, t);
+  };
+  constexpr bool HELD = NT <= 64;   // over the rows; a wider team sees few rows and reads them again, from the caches
+  if constexpr (HELD) parameters();
   int turn = 0;
   const long long step = (long long)gridDim.x * TEAMS;
   long long r = (long long)blockIdx.x * TEAMS + team;
-  Pack<T, V> next[NV];
-  if (r < a.rows) request_row<T, NT, NV, V>((const T*)a.x + r * a.ldx, a.cols, t, next);
+  LoosePack<T, V> next[NV];
+  if (r < a.rows) request_row<T, NT, NV, V, TAIL>((const T*)a.x + r * a.ldx, a.cols, t, next);
   for (; r < a.rows; r += step, turn ^= 1) {
     float v[NV][V], mean, rstd;
-    take_row<T, NT, NV, V>(next, a.cols, t, v);
-    if (r + step < a.rows) request_row<T, NT, NV, V>((const T*)a.x + (r + step) * a.ldx, a.cols, t, next);
-    centre_row<NT, NV, V>(v, a.cols, t, a.eps, red[turn], mean, rstd);
+    settle_row<T, NT, NV, V, TAIL>(a.cols, t, next);
+    each_pack<NT, NV, V>(a.cols, t, [&](int i, int) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+      for (int j = 0; j < V; ++j) v[i][j] = (float)next[i].e[j];
+    });
+    if (r + step < a.rows) request_row<T, NT, NV, V, TAIL>((const T*)a.x + (r + step) * a.ldx, a.cols, t, next);
+    if constexpr (!HELD) parameters();
+    centre_row<NT, NV, V, TAIL>(v, a.cols, t, a.eps, red[turn], mean, rstd);
+    T* y = (T*)a.y + r * a.ldy;
+    by_act(a.act, [&](auto act) {
+      each_pack<NT, NV, V>(a.cols, t, [&](int i, int c) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[i][j] = row_act(affine_r(rounded_mul(v[i][j], rstd), g[i][j], b[i][j]), a.act);
-    store_row<T, NT, NV, V>((T*)a.y + r * a.ldy, a.cols, t, v);
+        for (int j = 0; j < V; ++j) v[i][j] = rounded_mul(v[i][j], rstd);
+        if (a.gamma)
+#pragma unroll
+          for (int j = 0; j < V; ++j) v[i][j] = rounded_mul(v[i][j], (float)gamma.k[i].e[j]);
+        if (a.beta)
+#pragma unroll
+          for (int j = 0; j < V; ++j) v[i][j] += (float)beta.k[i].e[j];
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[i][j] = row_act<decltype(act)::value>(v[i][j]);
+        store_row_pack<T, V, TAIL>(y, c, a.cols, v[i]);
+      });
+    });
     if (t == 0 && a.mean) {
       a.mean[r] = mean;
       a.rstd[r] = rstd;
@@ -84,13 +68,14 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_fwd(LayerNormArgs a) {
   }
 }
 
-template <typename T, typename W, int NT, int NV, int V>
+template <typename T, typename W, int NT, int NV, int V, bool TAIL>
 __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_bwd(LayerNormGradArgs a) {
   constexpr int NB = NT > 256 ? NT : 256, TEAMS = NB / NT;
   __shared__ float red[2][NT > 64 ? 2 * NT / 64 : 1];
   const int t = TEAMS > 1 ? threadIdx.x % NT : threadIdx.x, team = TEAMS > 1 ? threadIdx.x / NT : 0;
-  float g[NV][V], sx[NV][V], sg[NV][V];
-  load_parameter<W, NT, NV, V>((const W*)a.gamma, a.cols, t, 1.f, g);
+  Parameter<W, NT, NV, V, TAIL> gamma;
+  gamma.load((const W*)a.gamma, a.cols, t);
+  float sx[NV][V], sg[NV][V];
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -99,57 +84,68 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_bwd(LayerNormGradArgs 
   int turn = 0;
   const long long step = (long long)gridDim.x * TEAMS;
   long long r = (long long)blockIdx.x * TEAMS + team;
-  Pack<T, V> next_x[NV], next_d[NV];
+  LoosePack<T, V> next_x[NV], next_d[NV];
   float next_mean = 0.f, next_rstd = 0.f;
   auto request = [&](long long row) {
-    request_row<T, NT, NV, V>((const T*)a.x + row * a.ldx, a.cols, t, next_x);
-    request_row<T, NT, NV, V>((const T*)a.dy + row * a.lddy, a.cols, t, next_d);
+    request_row<T, NT, NV, V, TAIL>((const T*)a.x + row * a.ldx, a.cols, t, next_x);
+    request_row<T, NT, NV, V, TAIL>((const T*)a.dy + row * a.lddy, a.cols, t, next_d);
     next_mean = a.mean[row];
     next_rstd = a.rstd[row];
   };
   if (r < a.rows) request(r);
   for (; r < a.rows; r += step, turn ^= 1) {
     float x[NV][V], d[NV][V];
-    take_row<T, NT, NV, V>(next_x, a.cols, t, x);
-    take_row<T, NT, NV, V>(next_d, a.cols, t, d);
+    settle_row<T, NT, NV, V, TAIL>(a.cols, t, next_x);
+    settle_row<T, NT, NV, V, TAIL>(a.cols, t, next_d);   // (d = 0 past the end: reaches no sum)
     const float mean = next_mean, rstd = next_rstd;
+    each_pack<NT, NV, V>(a.cols, t, [&](int i, int) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        x[i][j] = rounded_mul((float)next_x[i].e[j] - mean, rstd);
+        d[i][j] = (float)next_d[i].e[j];
+      }
+    });
     if (r + step < a.rows) request(r + step);   // (in flight while this row is summed and stored)
     if (a.act != ACT_NONE) {
-      float b[NV][V];
-      load_parameter<W, NT, NV, V>((const W*)a.beta, a.cols, t, 0.f, b);
+      Parameter<W, NT, NV, V, TAIL> beta;
+      beta.load((const W*)a.beta, a.cols, t);
+      const float below = a.act == ACT_LRELU ? 0.2f : 0.f;
+      each_pack<NT, NV, V>(a.cols, t, [&](int i, int) {
+        float z[V];
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
+        for (int j = 0; j < V; ++j) z[j] = a.gamma ? rounded_mul(x[i][j], (float)gamma.k[i].e[j]) : x[i][j];
+        if (a.beta)
 #pragma unroll
-        for (int j = 0; j < V; ++j) d[i][j] *= row_act_grad(affine_r(rounded_mul(x[i][j] - mean, rstd), g[i][j], b[i][j]), a.act);
+          for (int j = 0; j < V; ++j) z[j] += (float)beta.k[i].e[j];
+#pragma unroll
+        for (int j = 0; j < V; ++j) d[i][j] = z[j] > 0.f ? d[i][j] : below * d[i][j];
+      });
     }
     float s[2] = {0.f, 0.f};
+    each_pack<NT, NV, V>(a.cols, t, [&](int i, int) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < V; ++j) {   // (columns past the last have d = 0 and reach no sum)
-        x[i][j] = rounded_mul(x[i][j] - mean, rstd);
+      for (int j = 0; j < V; ++j) {
         sg[i][j] += d[i][j];
         sx[i][j] += d[i][j] * x[i][j];
-        d[i][j] *= g[i][j];
+        if (a.gamma) d[i][j] *= (float)gamma.k[i].e[j];
         s[0] += d[i][j];
         s[1] += d[i][j] * x[i][j];
       }
+    });
     if (!a.dx) continue;
     team_sum<NT>(s, red[turn]);
     const float m0 = s[0] * n, m1 = s[1] * n;
     T* dx = (T*)a.dx + r * a.lddx;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
+    each_pack<NT, NV, V>(a.cols, t, [&](int i, int c) {
 #pragma unroll
       for (int j = 0; j < V; ++j) d[i][j] = (d[i][j] - m0 - x[i][j] * m1) * rstd;
-    if (a.acc_x) {
-      load_row<T, NT, NV, V>(dx, a.cols, t, x);
+      if (a.acc_x) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < V; ++j) d[i][j] += x[i][j];
-    }
-    store_row<T, NT, NV, V>(dx, a.cols, t, d);
+        for (int j = 0; j < V; ++j)
+          if (c + j < a.cols) d[i][j] += (float)dx[c + j];
+      }
+      store_row_pack<T, V, TAIL>(dx, c, a.cols, d[i]);
+    });
   }
   if (!a.partial) return;
   float* out = a.partial + (size_t)blockIdx.x * 2 * a.cols;
@@ -175,9 +171,9 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_bwd(LayerNormGradArgs 
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * NT + t) * V;
-      if (c < a.cols)
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
+      for (int j = 0; j < V; ++j)
+        if (c + j < a.cols) {
           out[c + j] = sx[i][j];
           out[a.cols + c + j] = sg[i][j];
         }
@@ -210,7 +206,7 @@ __global__ __launch_bounds__(1024) void ln_bwd_finish(const float* partial, int 
   *out = (W)s;
 }
 
-template <typename T, int NT, int NV, int V>
+template <typename T, int NT, int NV, int V, bool TAIL>
 __global__ __launch_bounds__(NT > 256 ? NT : 256) void quantize_rows(QuantizeArgs a) {
   constexpr int NB = NT > 256 ? NT : 256, TEAMS = NB / NT;
   __shared__ double red[2][centre_lds(NT)];
@@ -219,27 +215,34 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void quantize_rows(QuantizeArg
   const int width = (int)min((long long)((a.cols + 15) & ~15), a.ldq);   // the row's last 16-byte group is filled up with zeros
   int turn = 0;
   for (long long r = (long long)blockIdx.x * TEAMS + team; r < a.rows; r += (long long)gridDim.x * TEAMS, turn ^= 1) {
+    LoosePack<T, V> k[NV];
+    request_row<T, NT, NV, V, TAIL>((const T*)a.x + r * a.ldx, a.cols, t, k);
+    settle_row<T, NT, NV, V, TAIL>(a.cols, t, k);
     float v[NV][V];
-    load_row<T, NT, NV, V>((const T*)a.x + r * a.ldx, a.cols, t, v);
-    if (a.norm) {
-      float mean, rstd, p[NV][V];
-      centre_row<NT, NV, V>(v, a.cols, t, a.eps, red[turn], mean, rstd);
-      load_parameter<float, NT, NV, V>(a.gamma, a.cols, t, 1.f, p);
+    each_pack<NT, NV, V>(a.cols, t, [&](int i, int) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[i][j] = rounded_mul(rounded_mul(v[i][j], rstd), p[i][j]);
-      load_parameter<float, NT, NV, V>(a.beta, a.cols, t, 0.f, p);
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[i][j] = v[i][j] + p[i][j];
-    }
+      for (int j = 0; j < V; ++j) v[i][j] = (float)k[i].e[j];
+    });
     float m = 0.f;
+    if (a.norm) {
+      Parameter<float, NT, NV, V, TAIL> gamma, beta;
+      gamma.load(a.gamma, a.cols, t);
+      beta.load(a.beta, a.cols, t);
+      float mean, rstd;
+      centre_row<NT, NV, V, TAIL>(v, a.cols, t, a.eps, red[turn], mean, rstd);
+      each_pack<NT, NV, V>(a.cols, t, [&](int i, int) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+        for (int j = 0; j < V; ++j) {
+          v[i][j] = rounded_mul(v[i][j], rstd);
+          if (a.gamma) v[i][j] = rounded_mul(v[i][j], gamma.k[i].e[j]);
+          if (a.beta) v[i][j] += beta.k[i].e[j];   // (zeros past the end)
+        }
+      });
+    }
+    each_pack<NT, NV, V>(a.cols, t, [&](int i, int) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) m = max_nan(m, (i * NT + t) * V < a.cols ? fabsf(v[i][j]) : 0.f);
+      for (int j = 0; j < V; ++j) m = max_nan(m, fabsf(v[i][j]));
+    });
     m = team_max<NT>(m, red_max[turn]);
     const double inv = quantize_factor(m);
     const bool fine = quantizable(m);
@@ -248,10 +251,14 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void quantize_rows(QuantizeArg
     for (int i = 0; i < NV; ++i) {
       const int c = (i * NT + t) * V;
       if (c >= width) continue;
-      Pack<unsigned char, V> k;
+      LoosePack<unsigned char, V> k;
 #pragma unroll
-      for (int j = 0; j < V; ++j) k.e[j] = (unsigned char)(fine && c < a.cols ? quantize1(v[i][j], inv) : 0u);
-      *reinterpret_cast<Pack<unsigned char, V>*>(q + c) = k;
+      for (int j = 0; j < V; ++j) k.e[j] = (unsigned char)(fine && c < a.cols ? quantize1(v[i][j], inv) : 0u);   // (zeros past the end give 0)
+      if (c + V <= width) *reinterpret_cast<LoosePack<unsigned char, V>*>(q + c) = k;
+      else
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (c + j < width) q[c + j] = k.e[j];
     }
     if (t == 0) a.scale[r] = quantize_scale(m);
   }
@@ -283,7 +290,10 @@ __global__ __launch_bounds__(kRowThreads) void ln_fwd_rows(LayerNormArgs a) {
     float mean, rstd;
     row_statistics<T>(x, a.cols, a.eps, red, mean, rstd);
     for (int c = threadIdx.x; c < a.cols; c += kRowThreads)
-      y[c] = (T)row_act(affine(rounded_mul((float)x[c] - mean, rstd), (const W*)a.gamma, (const W*)a.beta, c), a.act);
+      {
+      const float z = affine(rounded_mul((float)x[c] - mean, rstd), (const W*)a.gamma, (const W*)a.beta, c);
+      by_act(a.act, [&](auto act) { y[c] = (T)row_act<decltype(act)::value>(z); });
+    }
     if (threadIdx.x == 0 && a.mean) {
       a.mean[r] = mean;
       a.rstd[r] = rstd;
@@ -353,26 +363,22 @@ __global__ __launch_bounds__(256) void ln_bwd_columns(LayerNormGradArgs a) {
 static dim3 row_grid(long long rows) { return dim3((unsigned)std::min<long long>(rows, 1 << 20)); }
 static int part_groups(long long rows) { return (int)std::min<long long>(kPartBlocks, (rows + 3) / 4); }
 
-// Calls f(threads of a row, packs of a thread, elements of a pack) for the smallest team whose registers hold a row of `cols`; false: none does.
-// Packs of 16 bytes where every row begins at a multiple of 16 bytes and ends with a whole pack, else single elements.  A thread keeps at most MOST elements.
-template <int MOST, int V, typename F>
-static bool row_team(int cols, F f) {
-#define EG_TEAM(NT, NV) \
-  if constexpr ((NV) * V <= MOST) \
-    if (cols <= (NT) * (NV) * V) return f(std::integral_constant<int, NT>{}, std::integral_constant<int, NV>{}, std::integral_constant<int, V>{}), true;
-  if constexpr (V > 1) {
-    EG_TEAM(8, 1) EG_TEAM(16, 1) EG_TEAM(32, 1) EG_TEAM(64, 1) EG_TEAM(64, 2) EG_TEAM(64, 4) EG_TEAM(256, 2) EG_TEAM(256, 4) EG_TEAM(1024, 2) EG_TEAM(1024, 4)
-  } else {
-    EG_TEAM(32, 1) EG_TEAM(64, 4) EG_TEAM(64, 16) EG_TEAM(256, 8) EG_TEAM(256, 16) EG_TEAM(256, 32) EG_TEAM(1024, 16) EG_TEAM(1024, 32)
-  }
-#undef EG_TEAM
-  return false;
-}
-static bool aligned16(const void* p, long long ld, int elem) { return (uintptr_t)p % 16 == 0 && ld * elem % 16 == 0; }
+// Calls f(threads of a row, packs of a thread, elements of a pack, whether the last pack may be cut) for the smallest team whose registers hold a row of `cols`; false: none does.
+// A thread keeps at most MOST elements, 16 in a block of 1,024 (which has 128 registers a thread).
 template <typename T, int MOST, typename F>
-static bool row_team(bool packs, int cols, F f) {
+static bool row_team(int cols, F f) {
   constexpr int V = 16 / sizeof(T);
-  return packs && cols % V == 0 ? row_team<MOST, V>(cols, f) : row_team<MOST, 1>(cols, f);
+  using std::integral_constant;
+  auto pick = [&](auto tail) {
+#define EG_TEAM(NT, NV) \
+  if constexpr ((NV) * V <= ((NT) > 256 ? 16 : MOST)) \
+    if (cols <= (NT) * (NV) * V) return f(integral_constant<int, NT>{}, integral_constant<int, NV>{}, integral_constant<int, V>{}, tail), true;
+    EG_TEAM(8, 1) EG_TEAM(16, 1) EG_TEAM(32, 1) EG_TEAM(64, 1) EG_TEAM(64, 2) EG_TEAM(64, 4) EG_TEAM(256, 2) EG_TEAM(256, 4) EG_TEAM(1024, 2) EG_TEAM(1024, 4)
+#undef EG_TEAM
+    return false;
+  };
+  if (cols < V) return f(integral_constant<int, 8>{}, integral_constant<int, 1>{}, integral_constant<int, 1>{}, std::false_type{}), true;   // (shorter than a pack)
+  return cols % V ? pick(std::true_type{}) : pick(std::false_type{});
 }
 static dim3 team_grid(long long rows, int nt, int most) {
   const int teams = nt > 256 ? 1 : 256 / nt;
@@ -391,9 +397,8 @@ void launch_layer_norm(const LayerNormArgs& a, int type, int wtype, hipStream_t 
     using T = decltype(t);
     auto go = [&](auto w) {
       using W = decltype(w);
-      const bool packs = aligned16(a.x, a.ldx, sizeof(T)) && aligned16(a.y, a.ldy, sizeof(T)) && (uintptr_t)a.gamma % 16 == 0 && (uintptr_t)a.beta % 16 == 0;
-      if (!row_team<T, 32>(packs, a.cols, [&](auto nt, auto nv, auto v) {
-            row_launch(ln_fwd<T, W, nt, nv, v>, team_grid(a.rows, nt, 8192), team_block(nt), s, a);
+      if (!row_team<T, 32>(a.cols, [&](auto nt, auto nv, auto v, auto tail) {
+            row_launch(ln_fwd<T, W, nt, nv, v, tail>, team_grid(a.rows, nt, 8192), team_block(nt), s, a);
           }))
         row_launch(ln_fwd_rows<T, W>, row_grid(a.rows), dim3(kRowThreads), s, a);
     };
@@ -411,14 +416,12 @@ void launch_layer_norm_backward(const LayerNormGradArgs& given, int type, int wt
     using T = decltype(t);
     auto go = [&](auto w) {
       using W = decltype(w);
-      const bool packs = aligned16(a.x, a.ldx, sizeof(T)) && aligned16(a.dy, a.lddy, sizeof(T)) && aligned16(a.dx, a.lddx, sizeof(T)) &&
-                         (uintptr_t)a.gamma % 16 == 0 && (uintptr_t)a.beta % 16 == 0;
       int groups = 0;
       if (a.rows) {
-        const bool held = row_team<T, 16>(packs, a.cols, [&](auto nt, auto nv, auto v) {
+        const bool held = row_team<T, 16>(a.cols, [&](auto nt, auto nv, auto v, auto tail) {
           const dim3 grid = team_grid(a.rows, nt, nt > 64 ? kGradBlocks / 2 : kGradBlocks);
           groups = (int)grid.x;
-          row_launch(ln_bwd<T, W, nt, nv, v>, grid, team_block(nt), s, a);
+          row_launch(ln_bwd<T, W, nt, nv, v, tail>, grid, team_block(nt), s, a);
         });
         if (!held) {
           if (params) {   // (first: dx may be dy)
@@ -568,9 +571,9 @@ void launch_quantize_rows(const QuantizeArgs& a, int type, hipStream_t s) {
   if (!a.rows) return;
   by_type(type, [&](auto t) {
     using T = decltype(t);
-    const bool packs = aligned16(a.x, a.ldx, sizeof(T)) && aligned16(a.q, a.ldq, 1) && (uintptr_t)a.gamma % 16 == 0 && (uintptr_t)a.beta % 16 == 0;
-    if (!row_team<T, 32>(packs, a.cols, [&](auto nt, auto nv, auto v) {
-          row_launch(quantize_rows<T, nt, nv, v>, team_grid(a.rows, nt, 8192), team_block(nt), s, a);
+    // (a row shorter than a pack: its team would not reach the end of its 16 bytes)
+    if (a.cols < (int)(16 / sizeof(T)) || !row_team<T, 32>(a.cols, [&](auto nt, auto nv, auto v, auto tail) {
+          row_launch(quantize_rows<T, nt, nv, v, tail>, team_grid(a.rows, nt, 8192), team_block(nt), s, a);
         }))
       row_launch(quantize_kernel<T>, row_grid(a.rows), dim3(kRowThreads), s, a);
   });

@@ -33,11 +33,21 @@ __device__ __forceinline__ float rounded_mul(float a, float b) {
 #pragma clang fp contract(off)
   return a * b;
 }
-__device__ __forceinline__ float row_act(float z, int act) {
-  return act == ACT_NONE ? z : z > 0.f ? z : act == ACT_LRELU ? 0.2f * z : (z != z ? z : 0.f);
+template <int ACT>
+__device__ __forceinline__ float row_act(float z) {   // a NaN stays
+  if constexpr (ACT == ACT_RELU) return z < 0.f ? 0.f : z;
+  else if constexpr (ACT == ACT_LRELU) return fmaxf(z, 0.2f * z);
+  else return z;
 }
 // derivative of row_act at the pre-activation z
 __device__ __forceinline__ float row_act_grad(float z, int act) { return act == ACT_NONE || z > 0.f ? 1.f : act == ACT_LRELU ? 0.2f : 0.f; }
+// f(the activation as a type)
+template <typename F>
+__device__ __forceinline__ void by_act(int act, F f) {
+  if (act == ACT_RELU) f(std::integral_constant<int, ACT_RELU>{});
+  else if (act == ACT_LRELU) f(std::integral_constant<int, ACT_LRELU>{});
+  else f(std::integral_constant<int, ACT_NONE>{});
+}
 
 // One step of a butterfly over a wave, by data-parallel primitives (a few cycles; a shuffle goes through LDS): (a, b) are the values of the
 // two lanes whose numbers differ in X, the same pair in the same order or the other way round in both.  For X = 4, 8 the mirrored lane stands in, which holds the
@@ -187,26 +197,63 @@ __device__ __forceinline__ float affine(float xh, const W* gamma, const W* beta,
 }
 __device__ __forceinline__ float affine_r(float xh, float gamma, float beta) { return rounded_mul(xh, gamma) + beta; }
 
-// A vector of parameters in the order of a row: NT threads, each NV packs of V consecutive elements, pack i of thread t beginning at column (i NT + t) V.
-template <typename W, int NT, int NV, int V>
-__device__ __forceinline__ void load_parameter(const W* p, int cols, int t, float missing, float (&v)[NV][V]) {
+// A row of `cols` elements over NT threads, each NV packs of V consecutive elements: pack i of thread t begins at column (i NT + t) V.  A pack is one load or store at
+// any address of the element type (the hardware takes unaligned ones).  TAIL: cols need not be a multiple of V; the last pack then
+// goes element by element.  cols >= V.
+template <typename T, int V>
+struct __attribute__((packed, aligned(sizeof(T)))) LoosePack {
+  T e[V];
+};
+template <typename T, int NT, int NV, int V, bool TAIL>
+__device__ __forceinline__ void request_row(const T* p, int cols, int t, LoosePack<T, V> (&k)[NV]) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int at = (i * NT + t) * V, c = at < cols ? at : 0;
+  for (int i = 0; i < NV; ++i) k[i] = *reinterpret_cast<const LoosePack<T, V>*>(p + min((i * NT + t) * V, cols - V));   // (no branch: all of a thread's loads in flight at once)
+}
+// the cut pack: what was loaded are the row's last V elements, of which its first cols % V are the last ones; zeros behind them
+template <typename T, int NT, int NV, int V, bool TAIL>
+__device__ __forceinline__ void settle_row(int cols, int t, LoosePack<T, V> (&k)[NV]) {
+  if constexpr (TAIL) {
+    const int at = cols / V / NT, shift = V - cols % V;
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[i][j] = missing;
-    if (p) {
-      if constexpr (V * sizeof(W) <= 16) load_pack<W, V>(p + c, v[i]);
-      else {   // (16-bit rows with 32-bit parameters: two loads)
-        float lo[V / 2], hi[V / 2];
-        load_pack<W, V / 2>(p + c, lo);
-        load_pack<W, V / 2>(p + c + V / 2, hi);
+    for (int i = 0; i < NV; ++i)
+      if (i == at && (i * NT + t) * V + V > cols)
 #pragma unroll
-        for (int j = 0; j < V / 2; ++j) v[i][j] = lo[j], v[i][j + V / 2] = hi[j];
-      }
-    }
+        for (int by = 1; by < V; by *= 2)
+          if (shift & by)
+#pragma unroll
+            for (int j = 0; j < V; ++j) k[i].e[j] = j + by < V ? k[i].e[j + by] : (T)0.f;
   }
 }
+// f(i, column) for a thread's packs that begin inside the row (what the others hold is of no use)
+template <int NT, int NV, int V, typename F>
+__device__ __forceinline__ void each_pack(int cols, int t, F f) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * NT + t) * V;
+    if (c < cols) f(i, c);
+  }
+}
+template <typename T, int V, bool TAIL>
+__device__ __forceinline__ void store_row_pack(T* p, int c, int cols, const float (&v)[V]) {
+  LoosePack<T, V> k;
+#pragma unroll
+  for (int j = 0; j < V; ++j) k.e[j] = (T)v[j];
+  if (!TAIL || c + V <= cols) *reinterpret_cast<LoosePack<T, V>*>(p + c) = k;
+  else
+#pragma unroll
+    for (int j = 0; j < V - 1; ++j)
+      if (j < cols % V) p[c + j] = k.e[j];
+}
+// a vector of parameters in a row's order: its packs, if it is there
+template <typename W, int NT, int NV, int V, bool TAIL>
+struct Parameter {
+  LoosePack<W, V> k[NV];
+  __device__ __forceinline__ void load(const W* p, int cols, int t) {
+    if (!p) return;
+    request_row<W, NT, NV, V, TAIL>(p, cols, t, k);
+    settle_row<W, NT, NV, V, TAIL>(cols, t, k);
+  }
+};
 // pairwise: of equal values exactly
 template <int V>
 __device__ __forceinline__ float tree_sum(const float (&v)[V]) {
@@ -218,26 +265,27 @@ __device__ __forceinline__ float tree_sum(const float (&v)[V]) {
     return tree_sum(h);
   }
 }
-// mean and rstd of a row in registers, packs summed in f32 and their sums in f64; the row becomes x - mean
-template <int NT, int NV, int V>
+// mean and rstd of a row in registers, packs summed in f32 and their sums in f64; the row becomes x - mean (zeros past the end of a cut pack)
+template <int NT, int NV, int V, bool TAIL>
 __device__ __forceinline__ void centre_row(float (&v)[NV][V], int cols, int t, float eps, double* red, float& mean, float& rstd) {
   double s[1] = {0.};
-#pragma unroll
-  for (int i = 0; i < NV; ++i) s[0] += (double)tree_sum(v[i]);
+  each_pack<NT, NV, V>(cols, t, [&](int i, int) { s[0] += (double)tree_sum(v[i]); });
   team_sum<NT>(s, red);
-  mean = (float)(s[0] / cols);
+  const float m = (float)(s[0] / cols);
   s[0] = 0.;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
+  each_pack<NT, NV, V>(cols, t, [&](int i, int c) {
     float sq[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      v[i][j] = (i * NT + t) * V < cols ? v[i][j] - mean : 0.f;
-      sq[j] = rounded_mul(v[i][j], v[i][j]);   // (the same wherever it is inlined)
-    }
+    for (int j = 0; j < V; ++j) v[i][j] -= m;
+    if (TAIL && i == cols / V / NT)
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[i][j] = c + j < cols ? v[i][j] : 0.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) sq[j] = rounded_mul(v[i][j], v[i][j]);   // (the same wherever it is inlined)
     s[0] += (double)tree_sum(sq);
-  }
+  });
   team_sum<NT>(s, red + NT / 64);
+  mean = m;
   rstd = 1.f / sqrtf((float)(s[0] / cols) + eps);
 }
 constexpr int centre_lds(int nt) { return nt > 64 ? 2 * nt / 64 : 1; }   // doubles
