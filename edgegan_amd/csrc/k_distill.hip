@@ -99,18 +99,18 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // Tells the compiler that a pack may have changed: it then forms what follows from the pack again instead of keeping its converted elements and their
 // exponentials in registers from one pass over the row to the next.
 template <typename T, int V>
-__device__ __forceinline__ void opaque(Pack<T, V>& p) {
+__device__ __forceinline__ void opaque(LoosePack<T, V>& p) {
   if constexpr (sizeof(p) == 2) {
     unsigned u = __builtin_bit_cast(unsigned short, p);
     asm volatile("" : "+v"(u));
-    p = __builtin_bit_cast(Pack<T, V>, (unsigned short)u);
+    p = __builtin_bit_cast(LoosePack<T, V>, (unsigned short)u);
   } else {
     struct Words {
       unsigned w[sizeof(p) / 4];
     } k = __builtin_bit_cast(Words, p);
 #pragma unroll
     for (unsigned& w : k.w) asm volatile("" : "+v"(w));
-    p = __builtin_bit_cast(Pack<T, V>, k);
+    p = __builtin_bit_cast(LoosePack<T, V>, k);
   }
 }
 
@@ -122,7 +122,7 @@ struct RowMax {
   float m = -INFINITY;
   i16x2 hi = {-32768, -32768}, lo = {32767, 32767};
   template <int V>
-  __device__ __forceinline__ void take(const Pack<T, V>& p) {
+  __device__ __forceinline__ void take(const LoosePack<T, V>& p) {
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
       for (int j = 0; j < V; ++j) m = fmaxf(m, p.e[j]);
@@ -151,8 +151,8 @@ struct RowMax {
 };
 // A row in a team's registers.  A long row is alone in its registers: the teacher's part lies before the load and behind the
 // store (with it in between the compiler spilt the row).  The other block of a compute unit fills the waits.
-template <typename T, int NT, int NE, int V>
-__global__ __launch_bounds__(NT > 256 ? NT : 256) __attribute__((amdgpu_waves_per_eu(NT == 1024 && sizeof(T) == 2 && V > 1 ? 8 : 1))) void distill_rows(DistillArgs a) {
+template <typename T, int NT, int NE, int V, bool LOOSE>
+__global__ __launch_bounds__(NT > 256 ? NT : 256) __attribute__((amdgpu_waves_per_eu(NT == 1024 && sizeof(T) == 2 && !LOOSE ? 8 : 1))) void distill_rows(DistillArgs a) {
   constexpr int NB = NT > 256 ? NT : 256, TEAMS = NB / NT, NV = NE / V;
   __shared__ Kept all_kept[TEAMS][team_top(NT)];
   __shared__ float red_t[2][NT > 64 ? NT / 64 : 1], red[3][NT > 64 ? NT / 64 : 1];   // (one wave needs none)
@@ -166,25 +166,39 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) __attribute__((amdgpu_waves_pe
   const float w = (a.row_weight ? a.row_weight[r] : 1.f) * a.weight;
   const unsigned row_bytes = (unsigned)a.cols * sizeof(T);
   const __amdgpu_buffer_rsrc_t zb = row_buffer(z, row_bytes), gb = row_buffer(g, g ? row_bytes : 0);
-  Pack<T, V> v[NV];
+  LoosePack<T, V> v[NV];
+  // LOOSE: rows at any address, the last pack perhaps cut (filled up with -inf: e = 0). Else as a buffer. Packs past the end repeat the last one and are left out of
+  // the sum.
   auto load_row = [&] {
+    if constexpr (LOOSE) request_row<T, NT, NV, V>(z, a.cols, t, v);
+    else
 #pragma unroll
-    for (int i = 0; i < NV; ++i) v[i] = buffer_load<T, V>(zb, min((t + i * NT) * V, a.cols - V) * sizeof(T));   // (past the end: the last pack again, left out of the sum)
+      for (int i = 0; i < NV; ++i) v[i] = __builtin_bit_cast(LoosePack<T, V>, buffer_load<T, V>(zb, min((t + i * NT) * V, a.cols - V) * sizeof(T)));
+  };
+  auto store = [&](int i, int th, const float (&o)[V]) {
+    if constexpr (LOOSE) {
+      const int at = (th + i * NT) * V;
+      if (at < a.cols) store_row_pack<T, V, true>(g, at, a.cols, o);
+    } else
+      buffer_store<T, V>(gb, (th + i * NT) * V * sizeof(T), o);
   };
   constexpr bool EARLY = NE <= 16;   // few registers: the row is on its way while the teacher's part is worked on
   if constexpr (EARLY) load_row();
   float log_norm = 0.f;
   if (w == 0.f || !load_teacher<NT>(a, r, t, kept, red_t, it, log_norm)) {
+    if (g)
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const float zero[V] = {};
-      buffer_store<T, V>(gb, (t + i * NT) * V * sizeof(T), zero);
-    }
+      for (int i = 0; i < NV; ++i) {
+        const float zero[V] = {};
+        store(i, t, zero);
+      }
     if (t == 0) a.loss[r] = 0.f;
     return;
   }
   read_named<T, NT>(a, z, t, kept);
   if constexpr (!EARLY) load_row();
+  if constexpr (LOOSE && V > 1)
+    if (a.cols % V) settle_row<T, NT, NV, V, true>(a.cols, t, v, (T)-INFINITY);
   RowMax<T> most;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -218,7 +232,7 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) __attribute__((amdgpu_waves_pe
       float o[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) o[j] = (sizeof(T) == 4 ? (float)v[i].e[j] : __builtin_amdgcn_exp2f(((float)v[i].e[j] - m) * c)) * fi;
-      buffer_store<T, V>(gb, (t2 + i * NT) * V * sizeof(T), o);
+      store(i, t2, o);
       if constexpr (NE > 16) __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -236,13 +250,16 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) __attribute__((amdgpu_waves_pe
 constexpr int kChunkThreads = 256, kChunk = 8192;
 static int chunks_of(int cols) { return (cols + kChunk - 1) / kChunk; }
 
+// f(column, elements as a type): packs of V at any address, then what is left one by one
 template <int V, typename F>
 __device__ __forceinline__ void walk(int lo, int hi, F f) {
 #pragma unroll 4
-  for (int c = lo + threadIdx.x * V; c < hi; c += kChunkThreads * V) f(c);
+  for (int c = lo + threadIdx.x * V; c + V <= hi; c += kChunkThreads * V) f(c, std::integral_constant<int, V>{});
+  if ((int)threadIdx.x < (hi - lo) % V) f(hi - (hi - lo) % V + (int)threadIdx.x, std::integral_constant<int, 1>{});
 }
-template <typename T, int V>
+template <typename T>
 __global__ __launch_bounds__(kChunkThreads) void distill_chunk_sums(DistillArgs a, int chunks) {
+  constexpr int V = 16 / sizeof(T);
   __shared__ float red[2][kChunkThreads / 64];
   const float c = 1.f / a.temperature * kLog2e;
   const long long tasks = a.rows * chunks;
@@ -252,20 +269,18 @@ __global__ __launch_bounds__(kChunkThreads) void distill_chunk_sums(DistillArgs 
     const T* z = (const T*)a.logits + r * a.ld;
     float* out = a.partial + r * (2 * chunks + a.top);
     float m = -INFINITY;
-    walk<V>(lo, hi, [&](int at) {
-      float v[V];
-      load_pack<T, V>(z + at, v);
+    walk<V>(lo, hi, [&](int at, auto n) {
+      const auto k = *reinterpret_cast<const LoosePack<T, decltype(n)::value>*>(z + at);
 #pragma unroll
-      for (int j = 0; j < V; ++j) m = max_nan(m, v[j]);
+      for (int j = 0; j < decltype(n)::value; ++j) m = max_nan(m, (float)k.e[j]);
     });
     m = team_max<kChunkThreads>(m, red[0]);
     float s[1] = {0.f};
     if (m != -INFINITY)
-      walk<V>(lo, hi, [&](int at) {
-        float v[V];
-        load_pack<T, V>(z + at, v);
+      walk<V>(lo, hi, [&](int at, auto n) {
+        const auto k = *reinterpret_cast<const LoosePack<T, decltype(n)::value>*>(z + at);
 #pragma unroll
-        for (int j = 0; j < V; ++j) s[0] += __builtin_amdgcn_exp2f((v[j] - m) * c);
+        for (int j = 0; j < decltype(n)::value; ++j) s[0] += __builtin_amdgcn_exp2f(((float)k.e[j] - m) * c);
       });
     team_sum<kChunkThreads>(s, red[1]);
     if (threadIdx.x == 0) {
@@ -280,8 +295,9 @@ __global__ __launch_bounds__(kChunkThreads) void distill_chunk_sums(DistillArgs 
     __syncthreads();
   }
 }
-template <typename T, int V>
+template <typename T>
 __global__ __launch_bounds__(kChunkThreads) void distill_chunk_grad(DistillArgs a, int chunks) {
+  constexpr int V = 16 / sizeof(T);
   __shared__ Kept kept[kDistillTop];
   __shared__ float red_t[2][kChunkThreads / 64], red[3][kChunkThreads / 64];
   const int t = threadIdx.x;
@@ -316,12 +332,12 @@ __global__ __launch_bounds__(kChunkThreads) void distill_chunk_grad(DistillArgs 
     if (t == 0 && chunk == 0) a.loss[r] = w * a.temperature * a.temperature * loss;
     if (g) {
       const float f = w * a.temperature, fi = f / s[0];
-      walk<V>(lo, hi, [&](int at) {
-        float v[V], o[V];
-        load_pack<T, V>(z + at, v);
+      walk<V>(lo, hi, [&](int at, auto n) {
+        using P = LoosePack<T, decltype(n)::value>;
+        P k = *reinterpret_cast<const P*>(z + at);
 #pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = __builtin_amdgcn_exp2f((v[j] - m) * c) * fi;
-        store_pack<T, V>(g + at, o);
+        for (int j = 0; j < decltype(n)::value; ++j) k.e[j] = (T)(__builtin_amdgcn_exp2f(((float)k.e[j] - m) * c) * fi);
+        *reinterpret_cast<P*>(g + at) = k;
       });
       __syncthreads();
       write_named<T, kChunkThreads>(a, g, t, kept, f, [&](float z) { return it * (z - m) - log_sum; }, lo, hi);
@@ -337,25 +353,26 @@ size_t distill_partial_floats(long long rows, int cols, int top) {
   return distill_in_chunks(rows, cols) ? (size_t)rows * (2 * chunks_of(cols) + top) : 0;
 }
 
-template <typename T, int V>
+template <typename T, int NT, int NE, int V, bool LOOSE>
+static void distill_launch(const DistillArgs& a, hipStream_t s) {
+  constexpr int TEAMS = NT > 256 ? 1 : 256 / NT;
+  constexpr long long slab = 1 << 20;   // rows of a launch (a grid has fewer than 2^32 threads)
+  for (long long r = 0; r < a.rows; r += slab) {
+    DistillArgs p = a;
+    p.rows = std::min(slab, a.rows - r);
+    p.logits = (const T*)a.logits + r * a.ld;
+    p.index = (const char*)a.index + r * a.ld_index * (a.index64 ? 8 : 4);
+    p.teacher = a.teacher + r * a.ld_teacher;
+    if (a.row_weight) p.row_weight = a.row_weight + r;
+    p.loss = a.loss + r;
+    if (a.grad) p.grad = (T*)a.grad + r * a.ldg;
+    row_launch(distill_rows<T, NT, NE, V, LOOSE>, dim3((unsigned)((p.rows + TEAMS - 1) / TEAMS)), dim3(NT > 256 ? NT : 256), s, p);
+  }
+}
+template <typename T, bool LOOSE>
 static void distill_team(const DistillArgs& a, hipStream_t s) {
-  auto go = [&](auto nt, auto ne) {
-    constexpr int NT = decltype(nt)::value, NE = decltype(ne)::value, TEAMS = NT > 256 ? 1 : 256 / NT;
-    constexpr long long slab = 1 << 20;   // rows of a launch (a grid has fewer than 2^32 threads)
-    for (long long r = 0; r < a.rows; r += slab) {
-      DistillArgs p = a;
-      p.rows = std::min(slab, a.rows - r);
-      p.logits = (const T*)a.logits + r * a.ld;
-      p.index = (const char*)a.index + r * a.ld_index * (a.index64 ? 8 : 4);
-      p.teacher = a.teacher + r * a.ld_teacher;
-      if (a.row_weight) p.row_weight = a.row_weight + r;
-      p.loss = a.loss + r;
-      if (a.grad) p.grad = (T*)a.grad + r * a.ldg;
-      row_launch(distill_rows<T, NT, NE, V>, dim3((unsigned)((p.rows + TEAMS - 1) / TEAMS)), dim3(NT > 256 ? NT : 256), s, p);
-    }
-  };
-  using std::integral_constant;
-#define EG_TEAM(NT, NE) if (a.cols <= (NT) * (NE) && a.top <= team_top(NT)) return go(integral_constant<int, NT>{}, integral_constant<int, NE>{})
+  constexpr int V = 16 / sizeof(T);
+#define EG_TEAM(NT, NE) if (a.cols <= (NT) * (NE) && a.top <= team_top(NT)) return distill_launch<T, NT, NE, V, LOOSE>(a, s)
   EG_TEAM(64, 8);
   EG_TEAM(64, 16);
   EG_TEAM(256, 16);
@@ -368,20 +385,19 @@ static void distill_team(const DistillArgs& a, hipStream_t s) {
 
 void launch_distill(const DistillArgs& a, int type, hipStream_t s) {
   if (!a.rows) return;
-  EG_CHECK(a.top <= kDistillTop, "distillation: at most %d teacher logits a row", kDistillTop);
   by_type(type, [&](auto t) {
     using T = decltype(t);
-    auto go = [&](auto v) {
-      constexpr int V = decltype(v)::value;
-      if (!distill_in_chunks(a.rows, a.cols)) return distill_team<T, V>(a, s);
+    if (distill_in_chunks(a.rows, a.cols)) {
       const int chunks = chunks_of(a.cols);
-      row_launch(distill_chunk_sums<T, V>, dim3((unsigned)std::min<long long>(a.rows * chunks, 1 << 16)), dim3(kChunkThreads), s, a, chunks);
-      row_launch(distill_chunk_grad<T, V>, dim3((unsigned)std::min<long long>(a.rows * (a.grad ? chunks : 1), 1 << 16)), dim3(kChunkThreads), s, a, chunks);
-    };
+      row_launch(distill_chunk_sums<T>, dim3((unsigned)std::min<long long>(a.rows * chunks, 1 << 16)), dim3(kChunkThreads), s, a, chunks);
+      return row_launch(distill_chunk_grad<T>, dim3((unsigned)std::min<long long>(a.rows * (a.grad ? chunks : 1), 1 << 16)), dim3(kChunkThreads), s, a, chunks);
+    }
     constexpr int V = 16 / sizeof(T);
     const bool packs = a.cols % V == 0 && (uintptr_t)a.logits % 16 == 0 && a.ld * sizeof(T) % 16 == 0 && (!a.grad || ((uintptr_t)a.grad % 16 == 0 && a.ldg * sizeof(T) % 16 == 0));
-    if (packs) go(std::integral_constant<int, V>{});
-    else go(std::integral_constant<int, 1>{});
+    if (packs) distill_team<T, false>(a, s);
+    else if (a.cols >= V) distill_team<T, true>(a, s);
+    else if (a.top <= team_top(64)) distill_launch<T, 64, 8, 1, true>(a, s);   // (shorter than a pack)
+    else distill_launch<T, 256, 16, 1, true>(a, s);
   });
 }
 

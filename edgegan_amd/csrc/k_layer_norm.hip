@@ -34,7 +34,7 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_fwd(LayerNormArgs a) {
   const long long step = (long long)gridDim.x * TEAMS;
   long long r = (long long)blockIdx.x * TEAMS + team;
   LoosePack<T, V> next[NV];
-  if (r < a.rows) request_row<T, NT, NV, V, TAIL>((const T*)a.x + r * a.ldx, a.cols, t, next);
+  if (r < a.rows) request_row<T, NT, NV, V>((const T*)a.x + r * a.ldx, a.cols, t, next);
   for (; r < a.rows; r += step, turn ^= 1) {
     float v[NV][V], mean, rstd;
     settle_row<T, NT, NV, V, TAIL>(a.cols, t, next);
@@ -42,7 +42,7 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_fwd(LayerNormArgs a) {
 #pragma unroll
       for (int j = 0; j < V; ++j) v[i][j] = (float)next[i].e[j];
     });
-    if (r + step < a.rows) request_row<T, NT, NV, V, TAIL>((const T*)a.x + (r + step) * a.ldx, a.cols, t, next);
+    if (r + step < a.rows) request_row<T, NT, NV, V>((const T*)a.x + (r + step) * a.ldx, a.cols, t, next);
     if constexpr (!HELD) parameters();
     centre_row<NT, NV, V, TAIL>(v, a.cols, t, a.eps, red[turn], mean, rstd);
     T* y = (T*)a.y + r * a.ldy;
@@ -87,10 +87,14 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_bwd(LayerNormGradArgs 
   LoosePack<T, V> next_x[NV], next_d[NV];
   float next_mean = 0.f, next_rstd = 0.f;
   auto request = [&](long long row) {
-    request_row<T, NT, NV, V, TAIL>((const T*)a.x + row * a.ldx, a.cols, t, next_x);
-    request_row<T, NT, NV, V, TAIL>((const T*)a.dy + row * a.lddy, a.cols, t, next_d);
+    request_row<T, NT, NV, V>((const T*)a.x + row * a.ldx, a.cols, t, next_x);
+    request_row<T, NT, NV, V>((const T*)a.dy + row * a.lddy, a.cols, t, next_d);
     next_mean = a.mean[row];
     next_rstd = a.rstd[row];
+  };
+  auto all_packs = [&](auto f) {   // (those past the end too: d = 0 there, and a branch for each would part the loads from their use)
+#pragma unroll
+    for (int i = 0; i < NV; ++i) f(i);
   };
   if (r < a.rows) request(r);
   for (; r < a.rows; r += step, turn ^= 1) {
@@ -98,11 +102,11 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_bwd(LayerNormGradArgs 
     settle_row<T, NT, NV, V, TAIL>(a.cols, t, next_x);
     settle_row<T, NT, NV, V, TAIL>(a.cols, t, next_d);   // (d = 0 past the end: reaches no sum)
     const float mean = next_mean, rstd = next_rstd;
-    each_pack<NT, NV, V>(a.cols, t, [&](int i, int) {
+    all_packs([&](int i) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         x[i][j] = rounded_mul((float)next_x[i].e[j] - mean, rstd);
-        d[i][j] = (float)next_d[i].e[j];
+        d[i][j] = (i * NT + t) * V < a.cols ? (float)next_d[i].e[j] : 0.f;
       }
     });
     if (r + step < a.rows) request(r + step);   // (in flight while this row is summed and stored)
@@ -110,7 +114,7 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_bwd(LayerNormGradArgs 
       Parameter<W, NT, NV, V, TAIL> beta;
       beta.load((const W*)a.beta, a.cols, t);
       const float below = a.act == ACT_LRELU ? 0.2f : 0.f;
-      each_pack<NT, NV, V>(a.cols, t, [&](int i, int) {
+      all_packs([&](int i) {
         float z[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) z[j] = a.gamma ? rounded_mul(x[i][j], (float)gamma.k[i].e[j]) : x[i][j];
@@ -122,7 +126,7 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_bwd(LayerNormGradArgs 
       });
     }
     float s[2] = {0.f, 0.f};
-    each_pack<NT, NV, V>(a.cols, t, [&](int i, int) {
+    all_packs([&](int i) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         sg[i][j] += d[i][j];
@@ -216,7 +220,7 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void quantize_rows(QuantizeArg
   int turn = 0;
   for (long long r = (long long)blockIdx.x * TEAMS + team; r < a.rows; r += (long long)gridDim.x * TEAMS, turn ^= 1) {
     LoosePack<T, V> k[NV];
-    request_row<T, NT, NV, V, TAIL>((const T*)a.x + r * a.ldx, a.cols, t, k);
+    request_row<T, NT, NV, V>((const T*)a.x + r * a.ldx, a.cols, t, k);
     settle_row<T, NT, NV, V, TAIL>(a.cols, t, k);
     float v[NV][V];
     each_pack<NT, NV, V>(a.cols, t, [&](int i, int) {

@@ -195,7 +195,6 @@ __device__ __forceinline__ float affine(float xh, const W* gamma, const W* beta,
   const float z = gamma ? rounded_mul(xh, (float)gamma[c]) : xh;
   return beta ? z + (float)beta[c] : z;
 }
-__device__ __forceinline__ float affine_r(float xh, float gamma, float beta) { return rounded_mul(xh, gamma) + beta; }
 
 // A row of `cols` elements over NT threads, each NV packs of V consecutive elements: pack i of thread t begins at column (i NT + t) V.  A pack is one load or store at
 // any address of the element type (the hardware takes unaligned ones).  TAIL: cols need not be a multiple of V; the last pack then
@@ -204,14 +203,14 @@ template <typename T, int V>
 struct __attribute__((packed, aligned(sizeof(T)))) LoosePack {
   T e[V];
 };
-template <typename T, int NT, int NV, int V, bool TAIL>
+template <typename T, int NT, int NV, int V>
 __device__ __forceinline__ void request_row(const T* p, int cols, int t, LoosePack<T, V> (&k)[NV]) {
 #pragma unroll
   for (int i = 0; i < NV; ++i) k[i] = *reinterpret_cast<const LoosePack<T, V>*>(p + min((i * NT + t) * V, cols - V));   // (no branch: all of a thread's loads in flight at once)
 }
-// the cut pack: what was loaded are the row's last V elements, of which its first cols % V are the last ones; zeros behind them
+// the cut pack: what was loaded are the row's last V elements, of which its first cols % V are the last ones; `fill` behind them
 template <typename T, int NT, int NV, int V, bool TAIL>
-__device__ __forceinline__ void settle_row(int cols, int t, LoosePack<T, V> (&k)[NV]) {
+__device__ __forceinline__ void settle_row(int cols, int t, LoosePack<T, V> (&k)[NV], T fill = (T)0.f) {
   if constexpr (TAIL) {
     const int at = cols / V / NT, shift = V - cols % V;
 #pragma unroll
@@ -221,7 +220,7 @@ __device__ __forceinline__ void settle_row(int cols, int t, LoosePack<T, V> (&k)
         for (int by = 1; by < V; by *= 2)
           if (shift & by)
 #pragma unroll
-            for (int j = 0; j < V; ++j) k[i].e[j] = j + by < V ? k[i].e[j + by] : (T)0.f;
+            for (int j = 0; j < V; ++j) k[i].e[j] = j + by < V ? k[i].e[j + by] : fill;
   }
 }
 // f(i, column) for a thread's packs that begin inside the row (what the others hold is of no use)
@@ -250,7 +249,7 @@ struct Parameter {
   LoosePack<W, V> k[NV];
   __device__ __forceinline__ void load(const W* p, int cols, int t) {
     if (!p) return;
-    request_row<W, NT, NV, V, TAIL>(p, cols, t, k);
+    request_row<W, NT, NV, V>(p, cols, t, k);
     settle_row<W, NT, NV, V, TAIL>(cols, t, k);
   }
 };
