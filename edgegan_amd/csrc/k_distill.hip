@@ -5,7 +5,8 @@
 // of weight 0 have loss 0 and gradient 0, whatever the student's logits are.
 //
 // Bound by HBM: one read and one write of the logits.  A row stays in the registers of its team (a wave, 256 or 1,024 threads, at most 64 elements each) from
-// the load through maximum and sum to the store: in 16 bits as loaded (half the registers: two rows of 65,536 a compute unit; the exponentials are taken twice), in
+// the load through maximum and sum to the store: in 16 bits as loaded (half the registers: two rows of
+// 65,536 a compute unit; the exponentials are taken twice), in
 // 32 bits as exponentials.  The few columns that the teacher names are corrected
 // behind the store of the row by the threads that hold the teacher's entries, in the same block.  exp((z - m) / T) is 2^((z - m) c): the difference
 // first, so that rows of the type's lowest value stay finite.
@@ -151,8 +152,8 @@ struct RowMax {
 };
 // A row in a team's registers.  A long row is alone in its registers: the teacher's part lies before the load and behind the
 // store (with it in between the compiler spilt the row).  The other block of a compute unit fills the waits.
-template <typename T, int NT, int NE, int V, bool LOOSE>
-__global__ __launch_bounds__(NT > 256 ? NT : 256) __attribute__((amdgpu_waves_per_eu(NT == 1024 && sizeof(T) == 2 && !LOOSE ? 8 : 1))) void distill_rows(DistillArgs a) {
+template <typename T, int NT, int NE, int V>
+__global__ __launch_bounds__(NT > 256 ? NT : 256) void distill_rows(DistillArgs a) {
   constexpr int NB = NT > 256 ? NT : 256, TEAMS = NB / NT, NV = NE / V;
   __shared__ Kept all_kept[TEAMS][team_top(NT)];
   __shared__ float red_t[2][NT > 64 ? NT / 64 : 1], red[3][NT > 64 ? NT / 64 : 1];   // (one wave needs none)
@@ -164,23 +165,11 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) __attribute__((amdgpu_waves_pe
   const T* z = (const T*)a.logits + r * a.ld;
   T* g = a.grad ? (T*)a.grad + r * a.ldg : nullptr;
   const float w = (a.row_weight ? a.row_weight[r] : 1.f) * a.weight;
-  const unsigned row_bytes = (unsigned)a.cols * sizeof(T);
-  const __amdgpu_buffer_rsrc_t zb = row_buffer(z, row_bytes), gb = row_buffer(g, g ? row_bytes : 0);
   LoosePack<T, V> v[NV];
-  // LOOSE: rows at any address, the last pack perhaps cut (filled up with -inf: e = 0). Else as a buffer. Packs past the end repeat the last one and are left out of
-  // the sum.
-  auto load_row = [&] {
-    if constexpr (LOOSE) request_row<T, NT, NV, V>(z, a.cols, t, v);
-    else
-#pragma unroll
-      for (int i = 0; i < NV; ++i) v[i] = __builtin_bit_cast(LoosePack<T, V>, buffer_load<T, V>(zb, min((t + i * NT) * V, a.cols - V) * sizeof(T)));
-  };
+  auto load_row = [&] { request_row<T, NT, NV, V>(z, a.cols, t, v); };   // (packs past the end repeat the last ones: left out of the sum)
   auto store = [&](int i, int th, const float (&o)[V]) {
-    if constexpr (LOOSE) {
-      const int at = (th + i * NT) * V;
-      if (at < a.cols) store_row_pack<T, V, true>(g, at, a.cols, o);
-    } else
-      buffer_store<T, V>(gb, (th + i * NT) * V * sizeof(T), o);
+    const int at = (th + i * NT) * V;
+    if (at < a.cols) store_row_pack<T, V, true>(g, at, a.cols, o);
   };
   constexpr bool EARLY = NE <= 16;   // few registers: the row is on its way while the teacher's part is worked on
   if constexpr (EARLY) load_row();
@@ -197,8 +186,7 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) __attribute__((amdgpu_waves_pe
   }
   read_named<T, NT>(a, z, t, kept);
   if constexpr (!EARLY) load_row();
-  if constexpr (LOOSE && V > 1)
-    if (a.cols % V) settle_row<T, NT, NV, V, true>(a.cols, t, v, (T)-INFINITY);
+  if (V > 1 && a.cols % V) settle_row<T, NT, NV, V, true>(a.cols, t, v, (T)-INFINITY);
   RowMax<T> most;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -353,7 +341,7 @@ size_t distill_partial_floats(long long rows, int cols, int top) {
   return distill_in_chunks(rows, cols) ? (size_t)rows * (2 * chunks_of(cols) + top) : 0;
 }
 
-template <typename T, int NT, int NE, int V, bool LOOSE>
+template <typename T, int NT, int NE, int V>
 static void distill_launch(const DistillArgs& a, hipStream_t s) {
   constexpr int TEAMS = NT > 256 ? 1 : 256 / NT;
   constexpr long long slab = 1 << 20;   // rows of a launch (a grid has fewer than 2^32 threads)
@@ -366,13 +354,13 @@ static void distill_launch(const DistillArgs& a, hipStream_t s) {
     if (a.row_weight) p.row_weight = a.row_weight + r;
     p.loss = a.loss + r;
     if (a.grad) p.grad = (T*)a.grad + r * a.ldg;
-    row_launch(distill_rows<T, NT, NE, V, LOOSE>, dim3((unsigned)((p.rows + TEAMS - 1) / TEAMS)), dim3(NT > 256 ? NT : 256), s, p);
+    row_launch(distill_rows<T, NT, NE, V>, dim3((unsigned)((p.rows + TEAMS - 1) / TEAMS)), dim3(NT > 256 ? NT : 256), s, p);
   }
 }
-template <typename T, bool LOOSE>
+template <typename T>
 static void distill_team(const DistillArgs& a, hipStream_t s) {
   constexpr int V = 16 / sizeof(T);
-#define EG_TEAM(NT, NE) if (a.cols <= (NT) * (NE) && a.top <= team_top(NT)) return distill_launch<T, NT, NE, V, LOOSE>(a, s)
+#define EG_TEAM(NT, NE) if (a.cols <= (NT) * (NE) && a.top <= team_top(NT)) return distill_launch<T, NT, NE, V>(a, s)
   EG_TEAM(64, 8);
   EG_TEAM(64, 16);
   EG_TEAM(256, 16);
@@ -393,11 +381,9 @@ void launch_distill(const DistillArgs& a, int type, hipStream_t s) {
       return row_launch(distill_chunk_grad<T>, dim3((unsigned)std::min<long long>(a.rows * (a.grad ? chunks : 1), 1 << 16)), dim3(kChunkThreads), s, a, chunks);
     }
     constexpr int V = 16 / sizeof(T);
-    const bool packs = a.cols % V == 0 && (uintptr_t)a.logits % 16 == 0 && a.ld * sizeof(T) % 16 == 0 && (!a.grad || ((uintptr_t)a.grad % 16 == 0 && a.ldg * sizeof(T) % 16 == 0));
-    if (packs) distill_team<T, false>(a, s);
-    else if (a.cols >= V) distill_team<T, true>(a, s);
-    else if (a.top <= team_top(64)) distill_launch<T, 64, 8, 1, true>(a, s);   // (shorter than a pack)
-    else distill_launch<T, 256, 16, 1, true>(a, s);
+    if (a.cols >= V) distill_team<T>(a, s);
+    else if (a.top <= team_top(64)) distill_launch<T, 64, 8, 1>(a, s);   // (shorter than a pack)
+    else distill_launch<T, 256, 16, 1>(a, s);
   });
 }
 

@@ -147,20 +147,6 @@ template <typename T, int V>
 struct alignas(sizeof(T) * V) Pack {
   T e[V];
 };
-template <typename T, int V>
-__device__ __forceinline__ void load_pack(const T* p, float (&v)[V]) {
-  const Pack<T, V> k = *reinterpret_cast<const Pack<T, V>*>(p);
-#pragma unroll
-  for (int i = 0; i < V; ++i) v[i] = (float)k.e[i];
-}
-template <typename T, int V>
-__device__ __forceinline__ void store_pack(T* p, const float (&v)[V]) {
-  Pack<T, V> k;
-#pragma unroll
-  for (int i = 0; i < V; ++i) k.e[i] = (T)v[i];
-  *reinterpret_cast<Pack<T, V>*>(p) = k;
-}
-
 // A row as a buffer of its own: a load past its end gives zero and a store there is dropped, and an element's address is one register. The row
 // has to be the same one for the whole wave.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t row_buffer(const void* p, unsigned bytes) {
