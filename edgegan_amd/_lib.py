@@ -54,7 +54,7 @@ class Config:
     use_edge_discriminator: bool = True    # train.py:65-66
     image_dis_size: Optional[int] = None   # train.py:63-64 (None: dis_size)
     edge_dis_size: Optional[int] = None    # train.py:67    (None: dis_size)
-    E_norm: Optional[str] = 'instance'   # train.py:54-59: 'instance' | 'batch' | None (nn/modules/normalization.py:10-29)
+    E_norm: Optional[str] = 'instance'   # train.py:54-59: 'instance' | 'batch' | None (nn/modules/normalization.py:10-29), 'layernorm'
     G_norm: Optional[str] = 'instance'
     D_norm: Optional[str] = 'instance'
 
@@ -83,7 +83,7 @@ class Config:
                         _NORMS[self.E_norm], _NORMS[self.G_norm], _NORMS[self.D_norm])
 
 
-_NORMS = {'instance': 0, 'batch': 1, None: 2}   # (None: the identity branch, normalization.py:26-27)
+_NORMS = {'instance': 0, 'batch': 1, None: 2, 'layernorm': 3}   # (None: the identity branch, normalization.py:26-27; 'layernorm': no reference value)
 
 
 def _dtype_override(dtype: str) -> str:
@@ -104,7 +104,7 @@ EXPORTS = ['eg_default_config', 'eg_variable_count', 'eg_variable_info', 'eg_cre
            'eg_last_error', 'eg_set_variable', 'eg_get_variable', 'eg_upload_batch', 'eg_substep',
            'eg_train_step', 'eg_train_batch', 'eg_losses_wait', 'eg_read_losses', 'eg_eval_losses', 'eg_infer', 'eg_infer_upload', 'eg_infer_run', 'eg_infer_download', 'eg_sync', 'eg_comm_unique_id', 'eg_comm_init',
            'eg_comm_reduce_scalars', 'eg_comm_info', 'eg_comm_timing', 'eg_comm_timing_read',
-           'eg_profile_begin', 'eg_profile_end', 'eg_profile_layers', 'eg_memory_stats', 'eg_mfma_probe', 'eg_test_op', 'eg_net_forward', 'eg_crc32c',
+           'eg_profile_begin', 'eg_profile_end', 'eg_profile_layers', 'eg_memory_stats', 'eg_mfma_probe', 'eg_test_op', 'eg_net_forward', 'eg_crc32c', 'eg_set_teacher', 'eg_teacher_loss', 'eg_infer_precision',
            'eg_layer_norm', 'eg_layer_norm_workspace', 'eg_layer_norm_backward', 'eg_quantize_rows', 'eg_int8_matmul',
            'eg_int8_linear_workspace', 'eg_int8_linear', 'eg_distill_loss_workspace', 'eg_distill_loss']
 
@@ -157,6 +157,9 @@ def load_library() -> C.CDLL:
                                C.c_int, C.POINTER(fp), C.POINTER(C.c_longlong)]
     lib.eg_net_forward.argtypes = [C.c_void_p, C.c_char_p, fp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_float, fp,
                                    C.c_longlong]
+    lib.eg_set_teacher.argtypes = [C.c_void_p, ip, fp, C.c_int, C.c_float, C.c_float]
+    lib.eg_teacher_loss.argtypes = [C.c_void_p, fp]
+    lib.eg_infer_precision.argtypes = [C.c_void_p, C.c_int]
     lib.eg_crc32c.restype = C.c_uint
     lib.eg_crc32c.argtypes = [C.c_uint, C.c_void_p, C.c_ulonglong]
     # operators over rows in device memory: pointers as plain addresses

@@ -1,5 +1,6 @@
 // C ABI of libedgegan_hip.so (see include/edgegan_hip.h).  Translates exceptions to error codes.
 #include <algorithm>
+#include <cmath>
 #include <cstdlib>
 #include <sstream>
 
@@ -43,14 +44,17 @@ static Config to_config(const eg_config* k) {
   c.device = k->device;
   c.bf16 = k->compute_dtype == 1;
   c.x3 = k->compute_dtype == 2;
-  EG_CHECK((unsigned)k->e_norm <= 2u && (unsigned)k->g_norm <= 2u && (unsigned)k->d_norm <= 2u,
-           "e_norm / g_norm / d_norm: 0 = instance, 1 = batch, 2 = None");
+  EG_CHECK((unsigned)k->e_norm <= 3u && (unsigned)k->g_norm <= 3u && (unsigned)k->d_norm <= 3u,
+           "e_norm / g_norm / d_norm: 0 = instance, 1 = batch, 2 = None, 3 = layernorm");
   c.e_bn = k->e_norm == 1;
   c.g_bn = k->g_norm == 1;
   c.d_bn = k->d_norm == 1;
   c.e_nonorm = k->e_norm == 2;
   c.g_nonorm = k->g_norm == 2;
   c.d_nonorm = k->d_norm == 2;
+  c.e_ln = k->e_norm == 3;
+  c.g_ln = k->g_norm == 3;
+  c.d_ln = k->d_norm == 3;
   return c;
 }
 
@@ -287,6 +291,51 @@ int eg_train_batch(eg_ctx* ctx, const float* images, const float* z, const float
   EG_API_END(ctx)
 }
 
+int eg_set_teacher(eg_ctx* ctx, const int* index, const float* logits, int top, float temperature, float weight) {
+  EG_API_BEGIN_CTX(ctx)
+  Ctx& c = ctx->c;
+  comm_wait_all(c);
+  const int B = c.cfg.B;
+  EG_CHECK(c.cfg.multiclasses(), "eg_set_teacher: there is no classifier without classes");
+  EG_CHECK(top >= 0 && top <= 1024, "eg_set_teacher: top = %d (0 .. 1024)", top);
+  EG_CHECK(top == 0 || (index && logits), "eg_set_teacher: null argument");
+  EG_CHECK(top == 0 || (temperature > 0.f && std::isfinite(temperature) && std::isfinite(1.f / temperature) && std::isfinite(weight)),
+           "eg_set_teacher: temperature %g, weight %g", temperature, weight);
+  EG_HIP(hipDeviceSynchronize());   // (a classifier sub-step in flight on another lane may read the old ones)
+  c.teacher_top = 0;
+  if (top == 0) return 0;
+  if (top > c.teacher_cap) {
+    (void)hipFree(c.teacher_index);
+    (void)hipFree(c.teacher_logits);
+    c.teacher_index = nullptr;
+    c.teacher_logits = nullptr;
+    c.teacher_cap = 0;
+    EG_HIP(hipMalloc(&c.teacher_index, (size_t)B * top * 4));
+    EG_HIP(hipMalloc(&c.teacher_logits, (size_t)B * top * 4));
+    c.teacher_cap = top;
+  }
+  if (!c.teacher_loss) EG_HIP(hipMalloc(&c.teacher_loss, (size_t)(B + 1) * 4));
+  EG_HIP(hipMemcpyAsync(c.teacher_index, index, (size_t)B * top * 4, hipMemcpyHostToDevice, c.stream));
+  EG_HIP(hipMemcpyAsync(c.teacher_logits, logits, (size_t)B * top * 4, hipMemcpyHostToDevice, c.stream));
+  launch_fill(c.teacher_loss, 0.f, B + 1, c.stream);
+  EG_HIP(hipStreamSynchronize(c.stream));
+  c.teacher_top = top;
+  c.teacher_temperature = temperature;
+  c.teacher_weight = weight;
+  EG_API_END(ctx)
+}
+
+int eg_teacher_loss(eg_ctx* ctx, float* out) {
+  EG_API_BEGIN_CTX(ctx)
+  Ctx& c = ctx->c;
+  EG_CHECK(out, "eg_teacher_loss: null argument");
+  EG_CHECK(c.teacher_top > 0, "eg_teacher_loss: no teacher is set");
+  comm_wait_all(c);
+  EG_HIP(hipDeviceSynchronize());
+  EG_HIP(hipMemcpy(out, c.teacher_loss, 4, hipMemcpyDeviceToHost));
+  EG_API_END(ctx)
+}
+
 int eg_losses_wait(eg_ctx* ctx, int back, float* out12) {
   EG_API_BEGIN
   Ctx& c = ctx->c;
@@ -365,6 +414,14 @@ static void infer_reserve(Ctx& c, int nb) {
   EG_HIP(hipMalloc(&c.inf_cls, (size_t)nb * 4));
   if (!c.inf_eps) EG_HIP(hipMalloc(&c.inf_eps, 8));
   c.inf_cap = nb;
+}
+
+int eg_infer_precision(eg_ctx* ctx, int bits) {
+  EG_API_BEGIN_CTX(ctx)
+  EG_CHECK(bits == 0 || bits == 8, "eg_infer_precision: %d (0: as compute_dtype, 8)", bits);
+  ctx->c.inf_int8 = bits == 8;
+  ctx->c.inf_warm = false;   // (the next run builds the 8-bit filters and is waited for)
+  EG_API_END(ctx)
 }
 
 int eg_infer_upload(eg_ctx* ctx, const float* images, const int* classes, int nb, const float* eps2) {

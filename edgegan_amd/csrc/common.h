@@ -229,7 +229,11 @@ struct Param {
   bool wM_valid = false;
   // bf16 limb planes of a filter (k_gemm_x3.hip), K-step-major, [0] as stored / [1] per-tap transposed; same life cycle
   LimbCache wL[2];
-  void invalidate_derived() { wT_valid = wM_valid = wL[0].valid = wL[1].valid = false; }
+  // 8-bit rows of a dense filter's transpose, one scale for each output channel (inference in 8 bits: model.cpp dense8), same life cycle
+  signed char* q8 = nullptr;
+  float* q8_scale = nullptr;
+  bool q8_valid = false;
+  void invalidate_derived() { wT_valid = wM_valid = wL[0].valid = wL[1].valid = q8_valid = false; }
 };
 
 struct Ctx;

@@ -4,6 +4,7 @@
 
 #include "common.h"
 #include "kernels.h"
+#include "rowops.h"
 
 namespace eg {
 
@@ -19,6 +20,10 @@ struct Config {
   bool bf16 = false;  // dense contractions on the bf16 MFMA (operands rounded, fp32 accumulate / storage)
   bool x3 = false;    // fp32 contractions as three-limb bf16 splits on the bf16 MFMA (exact limb products, fp32 accumulate)
   bool e_bn = false, g_bn = false, d_bn = false;   // E_norm / G_norm / D_norm == 'batch' (train.py:54-59; default 'instance')
+  bool e_ln = false, g_ln = false, d_ln = false;   // ... == 'layernorm': over the channels of each position, learned scale / shift
+  bool e_in() const { return !e_bn && !e_nonorm && !e_ln; }
+  bool g_in_norm() const { return !g_bn && !g_nonorm && !g_ln; }
+  bool d_in() const { return !d_bn && !d_nonorm && !d_ln; }
   bool e_nonorm = false, g_nonorm = false, d_nonorm = false;   // ... == None: the block's norm is the identity (normalization.py:26-27)
   bool multiclasses() const { return num_classes > 0; }
   int g_in() const { return z_dim + (multiclasses() ? num_classes : 0); }
@@ -197,6 +202,12 @@ struct Ctx {
   std::vector<hipStream_t> placeholder_streams;   // model.cpp: stream -> hardware queue placement
   hipEvent_t ev_fork = nullptr, ev_gen = nullptr, ev_g1fwd = nullptr, ev_branch = nullptr, ev_cls = nullptr;
 
+  // teacher of the classifier (eg_set_teacher): its top logits of the resident batch, [B][top]
+  int* teacher_index = nullptr;
+  float *teacher_logits = nullptr, *teacher_loss = nullptr;   // teacher_loss: [1 + B], the sum and the rows' terms of the last sub-step 4
+  int teacher_top = 0, teacher_cap = 0;
+  float teacher_temperature = 1.f, teacher_weight = 0.f;
+
   // inference staging buffers (host <-> device hand-over of eg_infer), grown on demand and kept
   // Consecutive eg_infer_run calls on a resident batch are independent of one another: they rotate over kInferSlots slots
   // (own lanes = streams + arenas, own output buffers), so several calls are in flight at once and their small launches
@@ -213,6 +224,8 @@ struct Ctx {
   hipEvent_t ev_infer[kLanes] = {};   // fork event of the call whose main lane is i
   bool inf_inflight = false;   // eg_infer_run calls may still be running on lanes other than 0: every OTHER entry point drains them first (api_enter)
   bool inf_entering = false;   // ... set by eg_infer_run around its own api_enter
+  bool inf_int8 = false;       // eg_infer_precision: 8-bit operands for the dense layers of the inference graph
+  bool int8_now = false;       //   ... while such a graph is built
   bool inf_warm = false;       // the weights' lazily built derived copies (transposes, bf16 planes) are all in place: set by the first
                                // completed run, cleared whenever a variable changes -- until then a run is followed by a device sync
 
@@ -311,6 +324,12 @@ float* in_chunk_scratch(Ctx& c, int NB, int HW, int C);   // ops.cpp: scratch of
 T bn_relu(Ctx& c, T x, Param* gamma, Param* beta, Param* mm, Param* mv, int update_times, T* stats_out = nullptr);
 T bn_act(Ctx& c, T x, Param* gamma, Param* beta, Param* mm, Param* mv, int act, int update_times, T* stats_out = nullptr);
 T bn_act_tangent(Ctx& c, T tx, T x_prim, T out_prim, T stats_prim, Param* gamma, int act);
+// layer norm over the channels of each position, learned scale / shift, then the activation (E_norm / G_norm / D_norm = 'layernorm').  stats_out: [mean of every
+// position | 1 / sqrt(var + eps)] for the tangent pass
+T ln_act(Ctx& c, T x, Param* gamma, Param* beta, int act, T* stats_out = nullptr);
+T ln_act_tangent(Ctx& c, T tx, T x_prim, T stats_prim, Param* gamma, Param* beta, int act);
+// y = x w + bias with both operands in 8 bits (rows = positions: a linear layer or a 1x1 convolution), forward-only graphs
+T dense8(Ctx& c, T x, Param* w, Param* bias);
 T add(Ctx& c, T a, T b, bool relu);
 T pool2(Ctx& c, T x);
 T add_relu_pool2(Ctx& c, T a, T b);   // pool2(relu(a + b)): one pass in forward-only graphs

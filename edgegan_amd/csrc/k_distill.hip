@@ -387,4 +387,17 @@ void launch_distill(const DistillArgs& a, int type, hipStream_t s) {
   });
 }
 
+__global__ __launch_bounds__(256) void distill_join(const float* more, float* grad, int n, const float* loss, int rows, float* total) {
+  __shared__ float red[4];
+  for (int i = blockIdx.x * 256 + threadIdx.x; i < n; i += gridDim.x * 256) grad[i] += more[i];
+  if (blockIdx.x) return;
+  float s[1] = {0.f};
+  for (int r = threadIdx.x; r < rows; r += 256) s[0] += loss[r];
+  team_sum<256>(s, red);
+  if (threadIdx.x == 0) *total = s[0];
+}
+void launch_distill_join(const float* more, float* grad, int n, const float* loss, int rows, float* total, hipStream_t s) {
+  row_launch(distill_join, dim3((unsigned)std::min((n + 255) / 256, 256)), dim3(256), s, more, grad, n, loss, rows, total);
+}
+
 }  // namespace eg

@@ -68,6 +68,42 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_fwd(LayerNormArgs a) {
   }
 }
 
+// A block's sums of the parameter gradients to its row of partial [blocks][2][cols]; several teams of a block add up in their order.
+template <int NT, int NV, int V, int TEAMS>
+__device__ __forceinline__ void leave_partial(float* partial, int cols, int t, int team, const float (&sx)[NV][V], const float (&sg)[NV][V]) {
+  float* out = partial + (size_t)blockIdx.x * 2 * cols;
+  if constexpr (TEAMS > 1) {
+    __shared__ float sum[2][NT * NV * V];
+    for (int k = 0; k < TEAMS; ++k) {
+      if (team == k)
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const int c = (i * NT + t) * V + j;
+            sum[0][c] = (k ? sum[0][c] : 0.f) + sx[i][j];
+            sum[1][c] = (k ? sum[1][c] : 0.f) + sg[i][j];
+          }
+      __syncthreads();
+    }
+    for (int c = threadIdx.x; c < cols; c += NT * TEAMS) {
+      out[c] = sum[0][c];
+      out[cols + c] = sum[1][c];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * NT + t) * V;
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (c + j < cols) {
+          out[c + j] = sx[i][j];
+          out[cols + c + j] = sg[i][j];
+        }
+    }
+  }
+}
+
 template <typename T, typename W, int NT, int NV, int V, bool TAIL>
 __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_bwd(LayerNormGradArgs a) {
   constexpr int NB = NT > 256 ? NT : 256, TEAMS = NB / NT;
@@ -113,7 +149,6 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_bwd(LayerNormGradArgs 
     if (a.act != ACT_NONE) {
       Parameter<W, NT, NV, V, TAIL> beta;
       beta.load((const W*)a.beta, a.cols, t);
-      const float below = a.act == ACT_LRELU ? 0.2f : 0.f;
       all_packs([&](int i) {
         float z[V];
 #pragma unroll
@@ -122,7 +157,7 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_bwd(LayerNormGradArgs 
 #pragma unroll
           for (int j = 0; j < V; ++j) z[j] += (float)beta.k[i].e[j];
 #pragma unroll
-        for (int j = 0; j < V; ++j) d[i][j] = z[j] > 0.f ? d[i][j] : below * d[i][j];
+        for (int j = 0; j < V; ++j) d[i][j] *= row_act_grad(z[j], a.act);
       });
     }
     float s[2] = {0.f, 0.f};
@@ -151,38 +186,7 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_bwd(LayerNormGradArgs 
       store_row_pack<T, V, TAIL>(dx, c, a.cols, d[i]);
     });
   }
-  if (!a.partial) return;
-  float* out = a.partial + (size_t)blockIdx.x * 2 * a.cols;
-  if constexpr (TEAMS > 1) {   // the block's teams add up in their order
-    __shared__ float sum[2][NT * NV * V];
-    for (int k = 0; k < TEAMS; ++k) {
-      if (team == k)
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const int c = (i * NT + t) * V + j;
-            sum[0][c] = (k ? sum[0][c] : 0.f) + sx[i][j];
-            sum[1][c] = (k ? sum[1][c] : 0.f) + sg[i][j];
-          }
-      __syncthreads();
-    }
-    for (int c = threadIdx.x; c < a.cols; c += NB) {
-      out[c] = sum[0][c];
-      out[a.cols + c] = sum[1][c];
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * NT + t) * V;
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (c + j < a.cols) {
-          out[c + j] = sx[i][j];
-          out[a.cols + c + j] = sg[i][j];
-        }
-    }
-  }
+  if (a.partial) leave_partial<NT, NV, V, TEAMS>(a.partial, a.cols, t, team, sx, sg);
 }
 
 // partial [groups][2][cols] -> dgamma, dbeta: a block adds 32 of the 2 cols sums, 32 threads each every 32nd group
@@ -204,7 +208,7 @@ __global__ __launch_bounds__(1024) void ln_bwd_finish(const float* partial, int 
   W* out = i < cols ? dgamma : dbeta;
   if (!out) return;
   out += i < cols ? i : i - cols;
-  s = acc ? (float)*out : 0.f;
+  s = acc & (i < cols ? 1 : 2) ? (float)*out : 0.f;
 #pragma unroll
   for (int k = 0; k < 16; ++k) s += red[k][lane];
   *out = (W)s;
@@ -448,97 +452,126 @@ void launch_layer_norm_backward(const LayerNormGradArgs& given, int type, int wt
 // k = act' gamma u:  d/dt = P k,  dgamma = sum of act' u P t, and through P's own dependence on x
 //   d/dx = -r^2 (q - W b) xh - r (b P k + W P t),   b = mean(t xh), W = mean(k xh), q = mean(k (t - mean t))
 // (from <k, P t> = C r (q - W b) and dr = -r^2 mean(xh dx), d xh = P dx).
-__global__ __launch_bounds__(kRowThreads) void ln_tangent_rows(LayerNormTangentArgs a) {
-  __shared__ float red[2 * kRowThreads / 64];
-  for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
+// f32 rows without gaps, in registers like the others; gamma and beta are there.
+template <int NT, int NV, int V, bool TAIL>
+__device__ __forceinline__ void load_row(const float* p, int cols, int t, float (&v)[NV][V]) {
+  LoosePack<float, V> k[NV];
+  request_row<float, NT, NV, V>(p, cols, t, k);
+  settle_row<float, NT, NV, V, TAIL>(cols, t, k);
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[i][j] = (i * NT + t) * V < cols ? k[i].e[j] : 0.f;
+}
+template <int NT, int NV, int V, bool TAIL>
+__global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_tangent(LayerNormTangentArgs a) {
+  constexpr int NB = NT > 256 ? NT : 256, TEAMS = NB / NT;
+  __shared__ float red[2][NT > 64 ? 2 * NT / 64 : 1];
+  const int t = TEAMS > 1 ? threadIdx.x % NT : threadIdx.x, team = TEAMS > 1 ? threadIdx.x / NT : 0;
+  const float n = 1.f / a.cols;
+  int turn = 0;
+  for (long long r = (long long)blockIdx.x * TEAMS + team; r < a.rows; r += (long long)gridDim.x * TEAMS, turn ^= 1) {
     const size_t o = (size_t)r * a.cols;
+    float x[NV][V], v[NV][V], g[NV][V], b[NV][V];
+    load_row<NT, NV, V, TAIL>(a.x + o, a.cols, t, x);
+    load_row<NT, NV, V, TAIL>(a.tx + o, a.cols, t, v);
+    load_row<NT, NV, V, TAIL>(a.gamma, a.cols, t, g);
+    load_row<NT, NV, V, TAIL>(a.beta, a.cols, t, b);
     const float mean = a.mean[r], rstd = a.rstd[r];
     float s[2] = {0.f, 0.f};
-    for (int c = threadIdx.x; c < a.cols; c += kRowThreads) {
-      const float t = a.tx[o + c];
-      s[0] += t;
-      s[1] += t * rounded_mul(a.x[o + c] - mean, rstd);
-    }
-    team_sum<kRowThreads>(s, red);
-    const float mt = s[0] / a.cols, b = s[1] / a.cols;
-    for (int c = threadIdx.x; c < a.cols; c += kRowThreads) {
-      const float xh = rounded_mul(a.x[o + c] - mean, rstd);
-      const float d = row_act_grad(affine(xh, a.gamma, a.beta, c), a.act);
-      a.ty[o + c] = d * a.gamma[c] * (rstd * (a.tx[o + c] - mt - xh * b));
-    }
-    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {   // (past the end v = 0)
+        x[i][j] = rounded_mul(x[i][j] - mean, rstd);
+        s[0] += v[i][j];
+        s[1] += v[i][j] * x[i][j];
+      }
+    team_sum<NT>(s, red[turn]);
+    const float mt = s[0] * n, bt = s[1] * n;
+    each_pack<NT, NV, V>(a.cols, t, [&](int i, int c) {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        v[i][j] = row_act_grad(rounded_mul(x[i][j], g[i][j]) + b[i][j], a.act) * g[i][j] * (rstd * (v[i][j] - mt - x[i][j] * bt));
+      store_row_pack<float, V, TAIL>(a.ty + o, c, a.cols, v[i]);
+    });
   }
 }
-__global__ __launch_bounds__(kRowThreads) void ln_tangent_bwd_rows(LayerNormTangentArgs a) {
-  __shared__ float red[5 * kRowThreads / 64];
-  for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
+template <int NT, int NV, int V, bool TAIL>
+__global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_tangent_bwd(LayerNormTangentArgs a) {
+  constexpr int NB = NT > 256 ? NT : 256, TEAMS = NB / NT;
+  __shared__ float red[2][NT > 64 ? 5 * NT / 64 : 1];
+  const int t = TEAMS > 1 ? threadIdx.x % NT : threadIdx.x, team = TEAMS > 1 ? threadIdx.x / NT : 0;
+  const float n = 1.f / a.cols;
+  float sx[NV][V], sg[NV][V];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) sx[i][j] = sg[i][j] = 0.f;
+  int turn = 0;
+  for (long long r = (long long)blockIdx.x * TEAMS + team; r < a.rows; r += (long long)gridDim.x * TEAMS, turn ^= 1) {
     const size_t o = (size_t)r * a.cols;
+    float x[NV][V], v[NV][V], k[NV][V], g[NV][V], b[NV][V];
+    load_row<NT, NV, V, TAIL>(a.x + o, a.cols, t, x);
+    load_row<NT, NV, V, TAIL>(a.tx + o, a.cols, t, v);
+    load_row<NT, NV, V, TAIL>(a.dty + o, a.cols, t, k);
+    load_row<NT, NV, V, TAIL>(a.gamma, a.cols, t, g);
+    load_row<NT, NV, V, TAIL>(a.beta, a.cols, t, b);
     const float mean = a.mean[r], rstd = a.rstd[r];
     float s[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int c = threadIdx.x; c < a.cols; c += kRowThreads) {
-      const float xh = rounded_mul(a.x[o + c] - mean, rstd), t = a.tx[o + c];
-      const float k = row_act_grad(affine(xh, a.gamma, a.beta, c), a.act) * a.gamma[c] * a.dty[o + c];
-      s[0] += t;
-      s[1] += t * xh;
-      s[2] += k;
-      s[3] += k * xh;
-      s[4] += k * t;
-    }
-    team_sum<kRowThreads>(s, red);
-    const float n = 1.f / a.cols;
-    const float mt = s[0] * n, b = s[1] * n, mk = s[2] * n, w = s[3] * n, q = s[4] * n - mk * mt;
-    for (int c = threadIdx.x; c < a.cols; c += kRowThreads) {
-      const float xh = rounded_mul(a.x[o + c] - mean, rstd);
-      const float k = row_act_grad(affine(xh, a.gamma, a.beta, c), a.act) * a.gamma[c] * a.dty[o + c];
-      const float pk = rstd * (k - mk - xh * w), pt = rstd * (a.tx[o + c] - mt - xh * b);
-      a.dtx[o + c] = (a.acc_t ? a.dtx[o + c] : 0.f) + pk;
-      a.dx[o + c] = (a.acc_x ? a.dx[o + c] : 0.f) - rstd * (rstd * (q - w * b) * xh + b * pk + w * pt);
-    }
-    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {   // (past the end v = k = 0)
+        x[i][j] = rounded_mul(x[i][j] - mean, rstd);
+        k[i][j] *= row_act_grad(rounded_mul(x[i][j], g[i][j]) + b[i][j], a.act);
+        b[i][j] = k[i][j];            // act' dty: dgamma's
+        k[i][j] *= g[i][j];
+        s[0] += v[i][j];
+        s[1] += v[i][j] * x[i][j];
+        s[2] += k[i][j];
+        s[3] += k[i][j] * x[i][j];
+        s[4] += k[i][j] * v[i][j];
+      }
+    team_sum<NT>(s, red[turn]);
+    const float mt = s[0] * n, bt = s[1] * n, mk = s[2] * n, w = s[3] * n, q = s[4] * n - mk * mt;
+    each_pack<NT, NV, V>(a.cols, t, [&](int i, int c) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float pk = rstd * (k[i][j] - mk - x[i][j] * w), pt = rstd * (v[i][j] - mt - x[i][j] * bt);
+        sx[i][j] += b[i][j] * pt;
+        k[i][j] = pk;
+        v[i][j] = -rstd * (rstd * (q - w * bt) * x[i][j] + bt * pk + w * pt);
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (c + j < a.cols) {
+          if (a.acc_t) k[i][j] += a.dtx[o + c + j];
+          if (a.acc_x) v[i][j] += a.dx[o + c + j];
+        }
+      store_row_pack<float, V, TAIL>(a.dtx + o, c, a.cols, k[i]);
+      store_row_pack<float, V, TAIL>(a.dx + o, c, a.cols, v[i]);
+    });
   }
-}
-// columns of dgamma = sum over rows of act' dty P t; the row means of t and t xh are formed again from x and tx
-__global__ __launch_bounds__(256) void ln_tangent_bwd_columns(LayerNormTangentArgs a) {
-  __shared__ float red[2 * 4];
-  __shared__ float means[2];
-  const int tid = threadIdx.x;
-  // one block walks rows blockIdx.x, + gridDim.x, ...; its sums stay in memory of its own
-  float* out = a.partial + (size_t)blockIdx.x * 2 * a.cols;
-  bool first = true;
-  for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
-    const size_t o = (size_t)r * a.cols;
-    const float mean = a.mean[r], rstd = a.rstd[r];
-    float s[2] = {0.f, 0.f};
-    for (int c = tid; c < a.cols; c += 256) {
-      const float t = a.tx[o + c];
-      s[0] += t;
-      s[1] += t * rounded_mul(a.x[o + c] - mean, rstd);
-    }
-    team_sum<256>(s, red);
-    if (tid < 2) means[tid] = s[tid] / a.cols;
-    __syncthreads();
-    const float mt = means[0], b = means[1];
-    for (int c = tid; c < a.cols; c += 256) {
-      const float xh = rounded_mul(a.x[o + c] - mean, rstd);
-      const float v = row_act_grad(affine(xh, a.gamma, a.beta, c), a.act) * a.dty[o + c] * (rstd * (a.tx[o + c] - mt - xh * b));
-      out[c] = (first ? 0.f : out[c]) + v;
-    }
-    first = false;
-    __syncthreads();
-  }
-  for (int c = tid; c < a.cols; c += 256) out[a.cols + c] = 0.f;
+  if (a.dgamma) leave_partial<NT, NV, V, TEAMS>(a.partial, a.cols, t, team, sx, sg);
 }
 
 void launch_layer_norm_tangent(const LayerNormTangentArgs& a, hipStream_t s) {
-  if (a.rows && a.cols) row_launch(ln_tangent_rows, row_grid(a.rows), dim3(kRowThreads), s, a);
+  if (!a.rows || !a.cols) return;
+  const bool held = row_team<float, 16>(a.cols, [&](auto nt, auto nv, auto v, auto tail) {
+    row_launch(ln_tangent<nt, nv, v, tail>, team_grid(a.rows, nt, 8192), team_block(nt), s, a);
+  });
+  EG_CHECK(held, "layer norm tangent: %d channels", a.cols);
 }
 void launch_layer_norm_tangent_backward(const LayerNormTangentArgs& a, hipStream_t s) {
   if (!a.rows || !a.cols) return;
-  row_launch(ln_tangent_bwd_rows, row_grid(a.rows), dim3(kRowThreads), s, a);
-  if (!a.dgamma) return;
-  const int groups = part_groups(a.rows);
-  row_launch(ln_tangent_bwd_columns, dim3(groups), dim3(256), s, a);
-  row_launch(ln_bwd_finish<float>, dim3((2 * a.cols + 31) / 32), dim3(1024), s, a.partial, groups, a.cols, a.dgamma, nullptr, a.acc_w);
+  const bool held = row_team<float, 16>(a.cols, [&](auto nt, auto nv, auto v, auto tail) {
+    const dim3 grid = team_grid(a.rows, nt, nt > 64 ? kGradBlocks / 2 : kGradBlocks);
+    row_launch(ln_tangent_bwd<nt, nv, v, tail>, grid, team_block(nt), s, a);
+    if (a.dgamma)
+      row_launch(ln_bwd_finish<float>, dim3((2 * a.cols + 31) / 32), dim3(1024), s, a.partial, (int)grid.x, a.cols, a.dgamma, (float*)nullptr, a.acc_w);
+  });
+  EG_CHECK(held, "layer norm tangent: %d channels", a.cols);
 }
 
 // ---- quantisation of rows of any length -----------------------------------------------------------------------------------------

@@ -22,6 +22,12 @@ static void bn_vars(std::vector<VarInfo>& v, const std::string& scope, int C, in
   v.push_back({scope + "/batch_norm/BatchNorm/moving_variance", {C}, false, false, 0, 1.f, group});
 }
 
+// scale and shift of a layer norm (E_norm / G_norm / D_norm = 'layernorm')
+static void ln_vars(std::vector<VarInfo>& v, const std::string& scope, int C, int group) {
+  v.push_back({scope + "/layer_norm/LayerNorm/beta", {C}, true, false, 0, 0.f, group});
+  v.push_back({scope + "/layer_norm/LayerNorm/gamma", {C}, true, false, 0, 1.f, group});
+}
+
 static void gen_vars(std::vector<VarInfo>& v, const Config& cfg, int group) {
   const std::string p = kGroupPrefix[group];
   int h = cfg.H, w = cfg.W / 2;
@@ -42,6 +48,7 @@ static void gen_vars(std::vector<VarInfo>& v, const Config& cfg, int group) {
     v.push_back({b + "w", {5, 5, ch[i], ch[i - 1]}, true, false, 1, 0.02f, group});
     v.push_back({b + "b", {ch[i]}, true, false, 0, 0.f, group});
     if (cfg.g_bn && i < 4) bn_vars(v, p + "/g_dconv_" + std::to_string(i), ch[i], group);   // deconv_block (conv.py:124-130), G_norm = 'batch'
+    if (cfg.g_ln && i < 4) ln_vars(v, p + "/g_dconv_" + std::to_string(i), ch[i], group);
   }
 }
 
@@ -55,6 +62,7 @@ static void disc_vars(std::vector<VarInfo>& v, const Config& cfg, int group, int
   for (int i = 0; i < 4; ++i) {
     v.push_back({p + "/" + kDiscNames[i] + "/conv2d/w", {4, 4, ch[i], ch[i + 1]}, true, false, 2, 0.02f, group});
     if (cfg.d_bn && i > 0) bn_vars(v, p + "/" + kDiscNames[i], ch[i + 1], group);   // conv_block (conv.py:61-67), D_norm = 'batch'
+    if (cfg.d_ln && i > 0) ln_vars(v, p + "/" + kDiscNames[i], ch[i + 1], group);
     h = ceil_half(h);
     w = ceil_half(w);
   }
@@ -77,9 +85,11 @@ static void enc_vars(std::vector<VarInfo>& v, const Config& cfg) {
     v.push_back({b + "/res1/conv2d/w", {3, 3, cin, n}, true, false, 2, 0.02f, G_E});
     v.push_back({b + "/res1/conv2d/b", {n}, true, false, 0, 0.f, G_E});
     if (cfg.e_bn) bn_vars(v, b + "/res1", n, G_E);   // residual (conv.py:70-85), E_norm = 'batch'
+    if (cfg.e_ln) ln_vars(v, b + "/res1", n, G_E);
     v.push_back({b + "/res2/conv2d/w", {3, 3, n, n}, true, false, 2, 0.02f, G_E});
     v.push_back({b + "/res2/conv2d/b", {n}, true, false, 0, 0.f, G_E});
     if (cfg.e_bn) bn_vars(v, b + "/res2", n, G_E);
+    if (cfg.e_ln) ln_vars(v, b + "/res2", n, G_E);
     v.push_back({b + "/shortcut/conv2d/w", {1, 1, cin, n}, true, false, 2, 0.02f, G_E});
     v.push_back({b + "/shortcut/conv2d/b", {n}, true, false, 0, 0.f, G_E});
     cin = n;
@@ -400,12 +410,17 @@ static T block_bn(Ctx& c, T x, const std::string& scope, int a, int times, T* st
   return bn_act(c, x, P(c, b + "gamma"), P(c, b + "beta"), P(c, b + "moving_mean"), P(c, b + "moving_variance"), a, times, stats_out);
 }
 
+static T block_ln(Ctx& c, T x, const std::string& scope, int a, T* stats_out = nullptr) {
+  const std::string b = scope + "/layer_norm/LayerNorm/";
+  return ln_act(c, x, P(c, b + "gamma"), P(c, b + "beta"), a, stats_out);
+}
+
 T generator_forward(Ctx& c, int group, T zin, int bn_times, T* bn_stats_out, float* out_into) {
   const Config& cfg = c.cfg;
   const std::string p = kGroupPrefix[group];
   const int gf = cfg.gf, h16 = cfg.H / 16, w16 = cfg.W / 2 / 16;
   const int feat = gf * 8 * h16 * w16;
-  T z_ = linear(c, zin, wref_param(c, P(c, p + "/g_lin_0/Matrix"), 1, zin->c, feat), P(c, p + "/g_lin_0/bias"));
+  T z_ = c.int8_now ? dense8(c, zin, P(c, p + "/g_lin_0/Matrix"), P(c, p + "/g_lin_0/bias")) : linear(c, zin, wref_param(c, P(c, p + "/g_lin_0/Matrix"), 1, zin->c, feat), P(c, p + "/g_lin_0/bias"));
   T x = reshape(c, z_, zin->n, h16, w16, gf * 8);
   // (a one-launch form of linear + BatchNorm + ReLU for forward-only graphs was built and measured in round 6: 43 us against
   //  18 + 12 for the two launches it replaced -- 64 blocks of a latency-bound gather of 32-byte filter pieces -- and its batch
@@ -417,7 +432,7 @@ T generator_forward(Ctx& c, int group, T zin, int bn_times, T* bn_stats_out, flo
   const int ch[5] = {gf * 8, gf * 4, gf * 2, gf, cfg.c_dim};
   for (int i = 1; i <= 4; ++i) {
     const std::string b = p + "/g_dconv_" + std::to_string(i) + "/deconv2d/";
-    c.feeds_in = i < 4 && !cfg.g_bn && !cfg.g_nonorm;   // deconv_block: the InstanceNorm is the transposed convolution's only reader
+    c.feeds_in = i < 4 && cfg.g_in_norm();   // deconv_block: the InstanceNorm is the transposed convolution's only reader
     x = deconv2d(c, x, wref_param(c, P(c, b + "w"), 25, ch[i], ch[i - 1]), P(c, b + "b"), ch[i], i == 4 ? ACT_TANH : 0,
                  i == 4 ? out_into : nullptr);
     // (bf16 mode, forward-only graph: the next transposed convolution stages the bf16 plane -- the fp32 copy is not written;
@@ -426,6 +441,8 @@ T generator_forward(Ctx& c, int group, T zin, int bn_times, T* bn_stats_out, flo
       T bst = nullptr;
       x = block_bn(c, x, p + "/g_dconv_" + std::to_string(i), ACT_RELU, bn_times, &bst);
       c.gen_blk_stats[i - 1] = bst;
+    } else if (i < 4 && cfg.g_ln) {
+      x = block_ln(c, x, p + "/g_dconv_" + std::to_string(i), ACT_RELU);
     } else if (i < 4 && cfg.g_nonorm) {   // G_norm = None (normalization.py:26-27): deconv -> ReLU
       x = act(c, x, ACT_RELU);
     } else if (i < 4)
@@ -452,7 +469,7 @@ T disc_forward(Ctx& c, int group, T x, DiscSave* save, const DiscSave* tangent_o
     WRef* w = wref_param(c, P(c, p + "/" + kDiscNames[i] + "/conv2d/w"), 16, ch[i], ch[i + 1]);
     // (first block: conv + LeakyReLU, fused where the small-C kernel runs the conv; `pre` is then the activated output,
     //  which is all the tangent pass and the backward need of it)
-    c.feeds_in = i > 0 && !tangent_of && !cfg.d_bn && !cfg.d_nonorm;   // conv_block: the InstanceNorm is the convolution's only forward reader
+    c.feeds_in = i > 0 && !tangent_of && cfg.d_in();   // conv_block: the InstanceNorm is the convolution's only forward reader
     c.conv_plane_only_next = cfg.bf16 && i == 0 && !tangent_of && !save;   // (no tangent pass will read this output's values)
     T pre = conv2d(c, x, w, nullptr, 4, 2, PAD_SAME, nullptr, (i == 0 && !tangent_of) ? ACT_LRELU : 0);
     T out, st = nullptr;
@@ -461,6 +478,16 @@ T disc_forward(Ctx& c, int group, T x, DiscSave* save, const DiscSave* tangent_o
       out = !tangent_of ? block_bn(c, pre, scope, ACT_LRELU, c.bn_times_block, &st)
                         : bn_act_tangent(c, pre, tangent_of->pre[i], tangent_of->out[i], tangent_of->stats[i],
                                          P(c, scope + "/batch_norm/BatchNorm/gamma"), ACT_LRELU);
+      if (save && !tangent_of) {
+        save->pre[i] = pre;
+        save->out[i] = out;
+        save->stats[i] = st;
+      }
+    } else if (cfg.d_ln && i > 0) {   // D_norm = 'layernorm'
+      const std::string scope = p + "/" + kDiscNames[i];
+      out = !tangent_of ? block_ln(c, pre, scope, ACT_LRELU, &st)
+                        : ln_act_tangent(c, pre, tangent_of->pre[i], tangent_of->stats[i], P(c, scope + "/layer_norm/LayerNorm/gamma"),
+                                         P(c, scope + "/layer_norm/LayerNorm/beta"), ACT_LRELU);
       if (save && !tangent_of) {
         save->pre[i] = pre;
         save->out[i] = out;
@@ -498,24 +525,27 @@ T encoder_forward(Ctx& c, T x, const float* eps_dev, T* mu_out, T* ls_out, T* z1
     const std::string b = "E/e_resnet_" + std::to_string(n) + "_" + std::to_string(i++);
     const int main_lane = c.cur_lane;
     if (c.infer_side >= 0) EG_HIP(hipEventRecord(c.ev_infer[main_lane], c.stream));   // the block's input is complete here
-    c.feeds_in = !cfg.e_bn && !cfg.e_nonorm;   // residual: both 3x3 convolutions are read by their InstanceNorm alone
+    c.feeds_in = cfg.e_in();   // residual: both 3x3 convolutions are read by their InstanceNorm alone
     T o1 = conv2d(c, E, wref_param(c, P(c, b + "/res1/conv2d/w"), 9, cin, n), P(c, b + "/res1/conv2d/b"), 3, 1,
                   PAD_REFLECT);
     // E_norm = 'batch' (encoder.py:67 through conv.py:70-85): BatchNorm in both halves of the block
     // E_norm = None (normalization.py:26-27): conv -> ReLU -> conv
     o1 = cfg.e_bn ? block_bn(c, o1, b + "/res1", ACT_RELU, c.bn_times_block)
+         : cfg.e_ln ? block_ln(c, o1, b + "/res1", ACT_RELU)
          : cfg.e_nonorm ? act(c, o1, ACT_RELU)
                   : in_act(c, o1, ACT_RELU, nullptr, /*plane_only=*/cfg.bf16 && !o1->needs_grad);   // (forward-only graph: res2 stages the plane)
-    c.feeds_in = !cfg.e_bn && !cfg.e_nonorm;
+    c.feeds_in = cfg.e_in();
     T o2 = conv2d(c, o1, wref_param(c, P(c, b + "/res2/conv2d/w"), 9, n, n), P(c, b + "/res2/conv2d/b"), 3, 1,
                   PAD_REFLECT);
-    if (!cfg.e_nonorm) o2 = cfg.e_bn ? block_bn(c, o2, b + "/res2", ACT_NONE, c.bn_times_block) : in_act(c, o2, ACT_NONE);
+    if (!cfg.e_nonorm)
+      o2 = cfg.e_bn ? block_bn(c, o2, b + "/res2", ACT_NONE, c.bn_times_block) : cfg.e_ln ? block_ln(c, o2, b + "/res2", ACT_NONE) : in_act(c, o2, ACT_NONE);
     if (c.infer_side >= 0) {
       use_lane(c, c.infer_side);
       EG_HIP(hipStreamWaitEvent(c.stream, c.ev_infer[main_lane], 0));
     }
-    T sc = conv2d(c, E, wref_param(c, P(c, b + "/shortcut/conv2d/w"), 1, cin, n), P(c, b + "/shortcut/conv2d/b"),
-                  1, 1, PAD_REFLECT);
+    T sc = c.int8_now ? dense8(c, E, P(c, b + "/shortcut/conv2d/w"), P(c, b + "/shortcut/conv2d/b"))
+                      : conv2d(c, E, wref_param(c, P(c, b + "/shortcut/conv2d/w"), 1, cin, n), P(c, b + "/shortcut/conv2d/b"),
+                               1, 1, PAD_REFLECT);
     if (c.infer_side >= 0) {
       EG_HIP(hipEventRecord(c.lanes[c.infer_side].done, c.stream));
       use_lane(c, main_lane);
@@ -1029,7 +1059,7 @@ static void disc_substep_stacked(Ctx& c, int group, T real, T fake, const float*
 static void d_substep(Ctx& c, int group, T real, T fake, const float* alpha_dev, int slot_d, int slot_gp, bool apply) {
   static const bool tape_form = dbg_env("EG_D_TAPE") != nullptr;
   // (D_norm = 'batch': the tape form -- the stacked sweep's row classes are InstanceNorm's, and BatchNorm couples the rows of a call)
-  if (tape_form || c.cfg.d_bn || c.cfg.d_nonorm) disc_substep(c, group, real, fake, alpha_dev, slot_d, slot_gp, apply);
+  if (tape_form || !c.cfg.d_in()) disc_substep(c, group, real, fake, alpha_dev, slot_d, slot_gp, apply);
   else disc_substep_stacked(c, group, real, fake, alpha_dev, slot_d, slot_gp, apply);
 }
 
@@ -1136,6 +1166,14 @@ void run_substep(Ctx& c, int k, bool apply, const SubOpts* opts) {
       seed_grad(c, logits);
       launch_acgan_loss(logits->d, c.d_z + cfg.z_dim, cfg.z_dim + 1, c.d_losses + L_CLS_D, logits->g, B,
                         cfg.num_classes, 0, c.scratch, c.stream);
+      if (c.teacher_top) {   // + weight x mean over the batch of T^2 KL(teacher || classifier) on the teacher's top logits (eg_set_teacher)
+        const int n = B * cfg.num_classes;
+        float* more = c.arena.allocf(n);
+        launch_distill({logits->d, cfg.num_classes, c.teacher_index, c.teacher_top, 0, c.teacher_logits, c.teacher_top, nullptr, B, cfg.num_classes, c.teacher_top,
+                        c.teacher_temperature, c.teacher_weight / B, c.teacher_loss + 1, more, cfg.num_classes, nullptr},
+                       ROW_F32, c.stream);
+        launch_distill_join(more, logits->g, n, c.teacher_loss + 1, B, c.teacher_loss, c.stream);
+      }
       c.tape.backward();
       if (apply) apply_group(c, G_D2);
     } break;
@@ -1496,6 +1534,11 @@ void infer(Ctx& c, const float* d_images, const int* d_classes, int NB, const fl
   ensure_lane(c, main_lane);
   use_lane(c, main_lane);
   reset_step(c);
+  struct Int8 {   // (reset on every way out)
+    Ctx& c;
+    explicit Int8(Ctx& c_) : c(c_) { c.int8_now = c.inf_int8; }
+    ~Int8() { c.int8_now = false; }
+  } int8(c);
   for (int g = 0; g < G_COUNT; ++g) set_want_grad(c, g, false);
   T images = wrap_tensor(c, const_cast<float*>(d_images), NB, cfg.H, cfg.W, cfg.c_dim);
   T left = slice_w(c, images, 0, cfg.W / 2);

@@ -1568,6 +1568,92 @@ T bn_act_tangent(Ctx& c, T tx, T x_prim, T out_prim, T stats_prim, Param* gamma,
   return tout;
 }
 
+// E_norm / G_norm / D_norm = 'layernorm': fp32 in every mode, like the block BatchNorm (a plane-fed consumer converts for itself)
+T ln_act(Ctx& c, T x, Param* gamma, Param* beta, int a, T* stats_out) {
+  const int C = x->c;
+  const long long R = (long long)x->pixels();
+  need_f32(c, x);
+  T out = new_tensor(c, x->n, x->h, x->w, C, true);
+  T st = new_tensor(c, 1, 1, 2, (int)R, false);
+  launch_layer_norm({x->d, C, gamma->w, beta->w, R, C, 1e-5f, a, out->d, C, st->d, st->d + R}, ROW_F32, ROW_F32, c.stream);
+  if (stats_out) *stats_out = st;
+  const bool need = x->needs_grad || gamma->want_grad;
+  out->needs_grad = need;
+  if (need) {
+    Ctx* cp = &c;
+    c.tape.push([=]() {
+      Ctx& c = *cp;
+      if (!out->g_set) return;
+      float* dx = nullptr;
+      int acc = 0;
+      if (x->needs_grad) dx = grad_acc(c, x, &acc);
+      const bool pg = c.param_grad_enabled && gamma->want_grad;
+      if (!dx && !pg) return;
+      LayerNormGradArgs g{out->g, x->d, C, C, st->d, st->d + R, gamma->w, beta->w, R, C, a, dx, C, acc, pg ? gamma->g : nullptr, pg ? beta->g : nullptr,
+                          (gamma->g_set ? 1 : 0) | (beta->g_set ? 2 : 0), pg ? c.arena.allocf(layer_norm_partial_floats(R, C)) : nullptr};
+      launch_layer_norm_backward(g, ROW_F32, ROW_F32, c.stream);
+      if (pg) gamma->g_set = beta->g_set = true;
+    });
+  }
+  return out;
+}
+
+// forward-mode tangent of ln_act at the primal x; its reverse gives the gradients of the tangent, of the primal input and of gamma (the gradient
+// penalty through a layer-norm discriminator)
+T ln_act_tangent(Ctx& c, T tx, T x_prim, T stats_prim, Param* gamma, Param* beta, int a) {
+  const int C = tx->c;
+  const long long R = (long long)tx->pixels();
+  T tout = new_tensor(c, tx->n, tx->h, tx->w, C, true);
+  LayerNormTangentArgs f{};
+  f.x = x_prim->d;
+  f.mean = stats_prim->d;
+  f.rstd = stats_prim->d + R;
+  f.gamma = gamma->w;
+  f.beta = beta->w;
+  f.tx = tx->d;
+  f.rows = R;
+  f.cols = C;
+  f.act = a;
+  f.ty = tout->d;
+  launch_layer_norm_tangent(f, c.stream);
+  Ctx* cp = &c;
+  c.tape.push([=]() {
+    Ctx& c = *cp;
+    if (!tout->g_set) return;
+    LayerNormTangentArgs b = f;
+    b.dty = tout->g;
+    b.dtx = grad_acc(c, tx, &b.acc_t);
+    b.dx = grad_acc(c, x_prim, &b.acc_x);
+    const bool pg = c.param_grad_enabled && gamma->want_grad;
+    b.dgamma = pg ? gamma->g : nullptr;
+    b.acc_w = gamma->g_set ? 1 : 0;
+    b.partial = pg ? c.arena.allocf(layer_norm_partial_floats(R, C)) : nullptr;
+    launch_layer_norm_tangent_backward(b, c.stream);
+    if (pg) gamma->g_set = true;
+  });
+  return tout;
+}
+
+// The filter's transpose in 8 bits is a persistent derived copy of the variable (the first run after a change builds it and is waited for: capi.cpp eg_infer_run).
+T dense8(Ctx& c, T x, Param* w, Param* bias) {
+  const int in = x->c, out = (int)(w->numel / in);
+  EG_CHECK((size_t)in * out == w->numel, "dense8 %s: %d inputs", w->name.c_str(), in);
+  need_f32(c, x);
+  const int pitch = (in + 15) & ~15;
+  if (!w->q8_valid) {
+    if (!w->q8) EG_HIP(hipMalloc(&w->q8, (size_t)out * pitch));
+    if (!w->q8_scale) EG_HIP(hipMalloc(&w->q8_scale, (size_t)out * 4));
+    launch_quantize_rows({wref_transposed(c, wref_param(c, w, 1, in, out)), in, nullptr, nullptr, false, 1.f, out, in, w->q8, pitch, w->q8_scale}, ROW_F32, c.stream);
+    w->q8_valid = true;
+  }
+  T y = new_tensor(c, x->n, x->h, x->w, out, false);
+  const long long rows = (long long)x->pixels();
+  launch_int8_linear({x->d, in, nullptr, nullptr, false, 1.f, rows, in, nullptr, 0, nullptr},
+                     {nullptr, 0, nullptr, w->q8, pitch, w->q8_scale, bias ? bias->w : nullptr, rows, out, in, y->d, out}, ROW_F32, ROW_F32,
+                     c.arena.alloc(int8_linear_bytes(rows, in)), c.stream);
+  return y;
+}
+
 T add(Ctx& c, T a, T b, bool relu) {
   T out = new_tensor(c, a->n, a->h, a->w, a->c, a->needs_grad || b->needs_grad);
   launch_add(a->d, b->d, out->d, relu ? 1 : 0, a->numel(), c.stream);
@@ -2099,6 +2185,8 @@ Ctx::~Ctx() {
     {
       if (p->wT) (void)hipFree(p->wT);
       if (p->wM) (void)hipFree(p->wM);
+      (void)hipFree(p->q8);
+      (void)hipFree(p->q8_scale);
       for (int o = 0; o < 2; ++o) p->wL[o].release();
     }
   for (int i = 0; i < 2; ++i) {
@@ -2107,6 +2195,9 @@ Ctx::~Ctx() {
     if (feed_copied[i]) (void)hipEventDestroy(feed_copied[i]);
     if (loss_ready[i]) (void)hipEventDestroy(loss_ready[i]);
   }
+  (void)hipFree(teacher_index);
+  (void)hipFree(teacher_logits);
+  (void)hipFree(teacher_loss);
   (void)hipFree(inf_in);
   for (int i = 0; i < kInferSlots; ++i) {
     (void)hipFree(inf_edge[i]);

@@ -31,7 +31,7 @@ struct LayerNormGradArgs {
   long long lddx;
   int acc_x;                  // dx += (f32 only)
   void *dgamma, *dbeta;       // null: not wanted
-  int acc_w;                  // dgamma +=, dbeta += (f32 parameters only)
+  int acc_w;                  // bit 0: dgamma +=, bit 1: dbeta +=
   float* partial;             // layer_norm_partial_floats()
 };
 // J_v of the layer norm at x and its reverse (f32; the gradient penalty of a critic)
@@ -105,5 +105,7 @@ size_t int8_linear_bytes(long long m, int k);
 void launch_int8_linear(const QuantizeArgs& q, const Int8Args& a, int type, int out_type, void* workspace, hipStream_t s);
 size_t distill_partial_floats(long long rows, int cols, int top);
 void launch_distill(const DistillArgs& a, int type, hipStream_t s);
+// grad[i] += more[i] (n values), *total = the sum of loss[0 .. rows)
+void launch_distill_join(const float* more, float* grad, int n, const float* loss, int rows, float* total, hipStream_t s);
 
 }  // namespace eg

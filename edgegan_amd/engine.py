@@ -159,6 +159,23 @@ class EdgeGAN:
         d.update(out)
         return d
 
+    def set_teacher(self, index: Optional[np.ndarray], logits: Optional[np.ndarray] = None, temperature: float = 1.0, weight: float = 1.0):
+        """A teacher's top logits for the resident batch: index and logits [B, top] (an index outside [0, num_classes) is padding).  Sub-step 4
+        then also learns from them -- weight x the batch mean of T^2 KL(teacher || classifier) -- until the next call; None: no teacher."""
+        if index is None:
+            self._check(self._lib.eg_set_teacher(self._ctx, None, None, 0, 1.0, 0.0))
+            return
+        index, logits = np.ascontiguousarray(index, dtype=np.int32), np.ascontiguousarray(logits, dtype=np.float32)
+        if index.ndim != 2 or index.shape != logits.shape or index.shape[0] != self.config.batch_size:
+            raise EdgeGANLibError(f'set_teacher: index and logits [{self.config.batch_size}, top], not {index.shape} and {logits.shape}')
+        self._check(self._lib.eg_set_teacher(self._ctx, iptr(index), fptr(logits), index.shape[1], temperature, weight))
+
+    def teacher_loss(self) -> float:
+        """The weighted distillation loss of the last sub-step 4."""
+        out = np.zeros(1, dtype=np.float32)
+        self._check(self._lib.eg_teacher_loss(self._ctx, fptr(out)))
+        return float(out[0])
+
     def losses(self) -> Dict[str, float]:
         """Losses captured INSIDE the sub-steps of the last iteration (pre-update / mixed-stage weights; free).  The
         reference prints post-update re-evaluations instead: evaluate()."""
@@ -182,6 +199,10 @@ class EdgeGAN:
         self._check(self._lib.eg_sync(self._ctx))
 
     # -- inference --------------------------------------------------------------------------------
+    def infer_precision(self, bits: int):
+        """8: the inference graph's dense layers (generators' first layer, encoder's 1x1 shortcuts) in 8-bit integers; 0: as compute_dtype."""
+        self._check(self._lib.eg_infer_precision(self._ctx, int(bits)))
+
     def infer(self, images: np.ndarray, classes: Optional[np.ndarray] = None, eps2=None):
         """E(left half) -> z (+ one-hot) -> (edge_output, image_output)  (edgegan.py:492-517,606-609)."""
         cfg = self.config

@@ -57,7 +57,10 @@ typedef struct eg_config {
                           implementation: held to the fp32 tolerances, ~1.35x faster -- DESIGN.md 3.4); 1 = the
                           contractions take bf16-ROUNDED operands on the bf16 MFMA with fp32 accumulation; storage,
                           norms, losses and RMSProp stay fp32 in every mode (BASELINE configs 2,4,5) */
-  int e_norm, g_norm, d_norm; /* train.py:54-59 E_norm / G_norm / D_norm: 0 = 'instance' (the default), 1 = 'batch', 2 = None
+  int e_norm, g_norm, d_norm; /* train.py:54-59 E_norm / G_norm / D_norm: 0 = 'instance' (the default), 1 = 'batch', 3 = 'layernorm' (no
+                                 reference value: over the channels of each position, epsilon 1e-5 inside the root, learned scale
+                                 and shift in <block>/layer_norm/LayerNorm/{beta, gamma}; every sample on its own, as the critics'
+                                 gradient penalty assumes), 2 = None
                                  (normalization.py:26-27: the block keeps its activation only; reachable from Python, not from
                                  the string flags, whose 'None' fails normalization.py:12's assertion) -- the
                                  normalisation of the encoder's residual blocks (models/encoder.py:67), the generators'
@@ -113,6 +116,13 @@ int eg_read_losses(eg_ctx* ctx, float* out12);
 int eg_train_batch(eg_ctx* ctx, const float* images, const float* z, const float* alpha, const float* eps);
 int eg_losses_wait(eg_ctx* ctx, int back, float* out12);
 
+/* A teacher for the classifier (no reference counterpart): its top logits for the resident batch, index and logits [B][top] (top <= 1024; an index
+ * outside [0, num_classes) is padding).  Sub-step 4 (d_optim2) then also minimises weight x the batch mean of
+ * T^2 KL(softmax(teacher / T) || softmax(classifier / T)) over those logits -- eg_distill_loss below -- until another teacher is set (for
+ * the next batch) or top = 0.  loss_d_ac and eg_eval_losses stay the reference's; eg_teacher_loss returns that weighted mean of the last sub-step 4. */
+int eg_set_teacher(eg_ctx* ctx, const int* index, const float* logits, int top, float temperature, float weight);
+int eg_teacher_loss(eg_ctx* ctx, float* out);
+
 /* Post-update evaluation with the reference's semantics -- replaces the observe-only runs the reference issues AFTER
  * update_model: sess.run(d_sum), sess.run(g_sum) (models/edgegan.py:427-433) and the five evaluate() calls
  * (models/edgegan.py:464-480).  Forward-only on the resident batch with the CURRENT weights; alpha [3][B] and eps are
@@ -146,6 +156,11 @@ int eg_infer(eg_ctx* ctx, const float* images, const int* classes, int nb, const
 int eg_infer_upload(eg_ctx* ctx, const float* images, const int* classes, int nb, const float* eps2);
 int eg_infer_run(eg_ctx* ctx);
 int eg_infer_download(eg_ctx* ctx, float* edge_out, float* image_out);
+
+/* Operands of the inference graph's dense layers (the generators' first linear layer, the encoder's 1x1 shortcut convolutions): bits = 0 as
+ * compute_dtype says (the default), 8 = 8-bit integers with a scale for each position and output channel (eg_int8_linear below); the
+ * filters' 8-bit copies are rebuilt when a variable changes.  No reference counterpart; training is not affected. */
+int eg_infer_precision(eg_ctx* ctx, int bits);
 
 int eg_sync(eg_ctx* ctx);
 

@@ -332,6 +332,12 @@ def batch_norm_train(x: Tensor, gamma: Tensor, beta: Tensor, eps: float = 1e-5):
     return y, mean, var
 
 
+def layer_norm_channels(x: Tensor, gamma: Tensor, beta: Tensor, eps: float = 1e-5) -> Tensor:
+    """E_norm / G_norm / D_norm = 'layernorm' (no reference value): over the channels of each position of each sample."""
+    d = x - x.mean(dim=-1, keepdim=True)
+    return d / torch.sqrt((d * d).mean(dim=-1, keepdim=True) + eps) * gamma + beta
+
+
 def activation(x: Tensor, name: Optional[str]) -> Tensor:
     """edgegan/nn/modules/activation.py:4-15."""
     if name == 'relu':
@@ -362,6 +368,15 @@ def _bn_specs(scope: str, c: int):
             VarSpec(f'{scope}/batch_norm/BatchNorm/moving_variance', (c,), False, 'const:1')]
 
 
+def _ln_specs(scope: str, c: int):
+    return [VarSpec(f'{scope}/layer_norm/LayerNorm/beta', (c,), True, 'const:0'),
+            VarSpec(f'{scope}/layer_norm/LayerNorm/gamma', (c,), True, 'const:1')]
+
+
+def _norm_specs(scope: str, c: int, kind: Optional[str]):
+    return _bn_specs(scope, c) if kind == 'batch' else _ln_specs(scope, c) if kind == 'layernorm' else []
+
+
 def block_norm(p, scope: str, x: Tensor, kind: Optional[str]) -> Tensor:
     """`_norm(out, is_train, norm)` inside conv_block / deconv_block / residual (conv.py:65,75,80,128): 'instance', or 'batch'
     = contrib batch_norm over ALL rows of this call with the block's own beta / gamma (normalization.py:19-25; the moving
@@ -369,6 +384,8 @@ def block_norm(p, scope: str, x: Tensor, kind: Optional[str]) -> Tensor:
     if kind == 'batch':
         y, _, _ = batch_norm_train(x, p[f'{scope}/batch_norm/BatchNorm/gamma'], p[f'{scope}/batch_norm/BatchNorm/beta'])
         return y
+    if kind == 'layernorm':
+        return layer_norm_channels(x, p[f'{scope}/layer_norm/LayerNorm/gamma'], p[f'{scope}/layer_norm/LayerNorm/beta'])
     return norm(x, kind)
 
 
@@ -527,8 +544,8 @@ def generator_specs(prefix: str, cfg: Config) -> List[VarSpec]:
     for i in range(1, 5):
         v.append(VarSpec(f'{prefix}/g_dconv_{i}/deconv2d/w', (5, 5, chans[i], chans[i - 1]), True, 'normal:0.02'))
         v.append(VarSpec(f'{prefix}/g_dconv_{i}/deconv2d/b', (chans[i],), True, 'const:0'))
-        if cfg.G_norm == 'batch' and i < 4:
-            v += _bn_specs(f'{prefix}/g_dconv_{i}', chans[i])
+        if i < 4:
+            v += _norm_specs(f'{prefix}/g_dconv_{i}', chans[i], cfg.G_norm)
     return v
 
 
@@ -541,8 +558,8 @@ def discriminator_specs(prefix: str, cfg: Config, in_h: int, in_w: int) -> List[
     h, w = in_h, in_w
     for i, n in enumerate(names):
         v.append(VarSpec(f'{prefix}/{n}/conv2d/w', (4, 4, chans[i], chans[i + 1]), True, 'trunc:0.02'))
-        if cfg.D_norm == 'batch' and i > 0:
-            v += _bn_specs(f'{prefix}/{n}', chans[i + 1])
+        if i > 0:
+            v += _norm_specs(f'{prefix}/{n}', chans[i + 1], cfg.D_norm)
         h, w = _ceil_half(h), _ceil_half(w)
     v.append(VarSpec(f'{prefix}/d_linear_5/Matrix', (h * w * chans[-1], 1), True, 'normal:0.02'))
     v.append(VarSpec(f'{prefix}/d_linear_5/bias', (1,), True, 'const:0'))
@@ -563,11 +580,11 @@ def encoder_specs(cfg: Config) -> List[VarSpec]:
     cin = 64
     for i, n in enumerate(encoder_filters(cfg)):
         base = f'E/e_resnet_{n}_{i + 1}'
-        bn = cfg.E_norm == 'batch'
+        bn = cfg.E_norm
         v += [VarSpec(f'{base}/res1/conv2d/w', (3, 3, cin, n), True, 'trunc:0.02'),
-              VarSpec(f'{base}/res1/conv2d/b', (n,), True, 'const:0')] + (_bn_specs(f'{base}/res1', n) if bn else []) + [
+              VarSpec(f'{base}/res1/conv2d/b', (n,), True, 'const:0')] + _norm_specs(f'{base}/res1', n, bn) + [
               VarSpec(f'{base}/res2/conv2d/w', (3, 3, n, n), True, 'trunc:0.02'),
-              VarSpec(f'{base}/res2/conv2d/b', (n,), True, 'const:0')] + (_bn_specs(f'{base}/res2', n) if bn else []) + [
+              VarSpec(f'{base}/res2/conv2d/b', (n,), True, 'const:0')] + _norm_specs(f'{base}/res2', n, bn) + [
               VarSpec(f'{base}/shortcut/conv2d/w', (1, 1, cin, n), True, 'trunc:0.02'),
               VarSpec(f'{base}/shortcut/conv2d/b', (n,), True, 'const:0')]
         cin = n

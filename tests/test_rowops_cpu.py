@@ -91,3 +91,30 @@ def test_two_runtimes_are_refused(built_lib):
             'except _lib.EdgeGANLibError as e:\n    print("refused", len(runtimes))\n' % ROOT)
     out = subprocess.run([sys.executable, '-c', code], capture_output=True, text=True, timeout=300).stdout.split()
     assert out in (['refused', '2'], ['taken', '1']), out
+
+
+@pytest.mark.parametrize('flags', [dict(G_norm='layernorm'), dict(E_norm='layernorm', D_norm='layernorm'), dict(E_norm='layernorm', G_norm='layernorm', D_norm='layernorm', num_classes=0)])
+def test_registry_layer_norm_flags(built_lib, flags):
+    """E_norm / G_norm / D_norm = 'layernorm': every normalised block gains a scale and a shift, and nothing else changes."""
+    import edgegan_amd as ea
+    import edgegan_oracle as O
+    cfg = ea.Config(batch_size=2, **flags)
+    got = [(s.name, tuple(s.shape), s.trainable) for s in ea.variable_specs(cfg)]
+    assert got == [(s.name, tuple(s.shape), s.trainable) for s in O.variable_specs(O.Config(batch_size=2, **flags))]
+    names = {n: sh for n, sh, _ in got}
+    assert ('G2/g_dconv_3/layer_norm/LayerNorm/gamma' in names) == (cfg.G_norm == 'layernorm')
+    assert ('D/d_conv_4/layer_norm/LayerNorm/beta' in names) == (cfg.D_norm == 'layernorm')
+    assert ('E/e_resnet_512_4/res2/layer_norm/LayerNorm/gamma' in names) == (cfg.E_norm == 'layernorm')
+    assert 'D/d_conv_0/layer_norm/LayerNorm/beta' not in names
+    v = ea.init_variables(cfg, seed=1)
+    for n in names:
+        if n.endswith('LayerNorm/gamma'):
+            assert np.all(v[n] == 1)
+        elif n.endswith('LayerNorm/beta'):
+            assert np.all(v[n] == 0)
+
+
+def test_layer_norm_flag_reaches_the_engine():
+    from edgegan_amd import flags as F, train as TR
+    fl = TR.update_flags(F.parse(['--D_norm=layernorm', '--E_norm', 'layernorm'], F.TRAIN_FLAGS))
+    F.check_supported(fl)
