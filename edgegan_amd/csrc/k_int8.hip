@@ -64,50 +64,51 @@ __global__ __launch_bounds__(256) void int8_any(Int8Args a, int tiles_n, int ali
 }
 
 // ---- tiles in LDS ------------------------------------------------------------------------------------------------------------------
-// BM x BN outputs a block, WM x WN waves, 128 bytes of k a step, two buffers: while a step's 32x32x32 products run, the next step's tiles are on their way from memory
-// straight to LDS.  A tile row is eight 16-byte groups; group s of row r holds the row's group s ^ (r / 2 & 7), so that sixteen rows of a
-// fragment lie in all 64 banks (with r & 7 half of the LDS time was bank conflicts; the write is a wave's 1,024 consecutive bytes: the permutation is in the source addresses).
+// BM x BN outputs a block, WM x WN waves, 64 bytes of k a step, a ring of four buffers: while a step's 32x32x32 products run, the tiles of the next three are on their
+// way from memory straight to LDS.  A tile row is four 16-byte groups; group s of row r holds the row's group s ^ (r / 4 & 3), so that sixteen rows of a
+// fragment lie in all 64 banks (the write is a wave's 1,024 consecutive bytes: the permutation is in the source addresses).
 // Rows past the end repeat the last one (their results are not stored); groups past k read as zeros; the bytes past k in its last group are cleared
 // in a's fragments, which is enough.
 using i32x16 = __attribute__((ext_vector_type(16))) int;
-constexpr int kStep = 128;
+constexpr int kStep = 64, kRing = 4;
 
 template <int BM, int BN, int WM, int WN>
 struct TileShape {
-  static constexpr int NW = WM * WN, MI = BM / WM / 32, NI = BN / WN / 32, JA = BM / 8 / NW, JB = BN / 8 / NW;
-  static_assert(JA * 8 * NW == BM && JB * 8 * NW == BN, "whole rows of 8 for every wave");
+  static constexpr int NW = WM * WN, MI = BM / WM / 32, NI = BN / WN / 32, JA = BM / 16 / NW, JB = BN / 16 / NW, BYTES = (BM + BN) * kStep, B_AT = BM * kStep;
+  static_assert(JA * 16 * NW == BM && JB * 16 * NW == BN, "whole rows of 16 for every wave");
 };
-// A wave's part of a tile: N times 8 rows, straight into LDS
+// A wave's part of a tile: N times 16 rows, straight into LDS
 template <int N>
 __device__ __forceinline__ void request_tile(__amdgpu_buffer_rsrc_t from, const unsigned (&voff)[N], bool in, int k, signed char* to, int waves, int wave) {
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     const unsigned v = in ? voff[j] : 0x80000000u;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void*)(to + (j * waves + wave) * 8 * kStep), 16, v, k, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void*)(to + (j * waves + wave) * 16 * kStep), 16, v, k, 0, 0);
   }
 }
-// One step: the next tiles requested (into `na`, `nb`), the current ones multiplied.  The four buffers are different memory and said to be (restrict): the compiler
-// would otherwise wait for the requests before it reads the current tiles.
-template <typename S, bool TAIL>
-__device__ __forceinline__ void int8_step(const signed char* __restrict__ ca, const signed char* __restrict__ cb, signed char* __restrict__ na, signed char* __restrict__ nb,
-                                          __amdgpu_buffer_rsrc_t ab, __amdgpu_buffer_rsrc_t bb, const unsigned (&va)[S::JA], const unsigned (&vb)[S::JB], int koff, int k_all, int k,
-                                          int wave, int lane, int arow, int brow, i32x16 (&acc)[S::MI][S::NI]) {
-  if constexpr (!TAIL) {
-    const bool in = k + kStep + koff < k_all;
-    request_tile<S::JA>(ab, va, in, k + kStep, na, S::NW, wave);
-    request_tile<S::JB>(bb, vb, in, k + kStep, nb, S::NW, wave);
+// One step: the tiles of three steps on requested (into `next`), the current ones multiplied.  The buffers are different memory and said to be (restrict): the compiler
+// would otherwise wait for the requests before it reads the current tiles.  LAST: nothing to request, and a's bytes past k are cleared.
+template <typename S, bool LAST>
+__device__ __forceinline__ void int8_step(const signed char* __restrict__ cur, signed char* __restrict__ next, __amdgpu_buffer_rsrc_t ab, __amdgpu_buffer_rsrc_t bb,
+                                          const unsigned (&va)[S::JA], const unsigned (&vb)[S::JB], int koff, int k_all, int k, int wave, int lane, int arow, int brow,
+                                          i32x16 (&acc)[S::MI][S::NI]) {
+  if constexpr (!LAST) {
+    const int ahead = k + (kRing - 1) * kStep;
+    const bool in = ahead + koff < k_all;   // (past k: zeros, from no memory)
+    request_tile<S::JA>(ab, va, in, ahead, next, S::NW, wave);
+    request_tile<S::JB>(bb, vb, in, ahead, next + S::B_AT, S::NW, wave);
     __builtin_amdgcn_sched_barrier(0);   // (the requests first: the scheduler would put them behind the products)
   }
   const int l31 = lane & 31, lh = lane >> 5;
 #pragma unroll
   for (int ks = 0; ks < kStep / 32; ++ks) {
-    const int slot = ((ks * 2 + lh) ^ ((l31 >> 1) & 7)) * 16;
+    const int slot = ((ks * 2 + lh) ^ ((l31 >> 2) & 3)) * 16;
     i32x4 fa[S::MI], fb[S::NI];
 #pragma unroll
-    for (int x = 0; x < S::MI; ++x) fa[x] = *reinterpret_cast<const i32x4*>(ca + (arow + x * 32) * kStep + slot);
+    for (int x = 0; x < S::MI; ++x) fa[x] = *reinterpret_cast<const i32x4*>(cur + (arow + x * 32) * kStep + slot);
 #pragma unroll
-    for (int y = 0; y < S::NI; ++y) fb[y] = *reinterpret_cast<const i32x4*>(cb + (brow + y * 32) * kStep + slot);
-    if constexpr (TAIL) {   // the last step: a's bytes past k
+    for (int y = 0; y < S::NI; ++y) fb[y] = *reinterpret_cast<const i32x4*>(cur + S::B_AT + (brow + y * 32) * kStep + slot);
+    if constexpr (LAST) {
       const int ends = k_all - k - (ks * 2 + lh) * 16;
 #pragma unroll
       for (int d = 0; d < 4; ++d) {
@@ -123,16 +124,18 @@ __device__ __forceinline__ void int8_step(const signed char* __restrict__ ca, co
   }
 }
 
-// every wave's requests have arrived, every wave's reads are done
+// Every wave's requests but those of the last two steps have arrived, and every wave's reads of the buffer before are done.  (__syncthreads would wait for
+// all requests.)
+template <typename S>
 __device__ __forceinline__ void tiles_ready() {
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
+  static_assert(2 * (S::JA + S::JB) == 8, "the wait below counts the requests of two steps");
+  asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
 template <typename T, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM * WN * 64) void int8_tiles(Int8Args a, int tiles_m, int tiles_n) {
+__global__ __launch_bounds__(WM * WN * 64) void int8_tiles(Int8Args a, int tiles_n) {
   using S = TileShape<BM, BN, WM, WN>;
-  __shared__ __attribute__((aligned(16))) signed char tiles[2][(BM + BN) * kStep];   // a's tile, b's tile
+  __shared__ __attribute__((aligned(16))) signed char tiles[kRing][S::BYTES];   // a's tile, b's tile
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
   const int tile = blockIdx.x;
@@ -141,14 +144,13 @@ __global__ __launch_bounds__(WM * WN * 64) void int8_tiles(Int8Args a, int tiles
   const int j0 = tn * BN;
 
   const __amdgpu_buffer_rsrc_t ab = row_buffer(a.a + i0 * a.lda, 0x7ffffff0u), bb = row_buffer(a.b + (long long)j0 * a.ldb, 0x7ffffff0u);
-  const int koff = ((lane & 7) ^ ((wave * 4 + (lane >> 4)) & 7)) * 16;   // this lane's group of its rows (8 (j NW + wave) + lane / 8) in k
-  static_assert(S::NW % 2 == 0, "the same group for every j");
+  const int koff = ((lane & 3) ^ ((lane >> 4) & 3)) * 16;   // this lane's group of its rows (16 (j NW + wave) + lane / 4) in k
   const int rows_a = (int)min((long long)BM, a.m - i0) - 1, rows_b = min(BN, a.n - j0) - 1;
   unsigned va[S::JA], vb[S::JB];
 #pragma unroll
-  for (int j = 0; j < S::JA; ++j) va[j] = (unsigned)min((j * S::NW + wave) * 8 + (lane >> 3), rows_a) * (unsigned)a.lda + koff;
+  for (int j = 0; j < S::JA; ++j) va[j] = (unsigned)min((j * S::NW + wave) * 16 + (lane >> 2), rows_a) * (unsigned)a.lda + koff;
 #pragma unroll
-  for (int j = 0; j < S::JB; ++j) vb[j] = (unsigned)min((j * S::NW + wave) * 8 + (lane >> 3), rows_b) * (unsigned)a.ldb + koff;
+  for (int j = 0; j < S::JB; ++j) vb[j] = (unsigned)min((j * S::NW + wave) * 16 + (lane >> 2), rows_b) * (unsigned)a.ldb + koff;
   i32x16 acc[S::MI][S::NI];
 #pragma unroll
   for (int x = 0; x < S::MI; ++x)
@@ -158,15 +160,19 @@ __global__ __launch_bounds__(WM * WN * 64) void int8_tiles(Int8Args a, int tiles
       for (int v = 0; v < 16; ++v) acc[x][y][v] = 0;
   const int l31 = lane & 31, lh = lane >> 5;
   const int arow = wm * (BM / WM) + l31, brow = wn * (BN / WN) + l31;
-  request_tile<S::JA>(ab, va, koff < a.k, 0, tiles[0], S::NW, wave);
-  request_tile<S::JB>(bb, vb, koff < a.k, 0, tiles[0] + BM * kStep, S::NW, wave);
-  int k = 0, cur = 0;
-  for (; k + kStep < a.k; k += kStep, cur ^= 1) {
-    tiles_ready();
-    int8_step<S, false>(tiles[cur], tiles[cur] + BM * kStep, tiles[cur ^ 1], tiles[cur ^ 1] + BM * kStep, ab, bb, va, vb, koff, a.k, k, wave, lane, arow, brow, acc);
+#pragma unroll
+  for (int p = 0; p < kRing - 1; ++p) {
+    request_tile<S::JA>(ab, va, p * kStep + koff < a.k, p * kStep, tiles[p], S::NW, wave);
+    request_tile<S::JB>(bb, vb, p * kStep + koff < a.k, p * kStep, tiles[p] + S::B_AT, S::NW, wave);
   }
-  tiles_ready();
-  int8_step<S, true>(tiles[cur], tiles[cur] + BM * kStep, nullptr, nullptr, ab, bb, va, vb, koff, a.k, k, wave, lane, arow, brow, acc);
+  int k = 0, cur = 0;
+  for (; k + kStep < a.k; k += kStep, cur = (cur + 1) % kRing) {
+    tiles_ready<S>();
+    int8_step<S, false>(tiles[cur], tiles[(cur + kRing - 1) % kRing], ab, bb, va, vb, koff, a.k, k, wave, lane, arow, brow, acc);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (the last step; and no request is left that would write where the scales go)
+  __syncthreads();
+  int8_step<S, true>(tiles[cur], nullptr, ab, bb, va, vb, koff, a.k, k, wave, lane, arow, brow, acc);
   // result layout: lane l, register v: row 8 (v / 4) + 4 (l >> 5) + v % 4, column l & 31
   const int jw = wn * (BN / WN) + l31, iw = wm * (BM / WM) + lh * 4;
   float* scales = reinterpret_cast<float*>(tiles[0]);   // the rows' scales
@@ -414,10 +420,10 @@ void launch_int8_matmul(const Int8Args& given, int out_type, hipStream_t s) {
       const long long big = ((a.m + 255) / 256) * ((a.n + 255) / 256);
       if (big >= 200) {
         const dim3 g = grid(256, 256, tm, tn);
-        return row_launch(int8_tiles<T, 256, 256, 2, 4>, g, dim3(512), s, a, tm, tn);
+        return row_launch(int8_tiles<T, 256, 256, 2, 4>, g, dim3(512), s, a, tn);
       }
       const dim3 g = grid(128, 128, tm, tn);
-      return row_launch(int8_tiles<T, 128, 128, 2, 2>, g, dim3(256), s, a, tm, tn);
+      return row_launch(int8_tiles<T, 128, 128, 2, 2>, g, dim3(256), s, a, tn);
     }
     const dim3 g = grid(64, 64, tm, tn);
     row_launch(int8_any<T>, g, dim3(256), s, a, tn, al_a, al_b);

@@ -1,5 +1,6 @@
 // C entries of the row operators (include/edgegan_hip.h): argument checks, the device, error codes.
 #include <cmath>
+#include <initializer_list>
 
 #include "../../include/edgegan_hip.h"
 #include "common.h"
@@ -16,9 +17,11 @@ namespace {
 struct OnDevice {
   int before = -1;
   explicit OnDevice(int device) {
-    int now = -1;
+    int now = -1, count = 0;
     EG_HIP(hipGetDevice(&now));
     if (now == device) return;
+    EG_HIP(hipGetDeviceCount(&count));
+    EG_CHECK(device >= 0 && device < count, "device %d of %d", device, count);
     EG_HIP(hipSetDevice(device));
     before = now;
   }
@@ -42,6 +45,15 @@ void check_matrix(const char* what, const void* p, long long ld, long long rows,
   EG_CHECK(ld >= 0 && (rows == 1 || ld <= (1ll << 62) / rows / elem), "%s: too large", what);
   EG_CHECK((uintptr_t)p % elem == 0, "%s: misaligned for its type", what);
 }
+void check_parameters(const char* what, int dtype, int wtype, const void* gamma, const void* beta) {
+  type_of(wtype, what);
+  EG_CHECK(wtype == dtype || wtype == EG_F32, "%s: gamma and beta of the rows' type or f32, not %d beside %d", what, wtype, dtype);
+  const uintptr_t e = wtype == EG_F32 ? 4 : 2;
+  EG_CHECK((uintptr_t)gamma % e == 0 && (uintptr_t)beta % e == 0, "%s: gamma or beta misaligned for its type", what);
+}
+void check_floats(const char* what, std::initializer_list<const float*> v) {
+  for (const float* p : v) EG_CHECK((uintptr_t)p % 4 == 0, "%s: a vector of f32 is misaligned", what);
+}
 void check_act(int act) { EG_CHECK(act == EG_ACT_NONE || act == EG_ACT_RELU || act == EG_ACT_LRELU, "unknown activation %d", act); }
 void check_eps(float eps) { EG_CHECK(eps > 0.f && std::isfinite(eps), "eps must be positive and finite"); }
 int bytes_of(int type) { return type == EG_F32 ? 4 : 2; }
@@ -56,6 +68,7 @@ int entry(F f) {
     f();
     return 0;
   } catch (const eg::Error& e) {
+    if (e.code == 2) (void)hipGetLastError();   // (reported here: the caller's next check is not to find it again)
     eg_set_global_error(e.what());
     return e.code;
   } catch (const std::exception& e) {
@@ -72,7 +85,8 @@ int eg_layer_norm(int device, void* stream, int dtype, const void* x, long long 
                   long long cols, float eps, int act, void* y, long long ldy, float* mean, float* rstd) {
   return entry([&] {
     type_of(dtype, "eg_layer_norm");
-    type_of(wtype, "eg_layer_norm parameters");
+    check_parameters("eg_layer_norm", dtype, wtype, gamma, beta);
+    check_floats("eg_layer_norm", {mean, rstd});
     check_rows("eg_layer_norm", rows, cols);
     check_matrix("eg_layer_norm x", x, ldx, rows, cols, bytes_of(dtype));
     check_matrix("eg_layer_norm y", y, ldy, rows, cols, bytes_of(dtype));
@@ -96,7 +110,9 @@ int eg_layer_norm_backward(int device, void* stream, int dtype, const void* dy, 
                            long long lddx, void* dgamma, void* dbeta, void* workspace, long long workspace_bytes) {
   return entry([&] {
     type_of(dtype, "eg_layer_norm_backward");
-    type_of(wtype, "eg_layer_norm_backward parameters");
+    check_parameters("eg_layer_norm_backward", dtype, wtype, gamma, beta);
+    check_parameters("eg_layer_norm_backward gradients", dtype, wtype, dgamma, dbeta);
+    check_floats("eg_layer_norm_backward", {mean, rstd});
     check_rows("eg_layer_norm_backward", rows, cols);
     const int e = bytes_of(dtype);
     check_matrix("eg_layer_norm_backward dy", dy, lddy, rows, cols, e);
@@ -122,6 +138,7 @@ int eg_quantize_rows(int device, void* stream, int dtype, const void* x, long lo
     check_rows("eg_quantize_rows", rows, cols);
     check_matrix("eg_quantize_rows x", x, ldx, rows, cols, bytes_of(dtype));
     check_matrix("eg_quantize_rows q", q, ldq, rows, cols, 1);
+    check_floats("eg_quantize_rows", {gamma, beta, scale});
     EG_CHECK(norm || (!gamma && !beta), "eg_quantize_rows: gamma and beta belong to the norm");
     if (norm) check_eps(eps);
     if (rows == 0) return;
@@ -147,6 +164,7 @@ int eg_int8_matmul(int device, void* stream, const signed char* a, long long lda
     check_matrix("eg_int8_matmul out", out, ldo, m, n, bytes_of(out_type));
     if (m == 0 || n == 0) return;
     EG_CHECK(a_scale && b_scale, "eg_int8_matmul: null scale");
+    check_floats("eg_int8_matmul", {a_scale, b_scale, bias});
     OnDevice on(device);
     launch_int8_matmul({a, lda, a_scale, b, ldb, b_scale, bias, m, (int)n, (int)k, out, ldo}, out_type, (hipStream_t)stream);
   });
@@ -172,6 +190,7 @@ int eg_int8_linear(int device, void* stream, int dtype, const void* x, long long
     if (rows == 0 || cols == 0) return;
     EG_CHECK(inner > 0, "eg_int8_linear: rows without columns");
     EG_CHECK(weight_scale, "eg_int8_linear: null scale");
+    check_floats("eg_int8_linear", {gamma, beta, weight_scale, bias});
     check_workspace("eg_int8_linear", workspace, workspace_bytes, int8_linear_bytes(rows, (int)inner) / 4);
     OnDevice on(device);
     launch_int8_linear({x, ldx, gamma, beta, norm != 0, eps, rows, (int)inner, nullptr, 0, nullptr},
@@ -199,6 +218,7 @@ int eg_distill_loss(int device, void* stream, int dtype, const void* logits, lon
     EG_CHECK(temperature > 0.f && std::isfinite(temperature) && std::isfinite(1.f / temperature), "eg_distill_loss: the temperature must be positive and finite");
     if (rows == 0) return;
     EG_CHECK(loss, "eg_distill_loss: null loss");
+    check_floats("eg_distill_loss", {row_weight, loss});
     EG_CHECK(cols > 0, "eg_distill_loss: rows without columns");
     check_workspace("eg_distill_loss", workspace, workspace_bytes, distill_partial_floats(rows, (int)cols, (int)top));
     OnDevice on(device);

@@ -89,9 +89,17 @@ def _like(x: torch.Tensor) -> torch.Tensor:
 
 
 def _act(act) -> int:
-    if act not in _ACTS:
+    if not (act is None or isinstance(act, str)) or act not in _ACTS:
         _refuse(f'act: {act!r} is not one of {", ".join(repr(a) for a in _ACTS)}')
     return _ACTS[act]
+
+
+def _number(v, name: str) -> float:
+    if type(v) is float:
+        return v
+    if isinstance(v, (int, float)):
+        return float(v)
+    _refuse(f'{name}: a number is required, not {type(v).__name__}')
 
 
 def _check(rc: int):
@@ -134,7 +142,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     if statistics:
         mean, rstd = x.new_empty(x.shape[:-1], dtype=torch.float32), x.new_empty(x.shape[:-1], dtype=torch.float32)
         pm, pr = mean.data_ptr(), rstd.data_ptr()
-    _check(lib.eg_layer_norm(device, _stream(device), _TYPES[x.dtype], x.data_ptr(), ld, _TYPES[wtype], w, b, rows, cols, eps, _act(act), y.data_ptr(), cols, pm, pr))
+    _check(lib.eg_layer_norm(device, _stream(device), _TYPES[x.dtype], x.data_ptr(), ld, _TYPES[wtype], w, b, rows, cols, _number(eps, 'eps'), _act(act), y.data_ptr(), cols, pm, pr))
     return (y, mean, rstd) if statistics else y
 
 
@@ -174,7 +182,7 @@ def _norm_parameters(norm, cols, device):
         return 0, None, None, 1.0
     if not isinstance(norm, (tuple, list)) or len(norm) != 3:
         _refuse('norm: (weight or None, bias or None, eps) is required')
-    return 1, _vector(norm[0], cols, 'norm weight', device, torch.float32), _vector(norm[1], cols, 'norm bias', device, torch.float32), norm[2]
+    return 1, _vector(norm[0], cols, 'norm weight', device, torch.float32), _vector(norm[1], cols, 'norm bias', device, torch.float32), _number(norm[2], 'eps')
 
 
 def quantize_rows(x: torch.Tensor, norm=None) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -276,5 +284,5 @@ def distill_loss(logits: torch.Tensor, index: torch.Tensor, teacher: torch.Tenso
     size = lib.eg_distill_loss_workspace(rows, cols, top)
     keep, ws = _workspace(size, logits)
     _check(lib.eg_distill_loss(device, _stream(device), _TYPES[logits.dtype], logits.data_ptr(), ld, _INDEXES[index.dtype], index.data_ptr(), ldi, teacher.data_ptr(), ldt,
-                               w, rows, cols, top, temperature, loss.data_ptr(), pg, cols, ws, size))
+                               w, rows, cols, top, _number(temperature, 'temperature'), loss.data_ptr(), pg, cols, ws, size))
     return loss, dlogits

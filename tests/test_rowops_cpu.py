@@ -42,10 +42,11 @@ CASES = [
     (norm, dict(ldy=-8), 'elements apart'), (norm, dict(rows=-1), 'rows'), (norm, dict(cols=(1 << 24) + 1), 'columns'), (norm, dict(cols=0), 'without columns'),
     (norm, dict(eps=0.0), 'eps'), (norm, dict(eps=float('inf')), 'eps'), (norm, dict(act=3), 'activation'), (norm, dict(mean=P), 'together'), (norm, dict(x=P + 2), 'misaligned'),
     (norm, dict(ldx=1 << 62), 'too large'),
+    (norm, dict(wtype=1), 'beside'), (norm, dict(dtype=2, wtype=1), 'beside'), (norm, dict(mean=P + 2, rstd=P), 'misaligned'),
     (backward, dict(ws=None), 'workspace'), (backward, dict(size=4), 'workspace'), (backward, dict(ws=P + 4), 'workspace'), (backward, dict(mean=None), 'statistics'),
     (backward, dict(x=None), 'null'), (backward, dict(lddx=3), 'elements apart'), (backward, dict(cols=0), 'without columns'),
     (quantize, dict(q=None), 'null'), (quantize, dict(ldq=7), 'elements apart'), (quantize, dict(scale=None), 'scale'), (quantize, dict(gamma=P), 'norm'),
-    (quantize, dict(norm=1, eps=-1.0), 'eps'), (quantize, dict(cols=0), 'without columns'),
+    (quantize, dict(norm=1, eps=-1.0), 'eps'), (quantize, dict(cols=0), 'without columns'), (quantize, dict(scale=P + 1), 'misaligned'), (product, dict(sa=P + 2), 'misaligned'), (distill, dict(loss=P + 2), 'misaligned'),
     (product, dict(k=131072, lda=131072), 'overflow'), (product, dict(m=-1), 'sizes'), (product, dict(n=1 << 30), 'sizes'), (product, dict(a=None), 'null'), (product, dict(lda=63), 'elements apart'),
     (product, dict(sa=None), 'scale'), (product, dict(out_type=7), 'type'), (product, dict(ldo=3), 'elements apart'),
     (linear, dict(dtype=9), 'type'), (linear, dict(x=None), 'null'), (linear, dict(ldx=63), 'elements apart'), (linear, dict(gamma=P), 'norm'), (linear, dict(norm=1, eps=0.0), 'eps'),

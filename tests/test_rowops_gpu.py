@@ -619,7 +619,7 @@ def test_refusals(ops):
     bad = [
         lambda: ops.layer_norm(x.cpu()), lambda: ops.layer_norm(x.double()), lambda: ops.layer_norm(x.t()), lambda: ops.layer_norm(x, v[:31]),
         lambda: ops.layer_norm(x, v.cpu()), lambda: ops.layer_norm(x, v.half()), lambda: ops.layer_norm(x, v, v.bfloat16()), lambda: ops.layer_norm(x, eps=0.0),
-        lambda: ops.layer_norm(x, eps=math.nan), lambda: ops.layer_norm(x, act='tanh'), lambda: ops.layer_norm(torch.empty(3, 0, device='cuda')),
+        lambda: ops.layer_norm(x, eps=math.nan), lambda: ops.layer_norm(x, eps=None), lambda: ops.layer_norm(x, act=['relu']), lambda: ops.distill_loss(x, idx, u, temperature='2'), lambda: ops.layer_norm(x, act='tanh'), lambda: ops.layer_norm(torch.empty(3, 0, device='cuda')),
         lambda: ops.layer_norm(torch.zeros((), device='cuda')), lambda: ops.layer_norm(x.view(2, 2, 32).transpose(0, 1)), lambda: ops.layer_norm(x[:1].expand(4, 32)),
         lambda: ops.layer_norm_backward(x[:3], x, m, m), lambda: ops.layer_norm_backward(x.half(), x, m, m), lambda: ops.layer_norm_backward(x, x, m[:3], m),
         lambda: ops.layer_norm_backward(x, x, None, m), lambda: ops.layer_norm_backward(x, x, m.half(), m),
@@ -638,4 +638,50 @@ def test_refusals(ops):
         with pytest.raises(EdgeGANLibError):
             f()
             pytest.fail(f'case {i} was taken')
+    lib = ops._library()                             # a device that is not there: an error code, and the current device stays
+    before = torch.cuda.current_device()
+    assert lib.eg_layer_norm(63, None, 0, x.data_ptr(), 32, 0, None, None, 4, 32, 1e-5, 0, x.data_ptr(), 32, None, None) != 0
+    assert torch.cuda.current_device() == before
     assert torch.isfinite(ops.layer_norm(x)).all()   # nothing is left behind
+
+
+def test_in_place(ops):
+    """The C entries may write over x, dy and the logits (same distance between rows)."""
+    lib, st = ops._library(), torch.cuda.current_stream().cuda_stream
+    for rows, cols in ((9, 100), (5, 1001), (3, 5000), (2, 40003), (2, 70000)):
+        x, dy, w = rnd(rows, cols, seed=1).cuda(), rnd(rows, cols, seed=2).cuda(), rnd(cols, seed=3).cuda()
+        y, m, r = ops.layer_norm(x, w, w, act='lrelu', statistics=True)
+        dx, dw, db = ops.layer_norm_backward(dy, x, m, r, w, w, act='lrelu')
+        z = x.clone()
+        assert lib.eg_layer_norm(0, st, 0, z.data_ptr(), cols, 0, w.data_ptr(), w.data_ptr(), rows, cols, 1e-5, 2, z.data_ptr(), cols, None, None) == 0
+        assert torch.equal(z, y), (rows, cols)
+        g, gw = dy.clone(), torch.empty(2, cols, device='cuda')
+        size = lib.eg_layer_norm_workspace(rows, cols)
+        ws = torch.empty(size, dtype=torch.uint8, device='cuda')
+        assert lib.eg_layer_norm_backward(0, st, 0, g.data_ptr(), cols, x.data_ptr(), cols, m.data_ptr(), r.data_ptr(), 0, w.data_ptr(), w.data_ptr(), rows, cols, 2,
+                                          g.data_ptr(), cols, gw[0].data_ptr(), gw[1].data_ptr(), ws.data_ptr(), size) == 0
+        assert torch.equal(g, dx) and torch.equal(gw[0], dw) and torch.equal(gw[1], db), (rows, cols)
+        idx, u = torch.randint(0, cols, (rows, 6), device='cuda'), torch.randn(rows, 6, device='cuda')
+        loss, grad = ops.distill_loss(x, idx, u, 2.0)
+        z, l2 = x.clone(), torch.empty(rows, device='cuda')
+        size = lib.eg_distill_loss_workspace(rows, cols, 6)
+        ws = torch.empty(max(size, 16), dtype=torch.uint8, device='cuda')
+        assert lib.eg_distill_loss(0, st, 0, z.data_ptr(), cols, 8, idx.data_ptr(), 6, u.data_ptr(), 6, None, rows, cols, 6, 2.0, l2.data_ptr(), z.data_ptr(), cols,
+                                   ws.data_ptr(), size) == 0
+        assert torch.equal(z, grad) and torch.equal(l2, loss), (rows, cols)
+
+
+def test_gradient_parts(ops):
+    """dx alone and the parameters' gradients alone, through the C entry; both are the whole call's."""
+    lib, st = ops._library(), torch.cuda.current_stream().cuda_stream
+    for rows, cols in ((300, 70), (4, 3001), (2, 50001)):
+        x, dy, w = rnd(rows, cols, seed=1).cuda(), rnd(rows, cols, seed=2).cuda(), rnd(cols, seed=3).cuda()
+        _, m, r = ops.layer_norm(x, w, None, statistics=True)
+        dx, dw, _ = ops.layer_norm_backward(dy, x, m, r, w, None)
+        size = lib.eg_layer_norm_workspace(rows, cols)
+        ws = torch.empty(size, dtype=torch.uint8, device='cuda')
+        a, b = torch.empty_like(x), torch.empty(cols, device='cuda')
+        args = (0, st, 0, dy.data_ptr(), cols, x.data_ptr(), cols, m.data_ptr(), r.data_ptr(), 0, w.data_ptr(), None, rows, cols, 0)
+        assert lib.eg_layer_norm_backward(*args, a.data_ptr(), cols, None, None, None, 0) == 0
+        assert lib.eg_layer_norm_backward(*args, None, 0, b.data_ptr(), None, ws.data_ptr(), size) == 0
+        assert torch.equal(a, dx) and torch.equal(b, dw), (rows, cols)
