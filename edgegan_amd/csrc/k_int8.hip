@@ -70,11 +70,11 @@ __global__ __launch_bounds__(256) void int8_any(Int8Args a, int tiles_n, int ali
 // Rows past the end repeat the last one (their results are not stored); groups past k read as zeros; the bytes past k in its last group are cleared
 // in a's fragments, which is enough.
 using i32x16 = __attribute__((ext_vector_type(16))) int;
-constexpr int kStep = 64, kRing = 4;
+constexpr int kStep = 64;
 
-template <int BM, int BN, int WM, int WN>
+template <int BM, int BN, int WM, int WN, int RING_>
 struct TileShape {
-  static constexpr int NW = WM * WN, MI = BM / WM / 32, NI = BN / WN / 32, JA = BM / 16 / NW, JB = BN / 16 / NW, BYTES = (BM + BN) * kStep, B_AT = BM * kStep;
+  static constexpr int RING = RING_, NW = WM * WN, MI = BM / WM / 32, NI = BN / WN / 32, JA = BM / 16 / NW, JB = BN / 16 / NW, BYTES = (BM + BN) * kStep, B_AT = BM * kStep;
   static_assert(JA * 16 * NW == BM && JB * 16 * NW == BN, "whole rows of 16 for every wave");
 };
 // A wave's part of a tile: N times 16 rows, straight into LDS
@@ -88,12 +88,12 @@ __device__ __forceinline__ void request_tile(__amdgpu_buffer_rsrc_t from, const 
 }
 // One step: the tiles of three steps on requested (into `next`), the current ones multiplied.  The buffers are different memory and said to be (restrict): the compiler
 // would otherwise wait for the requests before it reads the current tiles.  LAST: nothing to request, and a's bytes past k are cleared.
-template <typename S, bool LAST>
+template <typename S, int TURN, bool LAST>
 __device__ __forceinline__ void int8_step(const signed char* __restrict__ cur, signed char* __restrict__ next, __amdgpu_buffer_rsrc_t ab, __amdgpu_buffer_rsrc_t bb,
                                           const unsigned (&va)[S::JA], const unsigned (&vb)[S::JB], int koff, int k_all, int k, int wave, int lane, int arow, int brow,
                                           i32x16 (&acc)[S::MI][S::NI]) {
   if constexpr (!LAST) {
-    const int ahead = k + (kRing - 1) * kStep;
+    const int ahead = k + (S::RING - 1) * TURN;
     const bool in = ahead + koff < k_all;   // (past k: zeros, from no memory)
     request_tile<S::JA>(ab, va, in, ahead, next, S::NW, wave);
     request_tile<S::JB>(bb, vb, in, ahead, next + S::B_AT, S::NW, wave);
@@ -124,19 +124,23 @@ __device__ __forceinline__ void int8_step(const signed char* __restrict__ cur, s
   }
 }
 
-// Every wave's requests but those of the last two steps have arrived, and every wave's reads of the buffer before are done.  (__syncthreads would wait for
+// Every wave's requests but those of the last RING - 2 steps have arrived, and every wave's reads of the buffer before are done.  (__syncthreads would wait for
 // all requests.)
 template <typename S>
 __device__ __forceinline__ void tiles_ready() {
-  static_assert(2 * (S::JA + S::JB) == 8, "the wait below counts the requests of two steps");
-  asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  static_assert((S::RING - 2) * (S::JA + S::JB) < 64, "what vmcnt can count");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((S::RING - 2) * (S::JA + S::JB)) : "memory");
 }
 
-template <typename T, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM * WN * 64) void int8_tiles(Int8Args a, int tiles_n) {
-  using S = TileShape<BM, BN, WM, WN>;
-  __shared__ __attribute__((aligned(16))) signed char tiles[kRing][S::BYTES];   // a's tile, b's tile
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+template <typename T, int BM, int BN, int WM, int WN, int KS, int RING>
+__global__ __launch_bounds__(KS * WM * WN * 64) void int8_tiles(Int8Args a, int tiles_n) {
+  using S = TileShape<BM, BN, WM, WN, RING>;
+  constexpr int TURN = KS * kStep;   // bytes of k a step of the block takes
+  constexpr int TILES = RING * S::BYTES, SUMS = KS > 1 ? KS * BM * BN * 4 : 0;   // a part's ring (of a's tile, b's tile); later the parts' sums
+  __shared__ __attribute__((aligned(16))) signed char lds[std::max(KS * TILES, SUMS + BM * 4)];
+  const int lane = threadIdx.x & 63, all_wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int part = KS > 1 ? all_wave / S::NW : 0, wave = all_wave - part * S::NW;
+  signed char* const ring = lds + part * TILES;
   const int wm = wave / WN, wn = wave % WN;
   const int tile = blockIdx.x;
   const int tm = __builtin_amdgcn_readfirstlane(tile / tiles_n), tn = tile - tm * tiles_n;
@@ -160,24 +164,31 @@ __global__ __launch_bounds__(WM * WN * 64) void int8_tiles(Int8Args a, int tiles
       for (int v = 0; v < 16; ++v) acc[x][y][v] = 0;
   const int l31 = lane & 31, lh = lane >> 5;
   const int arow = wm * (BM / WM) + l31, brow = wn * (BN / WN) + l31;
+  int k = part * kStep, cur = 0;
 #pragma unroll
-  for (int p = 0; p < kRing - 1; ++p) {
-    request_tile<S::JA>(ab, va, p * kStep + koff < a.k, p * kStep, tiles[p], S::NW, wave);
-    request_tile<S::JB>(bb, vb, p * kStep + koff < a.k, p * kStep, tiles[p] + S::B_AT, S::NW, wave);
+  for (int p = 0; p < RING - 1; ++p) {
+    request_tile<S::JA>(ab, va, p * TURN + k + koff < a.k, p * TURN + k, ring + p * S::BYTES, S::NW, wave);
+    request_tile<S::JB>(bb, vb, p * TURN + k + koff < a.k, p * TURN + k, ring + p * S::BYTES + S::B_AT, S::NW, wave);
   }
-  int k = 0, cur = 0;
-  for (; k + kStep < a.k; k += kStep, cur = (cur + 1) % kRing) {
+  for (int left = a.k; left > TURN; left -= TURN, k += TURN, cur = (cur + 1) % RING) {
     tiles_ready<S>();
-    int8_step<S, false>(tiles[cur], tiles[(cur + kRing - 1) % kRing], ab, bb, va, vb, koff, a.k, k, wave, lane, arow, brow, acc);
+    int8_step<S, TURN, false>(ring + cur * S::BYTES, ring + (cur + RING - 1) % RING * S::BYTES, ab, bb, va, vb, koff, a.k, k, wave, lane, arow, brow, acc);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (the last step; and no request is left that would write where the scales go)
   __syncthreads();
-  int8_step<S, true>(tiles[cur], nullptr, ab, bb, va, vb, koff, a.k, k, wave, lane, arow, brow, acc);
+  int8_step<S, TURN, true>(ring + cur * S::BYTES, nullptr, ab, bb, va, vb, koff, a.k, k, wave, lane, arow, brow, acc);
+  // The products behind here, then 16 idle cycles before anything reads the sums: the compiler's own count of them was seen to miss reads behind a
+  // branch (a single product a wave: sums of rows 27 and 31 came out wrong).
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 15" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
   // result layout: lane l, register v: row 8 (v / 4) + 4 (l >> 5) + v % 4, column l & 31
   const int jw = wn * (BN / WN) + l31, iw = wm * (BM / WM) + lh * 4;
-  float* scales = reinterpret_cast<float*>(tiles[0]);   // the rows' scales
+  int* sums = reinterpret_cast<int*>(lds) + wave * 64 + lane;   // of one register of one part: all its waves' lanes in a row
+  float* scales = reinterpret_cast<float*>(lds + SUMS);         // the rows' scales
+  constexpr int NEXT = S::NW * 64;
   __syncthreads();
-  for (int i = threadIdx.x; i < BM; i += S::NW * 64) scales[i] = a.a_scale[i0 + min(i, rows_a)];
+  for (int i = threadIdx.x; i < BM; i += KS * S::NW * 64) scales[i] = a.a_scale[i0 + min(i, rows_a)];
   float sb[S::NI], bias[S::NI];
 #pragma unroll
   for (int y = 0; y < S::NI; ++y) {
@@ -185,125 +196,109 @@ __global__ __launch_bounds__(WM * WN * 64) void int8_tiles(Int8Args a, int tiles
     sb[y] = a.b_scale[j];
     bias[y] = a.bias ? a.bias[j] : 0.f;
   }
+  if constexpr (KS > 1) {
+#pragma unroll
+    for (int x = 0; x < S::MI; ++x)
+#pragma unroll
+      for (int y = 0; y < S::NI; ++y)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) sums[(((part * S::MI + x) * S::NI + y) * 16 + v) * NEXT] = acc[x][y][v];
+  }
   __syncthreads();
   // (a row or column past the end has an offset past the buffer's: its store is dropped)
   const __amdgpu_buffer_rsrc_t ob = row_buffer((T*)a.out + i0 * a.ldo + j0, 0x7ffffff0u);
 #pragma unroll
   for (int x = 0; x < S::MI; ++x)
 #pragma unroll
-    for (int v = 0; v < 16; ++v) {
+    for (int u = 0; u < 16 / KS; ++u) {
+      const int v = KS > 1 ? part * (16 / KS) + u : u;   // each part finishes its share of the registers
       const int i = iw + x * 32 + (v >> 2) * 8 + (v & 3);
       const float sa = scales[i];
       const unsigned at = i <= rows_a ? (unsigned)(i * (int)a.ldo + jw) * (unsigned)sizeof(T) : 0x80000000u;
 #pragma unroll
       for (int y = 0; y < S::NI; ++y) {
-        const float o[1] = {int8_result(acc[x][y][v], sa, sb[y], bias[y])};
+        int sum;
+        if constexpr (KS > 1) {
+          sum = 0;
+#pragma unroll
+          for (int p = 0; p < KS; ++p) sum += sums[(((p * S::MI + x) * S::NI + y) * 16 + v) * NEXT];
+        } else {
+          sum = acc[x][y][u];
+        }
+        const float o[1] = {int8_result(sum, sa, sb[y], bias[y])};
         buffer_store<T, 1>(ob, jw + y * 32 <= rows_b ? at + y * 32 * (unsigned)sizeof(T) : 0x80000000u, o);
       }
-      if (v % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      if (u % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
 }
 
 // ---- few rows of a ----------------------------------------------------------------------------------------------------------------
-// Up to 16 MT rows: bound by the bytes of b. A block takes 16 NT rows of b, its eight waves k by turns of 128 bytes, eight or four loads of b a lane in
-// flight; a comes from the caches or, where it is quantised in the same launch, from LDS.  The waves' sums are joined through LDS.
-constexpr int kFewWaves = 8, kFewTurn = kFewWaves * 128;
-template <int MT, int NT>
-struct FewShape {
-  static constexpr int U = MT * NT > 2 ? 2 : 4;   // turns at once
-};
-template <int MT, int NT>
-__device__ __forceinline__ void few_request(__amdgpu_buffer_rsrc_t bb, const unsigned (&vb)[NT], int k0, int lk, int k_all, i32x4 (&fb)[FewShape<MT, NT>::U][2][NT]) {
+// Up to 16 rows: bound by the bytes of b and by the time a load takes. A block takes 16 rows of b, its eight waves k by turns of 128 bytes, eight loads of b a
+// lane in flight; a comes from the caches or, where it is quantised in the same launch, from LDS.  The waves' sums are joined through LDS.
+constexpr int kFewWaves = 8, kFewTurn = kFewWaves * 128, kFewAhead = 4;   // kFewAhead: turns at once
+using FewOperand = i32x4[kFewAhead][2];
+
+__device__ __forceinline__ void few_request(__amdgpu_buffer_rsrc_t from, unsigned row, int k0, int lk, int k_all, FewOperand& f) {
 #pragma unroll
-  for (int u = 0; u < FewShape<MT, NT>::U; ++u)
+  for (int u = 0; u < kFewAhead; ++u)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int k = k0 + u * kFewTurn + h * 64;
-      const unsigned off = k + lk < k_all ? k : 0x80000000u;   // (groups past k read as zeros)
-#pragma unroll
-      for (int y = 0; y < NT; ++y) fb[u][h][y] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(bb, vb[y] + off, 0, 0));
+      const unsigned off = k + lk < k_all ? row + k : 0x80000000u;   // (groups past k read as zeros)
+      f[u][h] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(from, off, 0, 0));
     }
 }
-template <int MT, int NT>
-__device__ __forceinline__ void few_products(const i32x4 (&fa)[FewShape<MT, NT>::U][2][MT], const i32x4 (&fb)[FewShape<MT, NT>::U][2][NT], i32x4 (&acc)[MT][NT]) {
+__device__ __forceinline__ void few_products(const FewOperand& fa, const FewOperand& fb, i32x4& acc) {
 #pragma unroll
-  for (int u = 0; u < FewShape<MT, NT>::U; ++u)
+  for (int u = 0; u < kFewAhead; ++u)
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int x = 0; x < MT; ++x)
-#pragma unroll
-        for (int y = 0; y < NT; ++y) acc[x][y] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fa[u][h][x], fb[u][h][y], acc[x][y], 0, 0, 0);
+    for (int h = 0; h < 2; ++h) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(fa[u][h], fb[u][h], acc, 0, 0, 0);
 }
 // joins the waves' sums and writes the block's outputs; a_scale of row i
-template <typename T, int MT, int NT, typename S>
-__device__ __forceinline__ void few_finish(const Int8Args& a, int (&sums)[kFewWaves][MT * NT * 4][64], const i32x4 (&acc)[MT][NT], int j0, int lane, int wave, S a_scale) {
+template <typename T, typename S>
+__device__ __forceinline__ void few_finish(const Int8Args& a, int (&sums)[kFewWaves][4][64], const i32x4& acc, int j0, int lane, int wave, S a_scale) {
 #pragma unroll
-  for (int x = 0; x < MT; ++x)
-#pragma unroll
-    for (int y = 0; y < NT; ++y)
-#pragma unroll
-      for (int v = 0; v < 4; ++v) sums[wave][(x * NT + y) * 4 + v][lane] = acc[x][y][v];
+  for (int v = 0; v < 4; ++v) sums[wave][v][lane] = acc[v];
   __syncthreads();
   // result layout: lane l, register v: row 4 (l >> 4) + v, column l & 15
-  for (int o = wave; o < MT * NT * 4; o += kFewWaves) {
-    const int x = o / (NT * 4), y = o / 4 % NT, v = o % 4;
-    const int i = x * 16 + (lane >> 4) * 4 + v, j = j0 + y * 16 + (lane & 15);
-    if (i >= a.m || j >= a.n) continue;
-    int sum = 0;
+  if (wave >= 4) return;
+  const int i = (lane >> 4) * 4 + wave, j = j0 + (lane & 15);
+  if (i >= a.m || j >= a.n) return;
+  int sum = 0;
 #pragma unroll
-    for (int w = 0; w < kFewWaves; ++w) sum += sums[w][o][lane];
-    ((T*)a.out)[i * a.ldo + j] = (T)int8_result(sum, a_scale(i), a.b_scale[j], a.bias ? a.bias[j] : 0.f);
-  }
+  for (int w = 0; w < kFewWaves; ++w) sum += sums[w][wave][lane];
+  ((T*)a.out)[i * a.ldo + j] = (T)int8_result(sum, a_scale(i), a.b_scale[j], a.bias ? a.bias[j] : 0.f);
 }
 
-template <typename T, int MT, int NT>
+template <typename T>
 __global__ __launch_bounds__(kFewWaves * 64) void int8_few(Int8Args a) {
-  __shared__ int sums[kFewWaves][MT * NT * 4][64];
-  constexpr int U = FewShape<MT, NT>::U;
+  __shared__ int sums[kFewWaves][4][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l15 = lane & 15, lk = (lane >> 4) * 16;
-  const int j0 = blockIdx.x * 16 * NT;
+  const int j0 = blockIdx.x * 16;
   const __amdgpu_buffer_rsrc_t ab = row_buffer(a.a, 0x7ffffff0u), bb = row_buffer(a.b + (long long)j0 * a.ldb, 0x7ffffff0u);
-  unsigned va[MT], vb[NT];
+  const unsigned va = (unsigned)min(l15, (int)a.m - 1) * (unsigned)a.lda + lk, vb = (unsigned)min(l15, a.n - 1 - j0) * (unsigned)a.ldb + lk;
+  i32x4 acc = {0, 0, 0, 0};
+  for (int k0 = wave * 128; k0 < a.k; k0 += kFewAhead * kFewTurn) {
+    FewOperand fa, fb;
+    few_request(bb, vb, k0, lk, a.k, fb);
+    few_request(ab, va, k0, lk, a.k, fa);
+    if ((a.k & 15) && k0 + (kFewAhead - 1) * kFewTurn + 128 > a.k - 16) {   // this wave may hold the group that k ends in: a's bytes past it
 #pragma unroll
-  for (int x = 0; x < MT; ++x) va[x] = (unsigned)min(x * 16 + l15, (int)a.m - 1) * (unsigned)a.lda + lk;
-#pragma unroll
-  for (int y = 0; y < NT; ++y) vb[y] = (unsigned)min(y * 16 + l15, a.n - 1 - j0) * (unsigned)a.ldb + lk;
-  i32x4 acc[MT][NT];
-#pragma unroll
-  for (int x = 0; x < MT; ++x)
-#pragma unroll
-    for (int y = 0; y < NT; ++y) acc[x][y] = i32x4{0, 0, 0, 0};
-  for (int k0 = wave * 128; k0 < a.k; k0 += U * kFewTurn) {
-    i32x4 fa[U][2][MT], fb[U][2][NT];
-    few_request<MT, NT>(bb, vb, k0, lk, a.k, fb);
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int k = k0 + u * kFewTurn + h * 64;
-        const unsigned off = k + lk < a.k ? k : 0x80000000u;
-#pragma unroll
-        for (int x = 0; x < MT; ++x) fa[u][h][x] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(ab, va[x] + off, 0, 0));
-      }
-    if ((a.k & 15) && k0 + (U - 1) * kFewTurn + 128 > a.k - 16) {   // this wave may hold the group that k ends in: a's bytes past it
-#pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int u = 0; u < kFewAhead; ++u)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int ends = a.k - (k0 + u * kFewTurn + h * 64 + lk);
 #pragma unroll
           for (int d = 0; d < 4; ++d) {
-            const int keep = min(max(ends - 4 * d, 0), 4), mask = keep == 4 ? -1 : (1 << (8 * keep)) - 1;
-#pragma unroll
-            for (int x = 0; x < MT; ++x) fa[u][h][x][d] &= mask;
+            const int keep = min(max(ends - 4 * d, 0), 4);
+            fa[u][h][d] &= keep == 4 ? -1 : (1 << (8 * keep)) - 1;
           }
         }
     }
-    few_products<MT, NT>(fa, fb, acc);
+    few_products(fa, fb, acc);
   }
-  few_finish<T, MT, NT>(a, sums, acc, j0, lane, wave, [&](int i) { return a.a_scale[i]; });
+  few_finish<T>(a, sums, acc, j0, lane, wave, [&](int i) { return a.a_scale[i]; });
 }
 
 // The same for up to ROWS rows that are quantised here (behind their layer norm, if there is one): every block forms them for itself while its first loads of b are
@@ -311,7 +306,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void int8_few(Int8Args a) {
 // quantize_rows.
 template <typename T, int ROWS, int NV>
 __global__ __launch_bounds__(kFewWaves * 64) void int8_few_linear(Int8Args a, QuantizeArgs q) {
-  constexpr int V = 16 / sizeof(T), NT = 256, TURNS = (ROWS + 1) / 2, PITCH = NT * NV * V + 16, U = FewShape<1, 1>::U;
+  constexpr int V = 16 / sizeof(T), NT = 256, TURNS = (ROWS + 1) / 2, PITCH = NT * NV * V + 16;
   __shared__ int sums[kFewWaves][4][64];
   __shared__ __attribute__((aligned(16))) unsigned char rows[ROWS][PITCH];
   __shared__ double red[2][TURNS][centre_lds(NT)];
@@ -320,9 +315,9 @@ __global__ __launch_bounds__(kFewWaves * 64) void int8_few_linear(Int8Args a, Qu
   const int l15 = lane & 15, lk = (lane >> 4) * 16;
   const int j0 = blockIdx.x * 16;
   const __amdgpu_buffer_rsrc_t bb = row_buffer(a.b + (long long)j0 * a.ldb, 0x7ffffff0u);
-  const unsigned vb[1] = {(unsigned)min(l15, a.n - 1 - j0) * (unsigned)a.ldb + lk};
-  i32x4 acc[1][1] = {{i32x4{0, 0, 0, 0}}};
-  i32x4 fa[U][2][1], fb[U][2][1];
+  const unsigned vb = (unsigned)min(l15, a.n - 1 - j0) * (unsigned)a.ldb + lk;
+  i32x4 acc = {0, 0, 0, 0};
+  FewOperand fa, fb;
 
   // the rows and the norm's parameters before b: loads arrive in order, and they are what the next lines wait for
   const int t = threadIdx.x & (NT - 1), side = wave >> 2;
@@ -343,7 +338,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void int8_few_linear(Int8Args a, Qu
       for (int j = 0; j < V; ++j) v[n][i][j] = (float)k.e[j];
     }
   }
-  few_request<1, 1>(bb, vb, wave * 128, lk, a.k, fb);
+  few_request(bb, vb, wave * 128, lk, a.k, fb);
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (int n = 0; n < TURNS; ++n) {
@@ -382,20 +377,23 @@ __global__ __launch_bounds__(kFewWaves * 64) void int8_few_linear(Int8Args a, Qu
   }
   __syncthreads();
   const unsigned char* mine = rows[min(l15, ROWS - 1)];
-  for (int k0 = wave * 128; k0 < a.k; k0 += U * kFewTurn) {
-    if (k0 != wave * 128) few_request<1, 1>(bb, vb, k0, lk, a.k, fb);
+  for (int k0 = wave * 128; k0 < a.k; k0 += kFewAhead * kFewTurn) {
+    if (k0 != wave * 128) few_request(bb, vb, k0, lk, a.k, fb);
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < kFewAhead; ++u)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int k = k0 + u * kFewTurn + h * 64 + lk;
-        fa[u][h][0] = *reinterpret_cast<const i32x4*>(mine + (k < a.k ? k : 0));   // (past k: anything, b's are zeros)
+        fa[u][h] = *reinterpret_cast<const i32x4*>(mine + (k < a.k ? k : 0));   // (past k: anything, b's are zeros)
       }
-    few_products<1, 1>(fa, fb, acc);
+    few_products(fa, fb, acc);
   }
-  few_finish<T, 1, 1>(a, sums, acc, j0, lane, wave, [&](int i) { return scales[i]; });
+  few_finish<T>(a, sums, acc, j0, lane, wave, [&](int i) { return scales[i]; });
 }
 
+template <int I>
+using N = std::integral_constant<int, I>;
+constexpr int kCUs = 256;
 
 void launch_int8_matmul(const Int8Args& given, int out_type, hipStream_t s) {
   Int8Args a = given;
@@ -414,16 +412,31 @@ void launch_int8_matmul(const Int8Args& given, int out_type, hipStream_t s) {
     using T = decltype(t);
     int tm, tn;
     if (al_a && al_b && a.lda <= 1 << 22 && a.ldb <= 1 << 22 && a.ldo <= 1 << 20 && a.k >= 16) {
-      if (a.m <= 16) return row_launch(int8_few<T, 1, 1>, dim3((a.n + 15) / 16), dim3(kFewWaves * 64), s, a);
-      if (a.m <= 32) return row_launch(int8_few<T, 2, 1>, dim3((a.n + 15) / 16), dim3(kFewWaves * 64), s, a);
-      if (a.m <= 64) return row_launch(int8_few<T, 4, 2>, dim3((a.n + 31) / 32), dim3(kFewWaves * 64), s, a);
-      const long long big = ((a.m + 255) / 256) * ((a.n + 255) / 256);
-      if (big >= 200) {
-        const dim3 g = grid(256, 256, tm, tn);
-        return row_launch(int8_tiles<T, 256, 256, 2, 4>, g, dim3(512), s, a, tn);
-      }
-      const dim3 g = grid(128, 128, tm, tn);
-      return row_launch(int8_tiles<T, 128, 128, 2, 2>, g, dim3(256), s, a, tn);
+      // Up to 16 rows: 16 columns a block while that is at most one block a CU (n = k = 4096: 5.8 us for 16 rows, 4.4 for one, with tiles 6.3; n = 8192, k = 1024:
+      // 5.1 against 3.7).
+      if (a.m <= 16 && a.n <= 16 * kCUs) return row_launch(int8_few<T>, dim3((a.n + 15) / 16), dim3(kFewWaves * 64), s, a);
+      // The smallest tiles that are at most one a CU; no larger ones than the rows or columns fill.  us, of the same product with each tile:
+      //   m x n x k           32x64  64x64  64x128  128x128  256x128  256x256
+      //   64 x 4096 x 4096      6.5    8.1    11.9     18        -        -
+      //   256 x 4096 x 4096      13     11    12.8     18        -        -
+      //   512 x 4096 x 4096      23     20    15.7     20        -        -
+      //   1024 x 4096 x 4096     41     38    27.6     23        -       25
+      //   2048 x 4096 x 4096     77     72      51     45       42       53
+      //   4096 x 4096 x 4096    148    140     103     88       81       69
+      //   65536 x 128 x 1024      -      -      21      -     17.5       23
+      auto few_enough = [&](int bm, int bn) { return ((a.m + bm - 1) / bm) * ((a.n + bn - 1) / bn) <= kCUs; };
+      auto tiles = [&](auto bm, auto bn, auto wm, auto wn, auto ks, auto ring) {
+        constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WM = decltype(wm)::value, WN = decltype(wn)::value, KS = decltype(ks)::value;
+        const dim3 g = grid(BM, BN, tm, tn);
+        row_launch(int8_tiles<T, BM, BN, WM, WN, KS, decltype(ring)::value>, g, dim3(KS * WM * WN * 64), s, a, tn);
+      };
+      if (a.m <= 32 || few_enough(32, 64)) tiles(N<32>(), N<64>(), N<1>(), N<2>(), N<4>(), N<3>());
+      else if (few_enough(64, 64)) tiles(N<64>(), N<64>(), N<2>(), N<2>(), N<4>(), N<3>());
+      else if (a.m <= 64 || few_enough(64, 128)) tiles(N<64>(), N<128>(), N<2>(), N<2>(), N<2>(), N<3>());
+      else if (a.m <= 128 || few_enough(128, 128)) tiles(N<128>(), N<128>(), N<2>(), N<2>(), N<2>(), N<3>());
+      else if (a.n <= 128 || few_enough(256, 128)) tiles(N<256>(), N<128>(), N<4>(), N<2>(), N<1>(), N<4>());
+      else tiles(N<256>(), N<256>(), N<2>(), N<4>(), N<1>(), N<4>());
+      return;
     }
     const dim3 g = grid(64, 64, tm, tn);
     row_launch(int8_any<T>, g, dim3(256), s, a, tn, al_a, al_b);
@@ -445,7 +458,7 @@ void launch_int8_linear(const QuantizeArgs& given, const Int8Args& product, int 
   const int elem = type == ROW_F32 ? 4 : 2;
   const bool aligned = (uintptr_t)q.x % 16 == 0 && (a.m == 1 || q.ldx * elem % 16 == 0) && a.k % (16 / elem) == 0 && (uintptr_t)q.gamma % 16 == 0 && (uintptr_t)q.beta % 16 == 0 &&
                        (uintptr_t)a.b % 16 == 0 && (a.n == 1 || a.ldb % 16 == 0) && a.ldb <= 1 << 22;
-  if (aligned && type == out_type && a.m <= few_rows(type, a.k)) {
+  if (aligned && type == out_type && a.m <= few_rows(type, a.k) && a.n <= 32 * kCUs) {
     by_type(type, [&](auto t) {
       using T = decltype(t);
       constexpr int V = 16 / sizeof(T);

@@ -332,6 +332,19 @@ def test_int8_matmul_extremes(ops):
     assert torch.isnan(got[3]).all() and torch.equal(got[5], b) and torch.isfinite(got[[0, 1, 2, 4, 6]]).all()
 
 
+@pytest.mark.parametrize('m,n', [(40, 70), (31, 9000), (520, 1030), (1000, 1500), (50, 20000), (2000, 1900), (100, 34000), (4000, 2000), (66000, 70), (4100, 2100)])
+@pytest.mark.parametrize('k', [16, 100, 256, 513])
+def test_int8_matmul_tile_sizes(ops, m, n, k):
+    """One output shape for each of the tile sizes and of the reasons for which it is taken; k that ends in every part of a step."""
+    a, w, sa, sw, b = int8_case(ops, m, n, k, BF16, bias=k % 2 == 0, seed=k)
+    padded = []
+    for t in (a, w):   # rows 16 bytes apart, and no zeros behind them
+        store = torch.full((t.shape[0], -(-k // 16) * 16), 113, dtype=torch.int8, device='cuda')
+        store[:, :k] = t.cuda()
+        padded.append(store[:, :k])
+    check_int8(ops, a, w, sa, sw, b, BF16, *padded)
+
+
 def test_int8_matmul_empty(ops):
     z = lambda *s: torch.zeros(*s, dtype=torch.int8, device='cuda')
     f = lambda n: torch.ones(n, device='cuda')
