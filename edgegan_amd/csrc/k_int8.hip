@@ -174,6 +174,17 @@ __global__ __launch_bounds__(KS * WM * WN * 64) void int8_tiles(Int8Args a, int 
     tiles_ready<S>();
     int8_step<S, TURN, false>(ring + cur * S::BYTES, ring + (cur + RING - 1) % RING * S::BYTES, ab, bb, va, vb, koff, a.k, k, wave, lane, arow, brow, acc);
   }
+  // the scales and the bias on their way before the last step
+  static_assert(BM <= KS * S::NW * 64, "a thread for each row's scale");
+  const int jw = wn * (BN / WN) + l31, iw = wm * (BM / WM) + lh * 4;
+  const float sa_mine = a.a_scale[i0 + min((int)threadIdx.x, rows_a)];
+  float sb[S::NI], bias[S::NI];
+#pragma unroll
+  for (int y = 0; y < S::NI; ++y) {
+    const int j = j0 + min(jw + y * 32, rows_b);
+    sb[y] = a.b_scale[j];
+    bias[y] = a.bias ? a.bias[j] : 0.f;
+  }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (the last step; and no request is left that would write where the scales go)
   __syncthreads();
   int8_step<S, TURN, true>(ring + cur * S::BYTES, nullptr, ab, bb, va, vb, koff, a.k, k, wave, lane, arow, brow, acc);
@@ -183,19 +194,11 @@ __global__ __launch_bounds__(KS * WM * WN * 64) void int8_tiles(Int8Args a, int 
   asm volatile("s_nop 15" ::: "memory");
   __builtin_amdgcn_sched_barrier(0);
   // result layout: lane l, register v: row 8 (v / 4) + 4 (l >> 5) + v % 4, column l & 31
-  const int jw = wn * (BN / WN) + l31, iw = wm * (BM / WM) + lh * 4;
   int* sums = reinterpret_cast<int*>(lds) + wave * 64 + lane;   // of one register of one part: all its waves' lanes in a row
   float* scales = reinterpret_cast<float*>(lds + SUMS);         // the rows' scales
   constexpr int NEXT = S::NW * 64;
   __syncthreads();
-  for (int i = threadIdx.x; i < BM; i += KS * S::NW * 64) scales[i] = a.a_scale[i0 + min(i, rows_a)];
-  float sb[S::NI], bias[S::NI];
-#pragma unroll
-  for (int y = 0; y < S::NI; ++y) {
-    const int j = j0 + min(jw + y * 32, rows_b);
-    sb[y] = a.b_scale[j];
-    bias[y] = a.bias ? a.bias[j] : 0.f;
-  }
+  if (threadIdx.x < BM) scales[threadIdx.x] = sa_mine;
   if constexpr (KS > 1) {
 #pragma unroll
     for (int x = 0; x < S::MI; ++x)
