@@ -394,6 +394,84 @@ __global__ __launch_bounds__(kFewWaves * 64) void int8_few_linear(Int8Args a, Qu
   few_finish<T>(a, sums, acc, j0, lane, wave, [&](int i) { return scales[i]; });
 }
 
+// ---- short rows -------------------------------------------------------------------------------------------------------------------
+// Rows of up to 32 KS values, quantised in the registers of the waves that multiply them: a wave takes 32 rows and up to 128 columns, lane l the groups of 16
+// consecutive k of row l & 31 that the products take from it, so that x is read once from memory (by other columns' blocks from the caches) and no
+// quantised copy is written.  Bound by the bytes of x and of the output.
+template <typename T, int KS>
+__global__ __launch_bounds__(256) void int8_short_linear(Int8Args a, QuantizeArgs q) {
+  constexpr int V = 16 / sizeof(T), P = 16 / V, NY = 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int l31 = lane & 31, lh = lane >> 5;
+  const long long i0 = (long long)blockIdx.x * 128 + wave * 32;
+  if (i0 >= a.m) return;
+  const int j0 = blockIdx.y * 32 * NY, rows = (int)min(32ll, a.m - i0), cols = min(32 * NY, a.n - j0);
+  const __amdgpu_buffer_rsrc_t xb = row_buffer((const T*)q.x + i0 * q.ldx, 0x7ffffff0u), bb = row_buffer(a.b + (long long)j0 * a.ldb, 0x7ffffff0u);
+  const unsigned xrow = (unsigned)min(l31, rows - 1) * (unsigned)(q.ldx * sizeof(T));
+  Pack<T, V> x[KS][P];
+#pragma unroll
+  for (int s = 0; s < KS; ++s)
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const int k = s * 32 + lh * 16 + p * V;
+      x[s][p] = buffer_load<T, V>(xb, k < a.k ? xrow + k * sizeof(T) : 0x80000000u);   // (past k: zeros)
+    }
+  i32x4 fb[NY][KS];
+  float sb[NY], bias[NY];
+#pragma unroll
+  for (int y = 0; y < NY; ++y) {
+    const int j = min(y * 32 + l31, cols - 1);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int k = s * 32 + lh * 16;
+      fb[y][s] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(bb, k < a.k ? (unsigned)j * (unsigned)a.ldb + k : 0x80000000u, 0, 0));
+    }
+    sb[y] = a.b_scale[j0 + j];
+    bias[y] = a.bias ? a.bias[j0 + j] : 0.f;
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  float m = 0.f;
+#pragma unroll
+  for (int s = 0; s < KS; ++s)
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+      for (int j = 0; j < V; ++j) m = max_nan(m, fabsf((float)x[s][p].e[j]));
+  m = max_nan(m, __shfl_xor(m, 32));
+  const double inv = quantize_factor(m);
+  const bool fine = quantizable(m);
+  i32x4 fa[KS];
+#pragma unroll
+  for (int s = 0; s < KS; ++s)
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      unsigned four = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) four |= quantize1((float)x[s][(d * 4 + j) / V].e[(d * 4 + j) % V], inv) << (8 * j);
+      fa[s][d] = fine ? (int)four : 0;
+    }
+  const float mine = quantize_scale(m);
+  float sa[16];   // of the rows of this lane's results: 8 (v / 4) + 4 (l >> 5) + v % 4, column l & 31
+#pragma unroll
+  for (int v = 0; v < 16; ++v) sa[v] = __shfl(mine, (v >> 2) * 8 + lh * 4 + (v & 3));
+  // (a row or column past the end has an offset past the buffer's: its store is dropped)
+  const __amdgpu_buffer_rsrc_t ob = row_buffer((T*)a.out + i0 * a.ldo + j0, 0x7ffffff0u);
+#pragma unroll
+  for (int y = 0; y < NY; ++y) {
+    i32x16 acc;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) acc[v] = 0;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[s], fb[y][s], acc, 0, 0, 0);
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      const int i = (v >> 2) * 8 + lh * 4 + (v & 3), j = y * 32 + l31;
+      const float o[1] = {int8_result(acc[v], sa[v], sb[y], bias[y])};
+      buffer_store<T, 1>(ob, i < rows && j < cols ? (unsigned)(i * (int)a.ldo + j) * (unsigned)sizeof(T) : 0x80000000u, o);
+    }
+  }
+}
+
 template <int I>
 using N = std::integral_constant<int, I>;
 constexpr int kCUs = 256;
@@ -469,6 +547,19 @@ void launch_int8_linear(const QuantizeArgs& given, const Int8Args& product, int 
       if (a.m == 1 && a.k <= 256 * V * 2) row_launch(int8_few_linear<T, 1, 2>, grid, block, s, a, q);
       else if (a.m <= 2 && a.k > 256 * V * 2) row_launch(int8_few_linear<T, 2, 4>, grid, block, s, a, q);
       else row_launch(int8_few_linear<T, 4, 2>, grid, block, s, a, q);
+    });
+    return;
+  }
+  // Short rows in one launch too. us, against two launches: 65536 rows of 64 values by 128 columns, f32: 10.6 / 16.5; 256 by 256: 4.7 / 5.3; of 128 values
+  // 15.6 / 20.4, but 6.9 / 5.4 for 256 by 256 and 50 / 39 for 512 columns (every 128 columns quantise again).
+  const bool short_rows = a.k <= 64 || (a.k <= 128 && a.n <= 128 && a.m >= 64 * kCUs);
+  if (aligned && type == out_type && !q.norm && short_rows && q.ldx <= 1 << 20 && a.ldo <= 1 << 20 && a.n < 1 << 22) {
+    by_type(type, [&](auto t) {
+      using T = decltype(t);
+      const dim3 grid((unsigned)((a.m + 127) / 128), (a.n + 127) / 128);
+      if (a.k <= 32) row_launch(int8_short_linear<T, 1>, grid, dim3(256), s, a, q);
+      else if (a.k <= 64) row_launch(int8_short_linear<T, 2>, grid, dim3(256), s, a, q);
+      else row_launch(int8_short_linear<T, 4>, grid, dim3(256), s, a, q);
     });
     return;
   }

@@ -374,6 +374,28 @@ def test_int8_linear(ops, rows, inner, cols, norm, dtype):
     near(got.cpu(), full, 5 * step + half(dtype) * full.abs() + 1e-4, 'against the unquantised layer')
 
 
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+@pytest.mark.parametrize('rows,inner,cols', [(5, 8, 1), (31, 16, 33), (33, 24, 127), (129, 32, 128), (1000, 40, 129), (300, 56, 5000), (257, 64, 300), (16384, 128, 128), (16411, 72, 100)])
+def test_int8_linear_short_rows(ops, rows, inner, cols, dtype):
+    """Rows that are quantised where they are multiplied give the bits of the two calls; rows with NaN and infinities, of zeros and of tiny values among them."""
+    g = torch.Generator().manual_seed(rows + inner)
+    store = torch.randn(rows, inner + 16, generator=g).to(dtype)
+    x = store[:, :inner]
+    x[1], x[2, 1], x[3, 2], x[4] = 0, float('nan'), float('-inf'), x[4] * torch.finfo(dtype).tiny
+    store[:, inner:] = float('nan')   # behind the rows
+    qw, sw = ops.quantize_rows(torch.randn(cols, inner, generator=g).cuda())
+    bias = torch.randn(cols, generator=g).cuda()
+    xd = store.cuda()[:, :inner]
+    out = ops.int8_linear(xd, qw, sw, bias)
+    want = ops.int8_matmul(*ops.quantize_rows(xd), qw, sw, bias, dtype)
+    assert torch.equal(out.view(torch.uint8), want.view(torch.uint8)) and out[2:4].isnan().all() and not out[4:].isnan().any()
+    q, s = quantize64(torch.where(x.isfinite(), x, torch.zeros_like(x)))   # (the two rows that are not finite are left out below)
+    exact = (q.double() @ qw.cpu().double().t()) * s.double()[:, None] * sw.cpu().double() + bias.cpu().double()
+    fine = [r for r in range(min(rows, 300)) if r not in (2, 3)]
+    close = exact[fine]
+    near(out.cpu()[fine], close, 4 * U * ((exact - bias.cpu().double())[fine].abs() + close.abs()) * (1 + half(dtype)) + half(dtype) * close.abs() + tiny(dtype), 'short rows')
+
+
 # ---- distillation ----------------------------------------------------------------------------------------------------------------
 
 def distill64(z, idx, u, t, w, dtype=torch.float64):
