@@ -232,7 +232,7 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void distill_rows(DistillArgs 
 }
 
 // ---- a row over several blocks ----------------------------------------------------------------------------------------------------
-// Rows too long for a team's registers, or long ones too few for the chip's 256 compute units: blocks of kChunk columns, first their maximum and sum of
+// Rows too long for a team's registers, or a few that would fill them: blocks of kChunk columns, first their maximum and sum of
 // exponentials (and the student's logits in the teacher's columns) into the workspace [rows][2 chunks + top], then, in a second launch, the
 // loss and the gradient.  The row is read twice.
 constexpr int kChunkThreads = 256, kChunk = 8192;
@@ -334,8 +334,9 @@ __global__ __launch_bounds__(kChunkThreads) void distill_chunk_grad(DistillArgs 
   }
 }
 
-// One row a team where the registers hold it and the rows are enough for the chip, else chunks.
-static bool distill_in_chunks(long long rows, int cols) { return cols > 65536 || (cols > 2 * kChunk && rows < 64); }
+// A row a team while its registers hold the row, else chunks; chunks also for rows that fill those registers where they are few. us, team / chunks, bf16:
+//   32,768 columns: 9.2 / 10.7 for one row, 10.1 / 11.8 for 64, 13.3 / 18.0 for 256;  65,536: 12.6 / 10.9, 14.0 / 13.3, 20.0 / 29.5 (128 rows: 16.3 / 17.4)
+static bool distill_in_chunks(long long rows, int cols) { return cols > 65536 || (cols > 32768 && rows <= 64); }
 
 size_t distill_partial_floats(long long rows, int cols, int top) {
   return distill_in_chunks(rows, cols) ? (size_t)rows * (2 * chunks_of(cols) + top) : 0;

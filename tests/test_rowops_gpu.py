@@ -454,6 +454,14 @@ def test_distill(ops, rows, cols, top, dtype):
     assert torch.equal(loss, again), 'without the gradient, 4-byte indexes'
 
 
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+@pytest.mark.parametrize('rows,cols', [(65, 32769), (64, 32769), (66, 65536), (3, 32768), (5, 16385)])
+def test_distill_on_both_sides_of_the_chunk_rule(ops, rows, cols, dtype):
+    z = rnd(rows, cols, seed=rows + cols, dtype=dtype, scale=2.0)
+    u, idx = torch.topk(z.float() + rnd(rows, cols, seed=cols), 40, dim=1)
+    check_distill(ops, z, idx, u, 2.0, None)
+
+
 @pytest.mark.parametrize('cols', [14, 500, 5000, 40000, 150000])
 def test_distill_padding_and_ignored_rows(ops, cols):
     """Padding indexes, the same index twice, rows without a teacher, rows of weight 0 that hold NaN, masked classes (-inf), -inf in the teacher."""
