@@ -106,7 +106,7 @@ EXPORTS = ['eg_default_config', 'eg_variable_count', 'eg_variable_info', 'eg_cre
            'eg_comm_reduce_scalars', 'eg_comm_info', 'eg_comm_timing', 'eg_comm_timing_read',
            'eg_profile_begin', 'eg_profile_end', 'eg_profile_layers', 'eg_memory_stats', 'eg_mfma_probe', 'eg_test_op', 'eg_net_forward', 'eg_crc32c', 'eg_set_teacher', 'eg_teacher_loss', 'eg_infer_precision',
            'eg_layer_norm', 'eg_layer_norm_workspace', 'eg_layer_norm_backward', 'eg_quantize_rows', 'eg_int8_matmul',
-           'eg_int8_linear_workspace', 'eg_int8_linear', 'eg_distill_loss_workspace', 'eg_distill_loss']
+           'eg_int8_linear_workspace', 'eg_int8_linear_in_one', 'eg_int8_linear', 'eg_distill_loss_workspace', 'eg_distill_loss']
 
 _lib = None
 
@@ -170,6 +170,7 @@ def load_library() -> C.CDLL:
     lib.eg_quantize_rows.argtypes = [i, p, i, p, n, i, p, p, f, n, n, p, n, p]
     lib.eg_int8_matmul.argtypes = [i, p, p, n, p, p, n, p, p, n, n, n, i, p, n]
     lib.eg_int8_linear_workspace.argtypes = [n, n]
+    lib.eg_int8_linear_in_one.argtypes = [i, p, n, i, p, p, p, n, n, n, n, i, n]
     lib.eg_int8_linear.argtypes = [i, p, i, p, n, i, p, p, f, p, n, p, p, n, n, n, i, p, n, p, n]
     lib.eg_distill_loss_workspace.argtypes = [n, n, n]
     lib.eg_distill_loss.argtypes = [i, p, i, p, n, i, p, n, p, n, p, n, n, n, f, p, p, n, p, n]

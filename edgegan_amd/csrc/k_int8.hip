@@ -531,35 +531,43 @@ static long long few_rows(int type, int k) {   // rows that int8_few_linear take
 static long long linear_pitch(int k) { return (k + 15) & ~15; }
 size_t int8_linear_bytes(long long m, int k) { return ((size_t)m * linear_pitch(k) + 15) / 16 * 16 + (size_t)m * 4; }
 
-// quantize_rows and the product, in one launch where the rows are few
+// The forms that quantise and multiply in one launch, where x and the weights are aligned and x's type is the output's.
+//   few rows (int8_few_linear): up to 32 columns for each CU, us against two launches: 1 x 4096 x 4096 4.5 / 7.6, 4 x 4096 x 4096 6.5 / 8.0, 4 x 8192 x 2048 7.4 / 8.3;
+//   of 16384 columns 12.8 / 11.2
+//   short rows (int8_short_linear): 65536 rows of 64 values by 128 columns, f32: 10.6 / 16.5; 256 by 256: 4.7 / 5.3; of 128 values 15.6 / 20.4, but 6.9 / 5.4 for
+//   256 by 256 and 50 / 39 for 512 columns (every 128 columns quantise again)
+enum LinearForm { TWO_LAUNCHES, FEW_ROWS, SHORT_ROWS };
+static LinearForm linear_form(const QuantizeArgs& q, const Int8Args& a, int type, int out_type) {
+  const int elem = type == ROW_F32 ? 4 : 2;
+  if (type != out_type || (uintptr_t)q.x % 16 || (a.m > 1 && q.ldx * elem % 16) || a.k % (16 / elem) || (uintptr_t)q.gamma % 16 || (uintptr_t)q.beta % 16 || (uintptr_t)a.b % 16 ||
+      (a.n > 1 && a.ldb % 16) || a.ldb > 1 << 22)
+    return TWO_LAUNCHES;
+  if (a.m <= few_rows(type, a.k) && a.n <= 32 * kCUs) return FEW_ROWS;
+  const bool is_short = a.k <= 64 || (a.k <= 128 && a.n <= 128 && a.m >= 64 * kCUs);
+  return !q.norm && is_short && q.ldx <= 1 << 20 && a.ldo <= 1 << 20 && a.n < 1 << 22 ? SHORT_ROWS : TWO_LAUNCHES;
+}
+bool int8_linear_in_one(const QuantizeArgs& q, const Int8Args& a, int type, int out_type) { return linear_form(q, a, type, out_type) != TWO_LAUNCHES; }
+
 void launch_int8_linear(const QuantizeArgs& given, const Int8Args& product, int type, int out_type, void* workspace, hipStream_t s) {
   QuantizeArgs q = given;
   Int8Args a = product;
   if (a.m == 0 || a.n == 0) return;
-  const int elem = type == ROW_F32 ? 4 : 2;
-  const bool aligned = (uintptr_t)q.x % 16 == 0 && (a.m == 1 || q.ldx * elem % 16 == 0) && a.k % (16 / elem) == 0 && (uintptr_t)q.gamma % 16 == 0 && (uintptr_t)q.beta % 16 == 0 &&
-                       (uintptr_t)a.b % 16 == 0 && (a.n == 1 || a.ldb % 16 == 0) && a.ldb <= 1 << 22;
-  if (aligned && type == out_type && a.m <= few_rows(type, a.k) && a.n <= 32 * kCUs) {
+  const LinearForm form = linear_form(q, a, type, out_type);
+  if (form != TWO_LAUNCHES) {
     by_type(type, [&](auto t) {
       using T = decltype(t);
       constexpr int V = 16 / sizeof(T);
-      const dim3 grid((a.n + 15) / 16), block(kFewWaves * 64);
-      if (a.m == 1 && a.k <= 256 * V * 2) row_launch(int8_few_linear<T, 1, 2>, grid, block, s, a, q);
-      else if (a.m <= 2 && a.k > 256 * V * 2) row_launch(int8_few_linear<T, 2, 4>, grid, block, s, a, q);
-      else row_launch(int8_few_linear<T, 4, 2>, grid, block, s, a, q);
-    });
-    return;
-  }
-  // Short rows in one launch too. us, against two launches: 65536 rows of 64 values by 128 columns, f32: 10.6 / 16.5; 256 by 256: 4.7 / 5.3; of 128 values
-  // 15.6 / 20.4, but 6.9 / 5.4 for 256 by 256 and 50 / 39 for 512 columns (every 128 columns quantise again).
-  const bool short_rows = a.k <= 64 || (a.k <= 128 && a.n <= 128 && a.m >= 64 * kCUs);
-  if (aligned && type == out_type && !q.norm && short_rows && q.ldx <= 1 << 20 && a.ldo <= 1 << 20 && a.n < 1 << 22) {
-    by_type(type, [&](auto t) {
-      using T = decltype(t);
-      const dim3 grid((unsigned)((a.m + 127) / 128), (a.n + 127) / 128);
-      if (a.k <= 32) row_launch(int8_short_linear<T, 1>, grid, dim3(256), s, a, q);
-      else if (a.k <= 64) row_launch(int8_short_linear<T, 2>, grid, dim3(256), s, a, q);
-      else row_launch(int8_short_linear<T, 4>, grid, dim3(256), s, a, q);
+      if (form == FEW_ROWS) {
+        const dim3 grid((a.n + 15) / 16), block(kFewWaves * 64);
+        if (a.m == 1 && a.k <= 256 * V * 2) row_launch(int8_few_linear<T, 1, 2>, grid, block, s, a, q);
+        else if (a.m <= 2 && a.k > 256 * V * 2) row_launch(int8_few_linear<T, 2, 4>, grid, block, s, a, q);
+        else row_launch(int8_few_linear<T, 4, 2>, grid, block, s, a, q);
+      } else {
+        const dim3 grid((unsigned)((a.m + 127) / 128), (a.n + 127) / 128), block(256);
+        if (a.k <= 32) row_launch(int8_short_linear<T, 1>, grid, block, s, a, q);
+        else if (a.k <= 64) row_launch(int8_short_linear<T, 2>, grid, block, s, a, q);
+        else row_launch(int8_short_linear<T, 4>, grid, block, s, a, q);
+      }
     });
     return;
   }

@@ -191,11 +191,20 @@ int eg_int8_linear(int device, void* stream, int dtype, const void* x, long long
     EG_CHECK(inner > 0, "eg_int8_linear: rows without columns");
     EG_CHECK(weight_scale, "eg_int8_linear: null scale");
     check_floats("eg_int8_linear", {gamma, beta, weight_scale, bias});
-    check_workspace("eg_int8_linear", workspace, workspace_bytes, int8_linear_bytes(rows, (int)inner) / 4);
+    const QuantizeArgs q{x, ldx, gamma, beta, norm != 0, eps, rows, (int)inner, nullptr, 0, nullptr};
+    const Int8Args a{nullptr, 0, nullptr, weight, ldw, weight_scale, bias, rows, (int)cols, (int)inner, out, ldo};
+    if (workspace || workspace_bytes || !int8_linear_in_one(q, a, dtype, out_type))
+      check_workspace("eg_int8_linear", workspace, workspace_bytes, int8_linear_bytes(rows, (int)inner) / 4);
     OnDevice on(device);
-    launch_int8_linear({x, ldx, gamma, beta, norm != 0, eps, rows, (int)inner, nullptr, 0, nullptr},
-                       {nullptr, 0, nullptr, weight, ldw, weight_scale, bias, rows, (int)cols, (int)inner, out, ldo}, dtype, out_type, workspace, (hipStream_t)stream);
+    launch_int8_linear(q, a, dtype, out_type, workspace, (hipStream_t)stream);
   });
+}
+
+int eg_int8_linear_in_one(int dtype, const void* x, long long ldx, int norm, const float* gamma, const float* beta, const signed char* weight, long long ldw,
+                          long long rows, long long cols, long long inner, int out_type, long long ldo) {
+  if (dtype < 0 || dtype > ROW_F16 || rows < 0 || cols < 0 || cols > INT_MAX || inner < 1 || inner > 131071) return 0;
+  return int8_linear_in_one({x, ldx, gamma, beta, norm != 0, 1.f, rows, (int)inner, nullptr, 0, nullptr},
+                            {nullptr, 0, nullptr, weight, ldw, nullptr, nullptr, rows, (int)cols, (int)inner, nullptr, ldo}, dtype, out_type);
 }
 
 long long eg_distill_loss_workspace(long long rows, long long cols, long long top) {

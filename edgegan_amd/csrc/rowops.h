@@ -102,6 +102,7 @@ void launch_layer_norm_tangent_backward(const LayerNormTangentArgs& a, hipStream
 void launch_quantize_rows(const QuantizeArgs& a, int type, hipStream_t s);
 void launch_int8_matmul(const Int8Args& a, int out_type, hipStream_t s);
 size_t int8_linear_bytes(long long m, int k);
+bool int8_linear_in_one(const QuantizeArgs& q, const Int8Args& a, int type, int out_type);   // one launch, which needs no workspace
 void launch_int8_linear(const QuantizeArgs& q, const Int8Args& a, int type, int out_type, void* workspace, hipStream_t s);
 size_t distill_partial_floats(long long rows, int cols, int top);
 void launch_distill(const DistillArgs& a, int type, hipStream_t s);

@@ -88,6 +88,16 @@ def _like(x: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
 
 
+def _empty(x: torch.Tensor, shape, dtype: torch.dtype) -> torch.Tensor:
+    """A new consecutive tensor on x's GPU (with strides given torch allocates it in 1.2 us rather than 1.7)."""
+    n = len(shape)
+    if n == 1:
+        return torch.empty_strided(shape, (1,), dtype=dtype, device=x.device)
+    if n == 2 and shape[1]:
+        return torch.empty_strided(shape, (shape[1], 1), dtype=dtype, device=x.device)
+    return torch.empty(shape, dtype=dtype, device=x.device)
+
+
 def _act(act) -> int:
     if not (act is None or isinstance(act, str)) or act not in _ACTS:
         _refuse(f'act: {act!r} is not one of {", ".join(repr(a) for a in _ACTS)}')
@@ -112,7 +122,7 @@ def _workspace(size: int, x: torch.Tensor) -> Tuple[Optional[torch.Tensor], Opti
         _refuse('sizes out of range')
     if size == 0:
         return None, None
-    w = x.new_empty(size, dtype=torch.uint8)
+    w = _empty(x, (size,), torch.uint8)
     return w, w.data_ptr()
 
 
@@ -140,7 +150,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     y = _like(x)
     mean = rstd = pm = pr = None
     if statistics:
-        mean, rstd = x.new_empty(x.shape[:-1], dtype=torch.float32), x.new_empty(x.shape[:-1], dtype=torch.float32)
+        mean, rstd = _empty(x, x.shape[:-1], torch.float32), _empty(x, x.shape[:-1], torch.float32)
         pm, pr = mean.data_ptr(), rstd.data_ptr()
     _check(lib.eg_layer_norm(device, _stream(device), _TYPES[x.dtype], x.data_ptr(), ld, _TYPES[wtype], w, b, rows, cols, _number(eps, 'eps'), _act(act), y.data_ptr(), cols, pm, pr))
     return (y, mean, rstd) if statistics else y
@@ -195,8 +205,8 @@ def quantize_rows(x: torch.Tensor, norm=None) -> Tuple[torch.Tensor, torch.Tenso
     device = x.get_device()
     on, g, b, eps = _norm_parameters(norm, cols, device)
     pitch = (cols + 15) // 16 * 16
-    q = x.new_empty(x.shape[:-1] + (pitch,), dtype=torch.int8)
-    scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    q = _empty(x, x.shape[:-1] + (pitch,), torch.int8)
+    scale = _empty(x, x.shape[:-1], torch.float32)
     _check(lib.eg_quantize_rows(device, _stream(device), _TYPES[x.dtype], x.data_ptr(), ld, on, g, b, eps, rows, cols, q.data_ptr(), pitch, scale.data_ptr()))
     return (q if pitch == cols else q[..., :cols]), scale
 
@@ -227,7 +237,7 @@ def int8_matmul(q: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, weig
     b = _vector(bias, n, 'bias', device, torch.float32)
     if s is None or ws is None:
         _refuse('scale, weight_scale: required')
-    out = q.new_empty(q.shape[:-1] + (n,), dtype=out_dtype)
+    out = _empty(q, q.shape[:-1] + (n,), out_dtype)
     _check(lib.eg_int8_matmul(device, _stream(device), q.data_ptr(), lda, s, weight.data_ptr(), ldb, ws, b, m, n, k, _TYPES[out_dtype], out.data_ptr(), n))
     return out
 
@@ -235,7 +245,7 @@ def int8_matmul(q: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, weig
 def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias: Optional[torch.Tensor] = None, norm=None,
                 out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """A linear layer in 8-bit integers: int8_matmul(*quantize_rows(x, norm), weight, weight_scale, bias), in x's type unless out_dtype says otherwise; for few rows
-    one launch."""
+    and for short ones (64 values, without a norm) one launch."""
     lib = _lib or _library()
     m, k, ld = _rows(x, 'x')
     device = x.get_device()
@@ -248,11 +258,13 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     ws, b = _vector(weight_scale, n, 'weight_scale', device, torch.float32), _vector(bias, n, 'bias', device, torch.float32)
     if ws is None:
         _refuse('weight_scale: required')
-    out = x.new_empty(x.shape[:-1] + (n,), dtype=out_dtype)
-    size = lib.eg_int8_linear_workspace(m, k)
-    keep, wp = _workspace(size, x)
-    _check(lib.eg_int8_linear(device, _stream(device), _TYPES[x.dtype], x.data_ptr(), ld, on, g, beta, eps, weight.data_ptr(), ldw, ws, b, m, n, k, _TYPES[out_dtype],
-                              out.data_ptr(), n, wp, size))
+    out = _empty(x, x.shape[:-1] + (n,), out_dtype)
+    xt, ot, px, pw = _TYPES[x.dtype], _TYPES[out_dtype], x.data_ptr(), weight.data_ptr()
+    size, keep, wp = 0, None, None
+    if not lib.eg_int8_linear_in_one(xt, px, ld, on, g, beta, pw, ldw, m, n, k, ot, n):
+        size = lib.eg_int8_linear_workspace(m, k)
+        keep, wp = _workspace(size, x)
+    _check(lib.eg_int8_linear(device, _stream(device), xt, px, ld, on, g, beta, eps, pw, ldw, ws, b, m, n, k, ot, out.data_ptr(), n, wp, size))
     return out
 
 
@@ -276,7 +288,7 @@ def distill_loss(logits: torch.Tensor, index: torch.Tensor, teacher: torch.Tenso
     _, top, ldi = _rows(index, 'index', _INDEXES)
     ldt = _rows(teacher, 'teacher', _F32)[2]
     w = _vector(row_weight, rows, 'row_weight', device, torch.float32)
-    loss = logits.new_empty(shape, dtype=torch.float32)
+    loss = _empty(logits, shape, torch.float32)
     dlogits = pg = None
     if grad:
         dlogits = _like(logits)

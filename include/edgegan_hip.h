@@ -258,8 +258,11 @@ int eg_int8_matmul(int device, void* stream, const signed char* a, long long lda
                    long long ldb, const float* b_scale, const float* bias, long long m, long long n, long long k, int out_type,
                    void* out, long long ldo);
 /* A linear layer in 8-bit integers: eg_quantize_rows of x [rows x inner] and eg_int8_matmul with weight [cols x inner], the same numbers,
- * for few rows in one launch. The workspace holds the quantised rows (bytes: eg_int8_linear_workspace, -1 for bad sizes). */
+ * for few rows and for short ones in one launch. The workspace holds the quantised rows (bytes: eg_int8_linear_workspace, -1 for bad
+ * sizes); NULL and 0 will do where eg_int8_linear_in_one says that the call with these arguments is one launch. */
 long long eg_int8_linear_workspace(long long rows, long long inner);
+int eg_int8_linear_in_one(int dtype, const void* x, long long ldx, int norm, const float* gamma, const float* beta, const signed char* weight,
+                          long long ldw, long long rows, long long cols, long long inner, int out_type, long long ldo);
 int eg_int8_linear(int device, void* stream, int dtype, const void* x, long long ldx, int norm, const float* gamma, const float* beta,
                    float eps, const signed char* weight, long long ldw, const float* weight_scale, const float* bias, long long rows,
                    long long cols, long long inner, int out_type, void* out, long long ldo, void* workspace, long long workspace_bytes);

@@ -119,3 +119,16 @@ def test_layer_norm_flag_reaches_the_engine():
     from edgegan_amd import flags as F, train as TR
     fl = TR.update_flags(F.parse(['--D_norm=layernorm', '--E_norm', 'layernorm'], F.TRAIN_FLAGS))
     F.check_supported(fl)
+
+
+def test_linear_in_one_launch(built_lib):
+    """Which calls need no workspace, and that the others do not go without one."""
+    def one(dtype=0, x=P, ldx=64, norm=0, gamma=None, w=P, ldw=64, rows=2, cols=4, inner=64, out_type=0, ldo=4):
+        return built_lib.eg_int8_linear_in_one(dtype, x, ldx, norm, gamma, None, w, ldw, rows, cols, inner, out_type, ldo)
+    assert one() and one(norm=1) and one(rows=4) and one(rows=100) and one(rows=1, ldx=3, inner=4096, ldw=4096)
+    assert one(rows=100000, inner=128, ldx=128, ldw=128, cols=100, ldo=100)
+    for no in (dict(x=P + 4), dict(ldx=65), dict(w=P + 8), dict(ldw=72), dict(out_type=1), dict(inner=66, ldx=68, ldw=80), dict(rows=100, norm=1), dict(norm=1, gamma=P + 4),
+               dict(rows=100, inner=128, ldx=128, ldw=128), dict(rows=5, inner=4096, ldx=4096, ldw=4096), dict(rows=3, cols=20000, norm=1), dict(dtype=7), dict(rows=-1), dict(inner=0),
+               dict(inner=131072), dict(cols=-1), dict(cols=1 << 40)):
+        assert not one(**no), no
+    assert linear(built_lib, rows=100, norm=1, work=None, size=0) != 0 and b'workspace' in built_lib.eg_last_error(None)
