@@ -371,17 +371,22 @@ __global__ __launch_bounds__(256) void ln_bwd_columns(LayerNormGradArgs a) {
 static dim3 row_grid(long long rows) { return dim3((unsigned)std::min<long long>(rows, 1 << 20)); }
 static int part_groups(long long rows) { return (int)std::min<long long>(kPartBlocks, (rows + 3) / 4); }
 
-// Calls f(threads of a row, packs of a thread, elements of a pack, whether the last pack may be cut) for the smallest team whose registers hold a row of `cols`; false: none does.
-// A thread keeps at most MOST elements, 16 in a block of 1,024 (which has 128 registers a thread).
-template <typename T, int MOST, typename F>
+// Calls f(threads of a row, packs of a thread, elements of a pack, whether the last pack may be cut) for the smallest team whose registers hold a row of `cols`;
+// false: none does. A thread keeps at most WAVE elements where the team is a wave or less, BLOCK of 256 threads, 16 of 1,024 (which have 128 registers a thread).
+// The smallest team has the fewest joins and the most rows in flight; too small a one has too few waves on a CU or runs out of registers. us, with at
+// most 16 / 32 elements a thread, rows x columns: forward bf16 8192 x 2048 (256 threads or a wave) 21.4 / 16.6, 4096 x 8192 (1,024 or 256) 55 / 30.4, f32 4096 x 6000
+// 45 / 34.6, but 64 x 6000 4.0 / 4.6; quantisation of the same 16.0 / 12.8, 40.8 / 21.7, 37 / 28.7, 3.6 / 4.2.  Gradient: bf16 8192 x 2048 29.2 / 35.7, so 16 in a wave;
+// 4096 x 8192 124 / 59.5, so 32 in a block of 256; f32 4096 x 6000 64.0 / 64.6, 64 x 6000 10.4 / 11.0, so 16 there.  With at most 8, bf16 8192 x 4096
+// takes 97 (forward) and 148 (gradient), against 26 and 45.
+template <typename T, int WAVE, int BLOCK, typename F>
 static bool row_team(int cols, F f) {
   constexpr int V = 16 / sizeof(T);
   using std::integral_constant;
   auto pick = [&](auto tail) {
 #define EG_TEAM(NT, NV) \
-  if constexpr ((NV) * V <= ((NT) > 256 ? 16 : MOST)) \
+  if constexpr ((NV) * V <= ((NT) > 256 ? 16 : (NT) == 256 ? BLOCK : WAVE)) \
     if (cols <= (NT) * (NV) * V) return f(integral_constant<int, NT>{}, integral_constant<int, NV>{}, integral_constant<int, V>{}, tail), true;
-    EG_TEAM(8, 1) EG_TEAM(16, 1) EG_TEAM(32, 1) EG_TEAM(64, 1) EG_TEAM(64, 2) EG_TEAM(64, 4) EG_TEAM(256, 2) EG_TEAM(256, 4) EG_TEAM(1024, 2) EG_TEAM(1024, 4)
+    EG_TEAM(8, 1) EG_TEAM(16, 1) EG_TEAM(32, 1) EG_TEAM(64, 1) EG_TEAM(64, 2) EG_TEAM(64, 4) EG_TEAM(256, 2) EG_TEAM(256, 4) EG_TEAM(256, 8) EG_TEAM(1024, 2) EG_TEAM(1024, 4)
 #undef EG_TEAM
     return false;
   };
@@ -405,7 +410,7 @@ void launch_layer_norm(const LayerNormArgs& a, int type, int wtype, hipStream_t 
     using T = decltype(t);
     auto go = [&](auto w) {
       using W = decltype(w);
-      if (!row_team<T, 32>(a.cols, [&](auto nt, auto nv, auto v, auto tail) {
+      if (!row_team<T, 32, 32>(a.cols, [&](auto nt, auto nv, auto v, auto tail) {
             row_launch(ln_fwd<T, W, nt, nv, v, tail>, team_grid(a.rows, nt, 8192), team_block(nt), s, a);
           }))
         row_launch(ln_fwd_rows<T, W>, row_grid(a.rows), dim3(kRowThreads), s, a);
@@ -426,7 +431,7 @@ void launch_layer_norm_backward(const LayerNormGradArgs& given, int type, int wt
       using W = decltype(w);
       int groups = 0;
       if (a.rows) {
-        const bool held = row_team<T, 16>(a.cols, [&](auto nt, auto nv, auto v, auto tail) {
+        const bool held = row_team<T, 16, sizeof(T) == 2 ? 32 : 16>(a.cols, [&](auto nt, auto nv, auto v, auto tail) {
           const dim3 grid = team_grid(a.rows, nt, nt > 64 ? kGradBlocks / 2 : kGradBlocks);
           groups = (int)grid.x;
           row_launch(ln_bwd<T, W, nt, nv, v, tail>, grid, team_block(nt), s, a);
@@ -558,14 +563,14 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_tangent_bwd(LayerNormT
 
 void launch_layer_norm_tangent(const LayerNormTangentArgs& a, hipStream_t s) {
   if (!a.rows || !a.cols) return;
-  const bool held = row_team<float, 16>(a.cols, [&](auto nt, auto nv, auto v, auto tail) {
+  const bool held = row_team<float, 16, 16>(a.cols, [&](auto nt, auto nv, auto v, auto tail) {
     row_launch(ln_tangent<nt, nv, v, tail>, team_grid(a.rows, nt, 8192), team_block(nt), s, a);
   });
   EG_CHECK(held, "layer norm tangent: %d channels", a.cols);
 }
 void launch_layer_norm_tangent_backward(const LayerNormTangentArgs& a, hipStream_t s) {
   if (!a.rows || !a.cols) return;
-  const bool held = row_team<float, 16>(a.cols, [&](auto nt, auto nv, auto v, auto tail) {
+  const bool held = row_team<float, 16, 16>(a.cols, [&](auto nt, auto nv, auto v, auto tail) {
     const dim3 grid = team_grid(a.rows, nt, nt > 64 ? kGradBlocks / 2 : kGradBlocks);
     row_launch(ln_tangent_bwd<nt, nv, v, tail>, grid, team_block(nt), s, a);
     if (a.dgamma)
@@ -609,7 +614,7 @@ void launch_quantize_rows(const QuantizeArgs& a, int type, hipStream_t s) {
   by_type(type, [&](auto t) {
     using T = decltype(t);
     // (a row shorter than a pack: its team would not reach the end of its 16 bytes)
-    if (a.cols < (int)(16 / sizeof(T)) || !row_team<T, 32>(a.cols, [&](auto nt, auto nv, auto v, auto tail) {
+    if (a.cols < (int)(16 / sizeof(T)) || !row_team<T, 32, 32>(a.cols, [&](auto nt, auto nv, auto v, auto tail) {
           row_launch(quantize_rows<T, nt, nv, v, tail>, team_grid(a.rows, nt, 8192), team_block(nt), s, a);
         }))
       row_launch(quantize_kernel<T>, row_grid(a.rows), dim3(kRowThreads), s, a);
