@@ -550,7 +550,7 @@ static LinearForm linear_form(const QuantizeArgs& q, const Int8Args& a, int type
     return TWO_LAUNCHES;
   if (a.m <= few_rows(type, a.k) && a.n <= 32 * kCUs) return FEW_ROWS;
   const bool is_short = a.k <= 64 || (a.k <= 128 && a.n <= 128 && a.m >= 64 * kCUs);
-  return !q.norm && is_short && q.ldx <= 1 << 20 && a.ldo <= 1 << 20 && a.n < 1 << 22 ? SHORT_ROWS : TWO_LAUNCHES;
+  return !q.norm && is_short && q.ldx <= 1 << 20 && a.ldo <= 1 << 20 && a.n < 1 << 22 && a.m < 1 << 30 ? SHORT_ROWS : TWO_LAUNCHES;
 }
 bool int8_linear_in_one(const QuantizeArgs& q, const Int8Args& a, int type, int out_type) { return linear_form(q, a, type, out_type) != TWO_LAUNCHES; }
 

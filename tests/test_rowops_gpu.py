@@ -562,6 +562,26 @@ def test_offsets_past_32_bits(ops):
     assert torch.equal(ops.int8_matmul(w, ws, qs, s), ops.int8_matmul(w, ws, q, s))
 
 
+def test_far_rows_of_products(ops):
+    """Operands and results past 2^32 bytes, in the one-launch form for short rows and in the tiles."""
+    m, k, n = (1 << 25) + 77, 64, 70
+    x = torch.zeros(m, k, dtype=BF16, device='cuda')
+    ends = torch.cat([torch.arange(3), torch.arange(m - 300, m)]).cuda()
+    x[ends] = rnd(303, k, seed=1, dtype=BF16).cuda()
+    w, ws = ops.quantize_rows(rnd(n, k, seed=2).cuda())
+    bias = rnd(n, seed=3).cuda()
+    out = ops.int8_linear(x, w, ws, bias)
+    assert torch.equal(out[ends], ops.int8_linear(x[ends], w, ws, bias))
+    assert torch.equal(out[m // 2], bias.to(BF16))
+    del out
+    q, s = ops.quantize_rows(x)
+    assert torch.equal(q[ends], ops.quantize_rows(x[ends])[0])
+    w, ws = ops.quantize_rows(rnd(130, k, seed=4).cuda())
+    out = ops.int8_matmul(q, s, w, ws, out_dtype=BF16)
+    assert torch.equal(out[ends], ops.int8_matmul(q[ends], s[ends], w, ws, out_dtype=BF16))
+    assert not out[m // 2].any()
+
+
 # ---- together, on streams, in graphs ---------------------------------------------------------------------------------------------
 
 def head_step(ops, feats, gamma, beta, W, teacher_q, teacher_s, teacher_norm, top, t):
@@ -636,6 +656,62 @@ def test_on_another_stream_and_in_a_graph(ops):
         now = work()
         for i, (a, b, c) in enumerate(zip(held, held2, now)):
             assert torch.equal(a, c) and torch.equal(b, c), (step, i)
+
+
+def test_products_in_a_graph(ops):
+    """Every form of the 8-bit linear layer, captured twice and replayed between eager calls."""
+    shapes = [(1, 256, 40), (3, 256, 9000), (20, 256, 70), (300, 40, 300), (600, 256, 1030), (70, 130, 20000), (2000, 136, 1900), (4000, 256, 2000), (4100, 256, 2100), (16384, 128, 100)]
+    data = []
+    for i, (m, k, n) in enumerate(shapes):
+        data.append((rnd(m, k, seed=i, dtype=BF16).cuda(), *ops.quantize_rows(rnd(n, k, seed=100 + i).cuda())))
+
+    def work():
+        return [ops.int8_linear(*d) for d in data]
+    work()
+    graphs, held = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for g in graphs:
+        with torch.cuda.graph(g):
+            held.append(work())
+    for step in range(3):
+        for i, d in enumerate(data):
+            d[0].copy_(rnd(*d[0].shape, seed=1000 * step + i, dtype=BF16))
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for a, b, c, shape in zip(*held, work(), shapes):
+            assert torch.equal(a, c) and torch.equal(b, c), (step, shape)
+
+
+def test_two_threads(ops):
+    """Calls of two threads on streams of their own, each with the results of a call alone."""
+    import threading
+    sets = []
+    for i in range(2):
+        x, w = rnd(300, 1000 + 24 * i, seed=i).cuda(), rnd(1000 + 24 * i, seed=5 + i).cuda()
+        q, s = ops.quantize_rows(rnd(500, 1000 + 24 * i, seed=7 + i).cuda())
+        sets.append((x, w, q, s, torch.randint(0, 1000, (300, 9), device='cuda'), rnd(300, 9, seed=9 + i).cuda()))
+
+    def work(x, w, q, s, idx, u):
+        y, m, r = ops.layer_norm(x, w, None, act='relu', statistics=True)
+        return [y, *ops.layer_norm_backward(y, x, m, r, w, None, act='relu')[:2], ops.int8_linear(x, q, s), *ops.distill_loss(x, idx, u)]
+    want = [work(*d) for d in sets]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                got = work(*sets[i])
+            stream.synchronize()
+        if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+            wrong.append(i)
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
 
 
 def test_repeats_bit_for_bit(ops):
