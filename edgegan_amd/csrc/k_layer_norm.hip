@@ -70,10 +70,9 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_fwd(LayerNormArgs a) {
   }
 }
 
-// A block's sums of the parameter gradients to its row of partial [blocks][2][cols]; several teams of a block add up in their order.
-template <int NT, int NV, int V, int TEAMS>
-__device__ __forceinline__ void leave_partial(float* partial, int cols, int t, int team, const float (&sx)[NV][V], const float (&sg)[NV][V]) {
-  float* out = partial + (size_t)blockIdx.x * 2 * cols;
+// A block's sums of the parameter gradients: put(column, sum of g xh, sum of g); several teams of a block add up in their order.
+template <int NT, int NV, int V, int TEAMS, typename F>
+__device__ __forceinline__ void block_sums(int cols, int t, int team, const float (&sx)[NV][V], const float (&sg)[NV][V], F put) {
   if constexpr (TEAMS > 1) {
     __shared__ float sum[2][NT * NV * V];
     for (int k = 0; k < TEAMS; ++k) {
@@ -88,22 +87,25 @@ __device__ __forceinline__ void leave_partial(float* partial, int cols, int t, i
           }
       __syncthreads();
     }
-    for (int c = threadIdx.x; c < cols; c += NT * TEAMS) {
-      out[c] = sum[0][c];
-      out[cols + c] = sum[1][c];
-    }
+    for (int c = threadIdx.x; c < cols; c += NT * TEAMS) put(c, sum[0][c], sum[1][c]);
   } else {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * NT + t) * V;
 #pragma unroll
       for (int j = 0; j < V; ++j)
-        if (c + j < cols) {
-          out[c + j] = sx[i][j];
-          out[cols + c + j] = sg[i][j];
-        }
+        if (c + j < cols) put(c + j, sx[i][j], sg[i][j]);
     }
   }
+}
+// ... to the block's row of partial [blocks][2][cols]
+template <int NT, int NV, int V, int TEAMS>
+__device__ __forceinline__ void leave_partial(float* partial, int cols, int t, int team, const float (&sx)[NV][V], const float (&sg)[NV][V]) {
+  float* out = partial + (size_t)blockIdx.x * 2 * cols;
+  block_sums<NT, NV, V, TEAMS>(cols, t, team, sx, sg, [&](int c, float x, float g) {
+    out[c] = x;
+    out[cols + c] = g;
+  });
 }
 
 template <typename T, typename W, int NT, int NV, int V, bool TAIL>
@@ -189,6 +191,12 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_bwd(LayerNormGradArgs 
     });
   }
   if (a.partial) leave_partial<NT, NV, V, TEAMS>(a.partial, a.cols, t, team, sx, sg);
+  else if (a.dgamma || a.dbeta)   // the only block
+    block_sums<NT, NV, V, TEAMS>(a.cols, t, team, sx, sg, [&](int c, float x, float g) {
+      W *dgamma = (W*)a.dgamma, *dbeta = (W*)a.dbeta;
+      if (dgamma) dgamma[c] = (W)((a.acc_w & 1 ? (float)dgamma[c] : 0.f) + x);
+      if (dbeta) dbeta[c] = (W)((a.acc_w & 2 ? (float)dbeta[c] : 0.f) + g);
+    });
 }
 
 // partial [groups][2][cols] -> dgamma, dbeta: a block adds 32 of the 2 cols sums, 32 threads each every 32nd group
@@ -406,6 +414,13 @@ static dim3 team_block(int nt) { return dim3(nt > 256 ? nt : 256); }
 constexpr int kGradBlocks = 1024;   // half of them where the block is one row's team
 size_t layer_norm_partial_floats(long long rows, int cols) { return (size_t)std::min<long long>(kGradBlocks, rows) * 2 * cols; }
 
+// Few rows by one block, which then has the whole sums: no second launch, no workspace. 4 rows for each of its teams (as many teams as f32 rows have), 2 where
+// the block is one team.  us of a call / of its kernels, against two launches: 16 x 1000 bf16 11.6 / 6.7 (15.7 / 6.0), 32 x 128 11.3 / 5.1 (15.6 / 6.5), 2 x 4096 11.1 / 9.0
+// (15.6 / 8.6); with 8 rows a team 32 x 1000 11.4 / 9.7 (15.7 / 6.0), and 4 x 12000, in 1,024 threads, 26.5 / 26.9 (21.0 / 21.2).
+bool layer_norm_gradient_in_one(long long rows, int cols) {
+  return rows > 0 && rows <= (cols <= 32 ? 128 : cols <= 64 ? 64 : cols <= 128 ? 32 : cols <= 1024 ? 16 : cols <= 8192 ? 2 : 0);
+}
+
 void launch_layer_norm(const LayerNormArgs& a, int type, int wtype, hipStream_t s) {
   if (a.rows == 0 || a.cols == 0) return;
   by_type(type, [&](auto t) {
@@ -425,8 +440,8 @@ void launch_layer_norm(const LayerNormArgs& a, int type, int wtype, hipStream_t 
 void launch_layer_norm_backward(const LayerNormGradArgs& given, int type, int wtype, hipStream_t s) {
   LayerNormGradArgs a = given;
   if (a.cols == 0) return;
-  const bool params = a.dgamma || a.dbeta;
-  if (!params) a.partial = nullptr;
+  const bool params = a.dgamma || a.dbeta, one = layer_norm_gradient_in_one(a.rows, a.cols);
+  if (!params || one) a.partial = nullptr;
   by_type(type, [&](auto t) {
     using T = decltype(t);
     auto go = [&](auto w) {
@@ -434,7 +449,7 @@ void launch_layer_norm_backward(const LayerNormGradArgs& given, int type, int wt
       int groups = 0;
       if (a.rows) {
         const bool held = row_team<T, 16, sizeof(T) == 2 ? 32 : 16>(a.cols, [&](auto nt, auto nv, auto v, auto tail) {
-          const dim3 grid = team_grid(a.rows, nt, nt > 64 ? kGradBlocks / 2 : kGradBlocks);
+          const dim3 grid = team_grid(a.rows, nt, params && one ? 1 : nt > 64 ? kGradBlocks / 2 : kGradBlocks);
           groups = (int)grid.x;
           row_launch(ln_bwd<T, W, nt, nv, v, tail>, grid, team_block(nt), s, a);
         });
@@ -446,7 +461,7 @@ void launch_layer_norm_backward(const LayerNormGradArgs& given, int type, int wt
           if (a.dx) row_launch(ln_bwd_rows<T, W>, row_grid(a.rows), dim3(kRowThreads), s, a);
         }
       }
-      if (params)
+      if (params && !one)
         row_launch(ln_bwd_finish<W>, dim3((2 * a.cols + 31) / 32), dim3(1024), s, a.partial, groups, a.cols, (W*)a.dgamma, (W*)a.dbeta, a.acc_w);
     };
     if (wtype == type) go(t);

@@ -102,7 +102,7 @@ int eg_layer_norm(int device, void* stream, int dtype, const void* x, long long 
 
 long long eg_layer_norm_workspace(long long rows, long long cols) {
   if (rows < 0 || cols < 0 || cols > kMaxCols) return -1;
-  return (long long)layer_norm_partial_floats(rows, (int)cols) * 4;
+  return layer_norm_gradient_in_one(rows, (int)cols) ? 0 : (long long)layer_norm_partial_floats(rows, (int)cols) * 4;
 }
 
 int eg_layer_norm_backward(int device, void* stream, int dtype, const void* dy, long long lddy, const void* x, long long ldx, const float* mean,
@@ -120,7 +120,8 @@ int eg_layer_norm_backward(int device, void* stream, int dtype, const void* dy, 
     if (dx) check_matrix("eg_layer_norm_backward dx", dx, lddx, rows, cols, e);
     check_act(act);
     EG_CHECK(rows == 0 || (mean && rstd), "eg_layer_norm_backward: null statistics");
-    if (dgamma || dbeta) check_workspace("eg_layer_norm_backward", workspace, workspace_bytes, layer_norm_partial_floats(rows, (int)cols));
+    if ((dgamma || dbeta) && (workspace_bytes || !layer_norm_gradient_in_one(rows, (int)cols)))
+      check_workspace("eg_layer_norm_backward", workspace, workspace_bytes, layer_norm_partial_floats(rows, (int)cols));
     if (cols == 0) {
       EG_CHECK(rows == 0, "eg_layer_norm_backward: rows without columns have no mean");
       return;
@@ -193,7 +194,7 @@ int eg_int8_linear(int device, void* stream, int dtype, const void* x, long long
     check_floats("eg_int8_linear", {gamma, beta, weight_scale, bias});
     const QuantizeArgs q{x, ldx, gamma, beta, norm != 0, eps, rows, (int)inner, nullptr, 0, nullptr};
     const Int8Args a{nullptr, 0, nullptr, weight, ldw, weight_scale, bias, rows, (int)cols, (int)inner, out, ldo};
-    if (workspace || workspace_bytes || !int8_linear_in_one(q, a, dtype, out_type))
+    if (workspace_bytes || !int8_linear_in_one(q, a, dtype, out_type))
       check_workspace("eg_int8_linear", workspace, workspace_bytes, int8_linear_bytes(rows, (int)inner) / 4);
     OnDevice on(device);
     launch_int8_linear(q, a, dtype, out_type, workspace, (hipStream_t)stream);

@@ -94,6 +94,7 @@ struct DistillArgs {
   float* partial;             // distill_partial_floats()
 };
 
+bool layer_norm_gradient_in_one(long long rows, int cols);   // one launch, which needs no partial sums
 size_t layer_norm_partial_floats(long long rows, int cols);
 void launch_layer_norm(const LayerNormArgs& a, int type, int wtype, hipStream_t s);
 void launch_layer_norm_backward(const LayerNormGradArgs& a, int type, int wtype, hipStream_t s);

@@ -240,7 +240,7 @@ enum { EG_ACT_NONE = 0, EG_ACT_RELU = 1, EG_ACT_LRELU = 2 };        /* LeakyReLU
 int eg_layer_norm(int device, void* stream, int dtype, const void* x, long long ldx, int wtype, const void* gamma, const void* beta,
                   long long rows, long long cols, float eps, int act, void* y, long long ldy, float* mean, float* rstd);
 /* The gradient: dx [rows x cols], dgamma and dbeta [cols] (type wtype); each may be NULL.  beta matters only to an activation's sign.
- * The workspace (bytes: eg_layer_norm_workspace, -1 for bad sizes) is needed for dgamma / dbeta. */
+ * The workspace (bytes: eg_layer_norm_workspace, 0 for few rows, -1 for bad sizes) is needed for dgamma / dbeta. */
 long long eg_layer_norm_workspace(long long rows, long long cols);
 int eg_layer_norm_backward(int device, void* stream, int dtype, const void* dy, long long lddy, const void* x, long long ldx,
                            const float* mean, const float* rstd, int wtype, const void* gamma, const void* beta, long long rows,
@@ -259,7 +259,7 @@ int eg_int8_matmul(int device, void* stream, const signed char* a, long long lda
                    void* out, long long ldo);
 /* A linear layer in 8-bit integers: eg_quantize_rows of x [rows x inner] and eg_int8_matmul with weight [cols x inner], the same numbers,
  * for few rows and for short ones in one launch. The workspace holds the quantised rows (bytes: eg_int8_linear_workspace, -1 for bad
- * sizes); NULL and 0 will do where eg_int8_linear_in_one says that the call with these arguments is one launch. */
+ * sizes); NULL and 0 bytes will do where eg_int8_linear_in_one says that the call with these arguments is one launch. */
 long long eg_int8_linear_workspace(long long rows, long long inner);
 int eg_int8_linear_in_one(int dtype, const void* x, long long ldx, int norm, const float* gamma, const float* beta, const signed char* weight,
                           long long ldw, long long rows, long long cols, long long inner, int out_type, long long ldo);

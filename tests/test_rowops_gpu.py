@@ -134,6 +134,23 @@ def check_norm(ops, x, dy, w, b, eps, act, x_dev=None, dy_dev=None):
     return y, dx, dw, db
 
 
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+@pytest.mark.parametrize('rows,cols', [(128, 32), (129, 32), (128, 3), (64, 64), (65, 33), (32, 128), (33, 100), (16, 1024), (17, 1000), (13, 701), (1, 8192), (2, 8192), (3, 8192), (2, 5001), (2, 8193), (1, 1)])
+def test_layer_norm_gradient_of_few_rows(ops, rows, cols, dtype):
+    """On both sides of the rule by which one block does it all; the parameters' gradients one by one are the same, and the rows' sum is the sum of single rows'."""
+    x, dy, w, b = (rnd(*shape, seed=i + rows, dtype=dtype).cuda() for i, shape in enumerate([(rows, cols), (rows, cols), (cols,), (cols,)]))
+    _, m, r = ops.layer_norm(x, w, b, act='lrelu', statistics=True)
+    dx, dw, db = ops.layer_norm_backward(dy, x, m, r, w, b, act='lrelu')
+    assert torch.equal(ops.layer_norm_backward(dy, x, m, r, w, None)[1], ops.layer_norm_backward(dy, x, m, r, w, torch.zeros_like(b))[1])
+    xh = (x.double() - m.double()[:, None]) * r.double()[:, None]
+    z = xh * w.double() + b.double()
+    g = dy.double() * torch.where(z > 0, 1.0, 0.2)
+    near_kink = (z.abs() < 1e-4 * (1 + xh.abs())).any(0)      # (32 bits may put such an element on the other side)
+    for got, want, terms in ((dw, (g * xh).sum(0), (g * xh).abs().sum(0) + (g.abs() * (1 + xh.abs())).sum(0)), (db, g.sum(0), g.abs().sum(0))):
+        tol = (chain(rows) + 8 * U) * terms * (1 + half(dtype)) + half(dtype) * want.abs() + tiny(dtype)
+        near(got.cpu()[~near_kink.cpu()], want.cpu()[~near_kink.cpu()], tol.cpu()[~near_kink.cpu()], 'sums')
+
+
 @pytest.mark.parametrize('weight,bias,act', [(False, False, None), (True, False, 'lrelu'), (False, True, 'relu')])
 @pytest.mark.parametrize('rows,cols', [(5, 96), (3, 1030), (2, 9000)])
 def test_layer_norm_without_parameters(ops, rows, cols, weight, bias, act):
