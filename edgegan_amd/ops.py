@@ -150,7 +150,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     y = _like(x)
     mean = rstd = pm = pr = None
     if statistics:
-        mean, rstd = _empty(x, x.shape[:-1], torch.float32), _empty(x, x.shape[:-1], torch.float32)
+        mean = _empty(x, x.shape[:-1], torch.float32)
+        rstd = torch.empty_like(mean)
         pm, pr = mean.data_ptr(), rstd.data_ptr()
     _check(lib.eg_layer_norm(device, _stream(device), _TYPES[x.dtype], x.data_ptr(), ld, _TYPES[wtype], w, b, rows, cols, _number(eps, 'eps'), _act(act), y.data_ptr(), cols, pm, pr))
     return (y, mean, rstd) if statistics else y
