@@ -132,3 +132,13 @@ def test_linear_in_one_launch(built_lib):
                dict(inner=131072), dict(cols=-1), dict(cols=1 << 40)):
         assert not one(**no), no
     assert linear(built_lib, rows=100, norm=1, work=None, size=0) != 0 and b'workspace' in built_lib.eg_last_error(None)
+
+
+def test_gradient_workspace_sizes(built_lib):
+    """Few rows need none, and take none in its place; the others do not go without."""
+    size = built_lib.eg_layer_norm_workspace
+    for rows, cols in ((128, 32), (64, 64), (32, 128), (16, 1024), (2, 8192), (0, 5), (7, 0)):
+        assert size(rows, cols) == 0, (rows, cols)
+    for rows, cols in ((129, 32), (65, 64), (33, 128), (17, 1024), (3, 8192), (1, 8193), (1 << 40, 7)):
+        assert size(rows, cols) > 0 and size(rows, cols) % 4 == 0, (rows, cols)
+    assert backward(built_lib, rows=1000, ws=None, size=0) != 0 and b'workspace' in built_lib.eg_last_error(None)
