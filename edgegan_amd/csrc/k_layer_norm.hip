@@ -224,13 +224,17 @@ __global__ __launch_bounds__(1024) void ln_bwd_finish(const float* partial, int 
   *out = (W)s;
 }
 
+// Bytes of a row to write: the whole row, and zeros up to the end of its last 16-byte group as far as ldq leaves room (a single row may come with any ldq,
+// less than its length too).
+__device__ __forceinline__ int quantized_width(const QuantizeArgs& a) { return max(a.cols, (int)min((long long)((a.cols + 15) & ~15), a.ldq)); }
+
 template <typename T, int NT, int NV, int V, bool TAIL>
 __global__ __launch_bounds__(NT > 256 ? NT : 256) void quantize_rows(QuantizeArgs a) {
   constexpr int NB = NT > 256 ? NT : 256, TEAMS = NB / NT;
   __shared__ double red[2][centre_lds(NT)];
   __shared__ float red_max[2][NT > 64 ? NT / 64 : 1];
   const int t = TEAMS > 1 ? threadIdx.x % NT : threadIdx.x, team = TEAMS > 1 ? threadIdx.x / NT : 0;
-  const int width = (int)min((long long)((a.cols + 15) & ~15), a.ldq);   // the row's last 16-byte group is filled up with zeros
+  const int width = quantized_width(a);
   int turn = 0;
   for (long long r = (long long)blockIdx.x * TEAMS + team; r < a.rows; r += (long long)gridDim.x * TEAMS, turn ^= 1) {
     LoosePack<T, V> k[NV];
@@ -619,7 +623,7 @@ __global__ __launch_bounds__(kRowThreads) void quantize_kernel(QuantizeArgs a) {
     m = team_max<kRowThreads>(m, red_max);
     const bool fine = quantizable(m);
     const double inv = quantize_factor(m);
-    const int width = (int)min((long long)((a.cols + 15) & ~15), a.ldq);   // the row's last 16-byte group is filled up with zeros
+    const int width = quantized_width(a);
     for (int c = threadIdx.x; c < width; c += kRowThreads) q[c] = (unsigned char)(fine && c < a.cols ? quantize1(value(c), inv) : 0u);
     if (threadIdx.x == 0) a.scale[r] = quantize_scale(m);
     __syncthreads();

@@ -248,7 +248,8 @@ int eg_layer_norm_backward(int device, void* stream, int dtype, const void* dy, 
                            long long workspace_bytes);
 /* Rows in 8 bits: scale = max |x| / 127, q = the whole number nearest to 127 x / max |x| (a tie to the even one); a row of zeros has scale
  * 0, a row with a NaN or an infinity scale NaN and q = 0.  norm != 0: of the row's layer norm (gamma / beta f32 or NULL) in the same pass.
- * Each row of q is filled up with zeros to a multiple of 16 bytes where ldq leaves room (the last row's allocation too). */
+ * Each row of q is filled up with zeros to a multiple of 16 bytes where ldq leaves room (the last row's allocation too; a single
+ * row with ldq < cols is written whole and not filled up). */
 int eg_quantize_rows(int device, void* stream, int dtype, const void* x, long long ldx, int norm, const float* gamma, const float* beta,
                      float eps, long long rows, long long cols, signed char* q, long long ldq, float* scale);
 /* out[i][j] = (sum_k a[i][k] b[j][k]) a_scale[i] b_scale[j] + bias[j]: a [m x k] a scale for each row (token, position), b [n x k] one for

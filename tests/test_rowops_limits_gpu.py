@@ -1,0 +1,42 @@
+"""edgegan_amd.ops and its C entries at the limits of what they take: pitches of single rows, derivatives at exactly zero, the largest and smallest
+finite values and temperatures, workspaces of exactly the size asked for.  References, tolerances and their derivation: test_rowops_gpu."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+import test_rowops_gpu as R
+from test_rowops_gpu import BF16, F16, F32, TYPES, U, half, near, rnd, tiny
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope='module')
+def ops(built_lib):
+    from edgegan_amd import ops as o
+    return o
+
+
+def stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+@pytest.mark.parametrize('norm', [0, 1])
+@pytest.mark.parametrize('cols', [5, 37, 100, 1021, 4096, 20005])
+def test_quantize_one_row_at_any_pitch(ops, cols, norm, dtype):
+    """A single row's distance to the next one says nothing: all of the row is written whatever it is, zeros behind it only as far as it reaches."""
+    lib = ops._library()
+    x = rnd(1, cols, seed=cols, dtype=dtype, scale=2.0).cuda()
+    want, want_s = ops.quantize_rows(x, norm=(None, None, 1e-5) if norm else None)
+    whole = (cols + 15) // 16 * 16
+    for ldq in sorted({0, 1, cols - 1, cols, cols + 3, whole, whole + 16}):
+        q, s = torch.full((whole + 64,), 77, dtype=torch.int8, device='cuda'), torch.zeros(1, device='cuda')
+        assert lib.eg_quantize_rows(0, stream(), R_TYPES[dtype], x.data_ptr(), 0, norm, None, None, 1e-5, 1, cols, q.data_ptr(), ldq, s.data_ptr()) == 0
+        end = max(cols, min(whole, ldq))
+        assert torch.equal(q[:cols], want[0]) and torch.equal(s, want_s), ldq
+        assert (q[cols:end] == 0).all() and (q[end:] == 77).all(), ldq
+
+
+R_TYPES = {F32: 0, BF16: 1, F16: 2}
