@@ -161,7 +161,7 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_bwd(LayerNormGradArgs 
 #pragma unroll
           for (int j = 0; j < V; ++j) z[j] += (float)beta.k[i].e[j];
 #pragma unroll
-        for (int j = 0; j < V; ++j) d[i][j] *= row_act_grad(z[j], a.act);
+        for (int j = 0; j < V; ++j) d[i][j] *= row_act_grad(z[j], a.act, a.at_zero);
       });
     }
     float s[2] = {0.f, 0.f};
@@ -329,7 +329,7 @@ template <typename T, typename W>
 __device__ __forceinline__ void grad_terms(const LayerNormGradArgs& a, const T* x, const T* dy, float mean, float rstd, int c, float& g, float& xh) {
   xh = rounded_mul((float)x[c] - mean, rstd);
   g = (float)dy[c];
-  if (a.act != ACT_NONE) g *= row_act_grad(affine(xh, (const W*)a.gamma, (const W*)a.beta, c), a.act);
+  if (a.act != ACT_NONE) g *= row_act_grad(affine(xh, (const W*)a.gamma, (const W*)a.beta, c), a.act, a.at_zero);
 }
 
 template <typename T, typename W>
@@ -518,7 +518,7 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_tangent(LayerNormTange
     each_pack<NT, NV, V>(a.cols, t, [&](int i, int c) {
 #pragma unroll
       for (int j = 0; j < V; ++j)
-        v[i][j] = row_act_grad(rounded_mul(x[i][j], g[i][j]) + b[i][j], a.act) * g[i][j] * (rstd * (v[i][j] - mt - x[i][j] * bt));
+        v[i][j] = row_act_grad(rounded_mul(x[i][j], g[i][j]) + b[i][j], a.act, kEngineLreluAtZero) * g[i][j] * (rstd * (v[i][j] - mt - x[i][j] * bt));
       store_row_pack<float, V, TAIL>(a.ty + o, c, a.cols, v[i]);
     });
   }
@@ -550,7 +550,7 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_tangent_bwd(LayerNormT
 #pragma unroll
       for (int j = 0; j < V; ++j) {   // (past the end v = k = 0)
         x[i][j] = rounded_mul(x[i][j] - mean, rstd);
-        k[i][j] *= row_act_grad(rounded_mul(x[i][j], g[i][j]) + b[i][j], a.act);
+        k[i][j] *= row_act_grad(rounded_mul(x[i][j], g[i][j]) + b[i][j], a.act, kEngineLreluAtZero);
         b[i][j] = k[i][j];            // act' dty: dgamma's
         k[i][j] *= g[i][j];
         s[0] += v[i][j];

@@ -1589,7 +1589,7 @@ T ln_act(Ctx& c, T x, Param* gamma, Param* beta, int a, T* stats_out) {
       if (x->needs_grad) dx = grad_acc(c, x, &acc);
       const bool pg = c.param_grad_enabled && gamma->want_grad;
       if (!dx && !pg) return;
-      LayerNormGradArgs g{out->g, x->d, C, C, st->d, st->d + R, gamma->w, beta->w, R, C, a, dx, C, acc, pg ? gamma->g : nullptr, pg ? beta->g : nullptr,
+      LayerNormGradArgs g{out->g, x->d, C, C, st->d, st->d + R, gamma->w, beta->w, R, C, a, kEngineLreluAtZero, dx, C, acc, pg ? gamma->g : nullptr, pg ? beta->g : nullptr,
                           (gamma->g_set ? 1 : 0) | (beta->g_set ? 2 : 0), pg ? c.arena.allocf(layer_norm_partial_floats(R, C)) : nullptr};
       launch_layer_norm_backward(g, ROW_F32, ROW_F32, c.stream);
       if (pg) gamma->g_set = beta->g_set = true;

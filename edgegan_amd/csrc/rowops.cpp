@@ -127,7 +127,7 @@ int eg_layer_norm_backward(int device, void* stream, int dtype, const void* dy, 
       return;
     }
     OnDevice on(device);
-    launch_layer_norm_backward({dy, x, lddy, ldx, mean, rstd, gamma, beta, rows, (int)cols, act, dx, lddx, 0, dgamma, dbeta, 0, (float*)workspace}, dtype,
+    launch_layer_norm_backward({dy, x, lddy, ldx, mean, rstd, gamma, beta, rows, (int)cols, act, kLreluAtZero, dx, lddx, 0, dgamma, dbeta, 0, (float*)workspace}, dtype,
                                wtype, (hipStream_t)stream);
   });
 }

@@ -19,6 +19,9 @@ struct LayerNormArgs {
   long long ldy;
   float *mean, *rstd;         // [rows]; null: not stored (forward), required (backward)
 };
+// LeakyReLU's derivative at a pre-activation of exactly 0, where a row of one value has all of its elements unless there is a shift: the operators of
+// include/edgegan_hip.h take its slope, the engine 1, as its LeakyReLUs everywhere (max(z, 0.2 z), whose gradient goes to z where both are equal)
+constexpr float kLreluAtZero = 0.2f, kEngineLreluAtZero = 1.f;
 struct LayerNormGradArgs {
   const void *dy, *x;
   long long lddy, ldx;
@@ -27,6 +30,7 @@ struct LayerNormGradArgs {
   long long rows;
   int cols;
   int act;
+  float at_zero;              // kLreluAtZero / kEngineLreluAtZero
   void* dx;                   // null: not wanted
   long long lddx;
   int acc_x;                  // dx += (f32 only)
@@ -34,7 +38,7 @@ struct LayerNormGradArgs {
   int acc_w;                  // bit 0: dgamma +=, bit 1: dbeta +=
   float* partial;             // layer_norm_partial_floats()
 };
-// J_v of the layer norm at x and its reverse (f32; the gradient penalty of a critic)
+// J_v of the layer norm at x and its reverse (f32; the gradient penalty of a critic; LeakyReLU's derivative at 0 is kEngineLreluAtZero)
 struct LayerNormTangentArgs {
   const float *x, *mean, *rstd, *gamma, *beta, *tx;
   long long rows;

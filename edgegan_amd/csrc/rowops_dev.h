@@ -39,8 +39,8 @@ __device__ __forceinline__ float row_act(float z) {   // a NaN stays
   else if constexpr (ACT == ACT_LRELU) return fmaxf(z, 0.2f * z);
   else return z;
 }
-// derivative of row_act at the pre-activation z; at zero ReLU's is 0 and LeakyReLU's 1, as everywhere in the engine
-__device__ __forceinline__ float row_act_grad(float z, int act) { return act == ACT_NONE || z > 0.f ? 1.f : act == ACT_LRELU ? (z < 0.f ? 0.2f : 1.f) : 0.f; }
+// derivative of row_act at the pre-activation z; at zero ReLU's is 0 and LeakyReLU's `at_zero`
+__device__ __forceinline__ float row_act_grad(float z, int act, float at_zero) { return act == ACT_NONE || z > 0.f ? 1.f : act == ACT_LRELU ? (z < 0.f ? 0.2f : at_zero) : 0.f; }
 // f(the activation as a type)
 template <typename F>
 __device__ __forceinline__ void by_act(int act, F f) {

@@ -159,7 +159,9 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 
 def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, weight: Optional[torch.Tensor] = None,
                         bias: Optional[torch.Tensor] = None, act: Optional[str] = None):
-    """(dx, dweight, dbias) of layer_norm at x, with the statistics that it returned; dweight is None without a weight, dbias without a bias."""
+    """(dx, dweight, dbias) of layer_norm at x, with the statistics that it returned; dweight is None without a weight, dbias without a bias.
+
+    Where the pre-activation is exactly 0 the derivative of 'lrelu' is its slope 0.2, that of 'relu' 0."""
     lib = _lib or _library()
     rows, cols, ld = _rows(x, 'x')
     device = x.get_device()

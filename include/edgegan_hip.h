@@ -240,6 +240,8 @@ enum { EG_ACT_NONE = 0, EG_ACT_RELU = 1, EG_ACT_LRELU = 2 };        /* LeakyReLU
 int eg_layer_norm(int device, void* stream, int dtype, const void* x, long long ldx, int wtype, const void* gamma, const void* beta,
                   long long rows, long long cols, float eps, int act, void* y, long long ldy, float* mean, float* rstd);
 /* The gradient: dx [rows x cols], dgamma and dbeta [cols] (type wtype); each may be NULL.  beta matters only to an activation's sign.
+ * Where the pre-activation is exactly 0 (a row of one value with no shift or one of 0), LeakyReLU's derivative is its slope 0.2 and ReLU's 0; the engine's own
+ * block norms take 1 for LeakyReLU there, as the gradient of max(z, 0.2 z).
  * The workspace (bytes: eg_layer_norm_workspace, 0 for few rows, -1 for bad sizes) is needed for dgamma / dbeta. */
 long long eg_layer_norm_workspace(long long rows, long long cols);
 int eg_layer_norm_backward(int device, void* stream, int dtype, const void* dy, long long lddy, const void* x, long long ldx,

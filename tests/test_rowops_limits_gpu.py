@@ -40,3 +40,20 @@ def test_quantize_one_row_at_any_pitch(ops, cols, norm, dtype):
 
 
 R_TYPES = {F32: 0, BF16: 1, F16: 2}
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+@pytest.mark.parametrize('act', ['relu', 'lrelu'])
+@pytest.mark.parametrize('rows,cols', [(4, 3), (4, 24), (300, 100), (5, 1000), (40, 1001), (3, 5001), (3, 9000), (3, 20003)])
+def test_gradient_of_activations_at_zero(ops, rows, cols, act, dtype):
+    """Rows of one value (padding, mostly) have xh = 0, so with no shift or one of zeros every pre-activation is exactly 0: the derivative there is LeakyReLU's slope
+    (ReLU: 0), in every kernel, as in torch."""
+    x, dy = rnd(rows, cols, seed=1, dtype=dtype), rnd(rows, cols, seed=2, dtype=dtype)
+    x[0], x[1::3], x[2] = 0, 3.5, -0.25
+    w = rnd(cols, seed=3, dtype=dtype, scale=0.2, shift=1.0)
+    zero = torch.zeros(cols, dtype=dtype)
+    for weight, bias in ((w, None), (w, zero), (None, zero), (zero, zero), (None, None)):
+        y, dx, dw, db = R.check_norm(ops, x, dy, weight, bias, 1e-5, act)
+        assert (y[:3] == 0).all()
+    if act == 'relu':
+        assert (dx[:3] == 0).all()
