@@ -335,9 +335,8 @@ __global__ __launch_bounds__(kFewWaves * 64) void int8_few_linear(Int8Args a, Qu
     gamma.load(q.gamma, a.k, t);
     beta.load(q.beta, a.k, t);
   }
-  float v[TURNS][NV][V];
-#pragma unroll
-  for (int n = 0; n < TURNS; ++n) {
+  float v[TURNS][NV][V], mean[TURNS], rstd[TURNS];
+  auto load = [&](int n) {
     const long long r = min((long long)(2 * n + side), a.m - 1);
     const __amdgpu_buffer_rsrc_t xb = row_buffer((const T*)q.x + r * q.ldx, (unsigned)a.k * sizeof(T));
 #pragma unroll
@@ -346,23 +345,40 @@ __global__ __launch_bounds__(kFewWaves * 64) void int8_few_linear(Int8Args a, Qu
 #pragma unroll
       for (int j = 0; j < V; ++j) v[n][i][j] = (float)k.e[j];
     }
-  }
+  };
+#pragma unroll
+  for (int n = 0; n < TURNS; ++n) load(n);
   few_request(bb, vb, wave * 128, lk, a.k, fb);
   __builtin_amdgcn_sched_barrier(0);
+  if (q.norm) {
+    bool over[TURNS], any_over = false;   // this side's rows whose sums ran over; any row of the block
+#pragma unroll
+    for (int n = 0; n < TURNS; ++n) {
+      over[n] = centre_row<NT, NV, V, false>(v[n], a.k, t, q.eps, red[side][n], mean[n], rstd[n]);
+      double other = red[side ^ 1][n][NT / 64];   // the other side's sum, as its threads formed it
+#pragma unroll
+      for (int w = 1; w < NT / 64; ++w) other += red[side ^ 1][n][NT / 64 + w];
+      any_over |= over[n] | !finite(other);
+    }
+    if (may_run_over<T> && __builtin_expect(any_over, 0)) {   // (both sides come by its barriers)
+#pragma unroll
+      for (int n = 0; n < TURNS; ++n) load(n);
+      __syncthreads();
+#pragma unroll
+      for (int n = 0; n < TURNS; ++n) centre_row_again<NT, NV, V, false>(v[n], a.k, t, q.eps, red[side][n], over[n], mean[n], rstd[n]);
+    }
+  }
 #pragma unroll
   for (int n = 0; n < TURNS; ++n) {
-    if (q.norm) {
-      float mean, rstd;
-      centre_row<NT, NV, V, false>(v[n], a.k, t, q.eps, red[side][n], mean, rstd);
+    if (q.norm)
       each_pack<NT, NV, V>(a.k, t, [&](int i, int) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          v[n][i][j] = rounded_mul(v[n][i][j], rstd);
+          v[n][i][j] = rounded_mul(v[n][i][j], rstd[n]);
           if (q.gamma) v[n][i][j] = rounded_mul(v[n][i][j], gamma.k[i].e[j]);
           if (q.beta) v[n][i][j] += beta.k[i].e[j];
         }
       });
-    }
     float m = 0.f;
     each_pack<NT, NV, V>(a.k, t, [&](int i, int) {
 #pragma unroll

@@ -8,8 +8,10 @@
 //
 // All of it is bound by HBM, so a row is read once: it stays in the registers of the team of threads that owns it (8 to 64 lanes of a
 // wave, 256 or 1,024 threads: row_team) between the statistics and the result.  A team of a wave needs no LDS and no barrier; a wider one joins its
-// waves' sums through LDS.  The mean and the variance are summed in 64 bits, packs of a thread pairwise in 32 (the
-// mean decides every x - m, and a row of one value has xh = 0 exactly; and the statistics hardly ever depend on the team), the gradient's sums in 32.  xh gamma + beta is formed by the same three rounded operations in the forward and the gradient (no
+// waves' sums through LDS.  The mean and the variance are summed in 64 bits, packs of a thread pairwise in 32: the
+// mean decides every x - m, and the statistics hardly ever depend on the team.  A row of one value has xh = 0 exactly (its sums are exact; the rounded sum of a
+// last pack of three is off by less than what rounding the mean of seven or more takes back).  Where a pack's sum runs over in 32 bits, the row is
+// summed again in 64 (rows_that_ran_over).  The gradient's sums are in 32.  xh gamma + beta is formed by the same three rounded operations in the forward and the gradient (no
 // contraction into an fma), so the gradient's sign of it is the forward's.
 // Measured: forward 65,536 x 128 f32 12.8 us (5.2 TB/s; a copy of these bytes 6.5), 8,192 x 4,096 bf16 26 us; gradient 16,384 x 4,096 bf16 80 + 5 us
 // (4.7 TB/s with three tensors); quantisation 8,192 x 4,096 bf16 24 - 27 us (3.9 TB/s).
@@ -32,24 +34,11 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_fwd(LayerNormArgs a) {
   };
   constexpr bool HELD = NT <= 64;   // over the rows; a wider team sees few rows and reads them again, from the caches
   if constexpr (HELD) parameters();
-  int turn = 0;
-  const long long step = (long long)gridDim.x * TEAMS;
-  long long r = (long long)blockIdx.x * TEAMS + team;
-  LoosePack<T, V> next[NV];
-  if (r < a.rows) request_row<T, NT, NV, V>((const T*)a.x + r * a.ldx, a.cols, t, next);
-  for (; r < a.rows; r += step, turn ^= 1) {
-    float v[NV][V], mean, rstd;
-    settle_row<T, NT, NV, V, TAIL>(a.cols, t, next);
-    each_pack<NT, NV, V>(a.cols, t, [&](int i, int) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) v[i][j] = (float)next[i].e[j];
-    });
-    if (r + step < a.rows) request_row<T, NT, NV, V>((const T*)a.x + (r + step) * a.ldx, a.cols, t, next);
-    if constexpr (!HELD) parameters();
-    centre_row<NT, NV, V, TAIL>(v, a.cols, t, a.eps, red[turn], mean, rstd);
-    T* y = (T*)a.y + r * a.ldy;
+  auto finish = [&](long long row, float(&v)[NV][V], float mean, float rstd, bool store) {
+    T* y = (T*)a.y + row * a.ldy;
+    const int end = store ? a.cols : 0;
     by_act(a.act, [&](auto act) {
-      each_pack<NT, NV, V>(a.cols, t, [&](int i, int c) {
+      each_pack<NT, NV, V>(end, t, [&](int i, int c) {
 #pragma unroll
         for (int j = 0; j < V; ++j) v[i][j] = rounded_mul(v[i][j], rstd);
         if (a.gamma)
@@ -64,9 +53,33 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_fwd(LayerNormArgs a) {
       });
     });
     if (t == 0 && a.mean) {
-      a.mean[r] = mean;
-      a.rstd[r] = rstd;
+      a.mean[row] = mean;
+      a.rstd[row] = rstd;
     }
+  };
+  int turn = 0;
+  const long long step = (long long)gridDim.x * TEAMS, first = (long long)blockIdx.x * TEAMS + team;
+  long long r = first;
+  bool any_over = false;
+  LoosePack<T, V> next[NV];
+  if (r < a.rows) request_row<T, NT, NV, V>((const T*)a.x + r * a.ldx, a.cols, t, next);
+  for (; r < a.rows; r += step, turn ^= 1) {
+    float v[NV][V], mean, rstd;
+    settle_row<T, NT, NV, V, TAIL>(a.cols, t, next);
+    each_pack<NT, NV, V>(a.cols, t, [&](int i, int) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[i][j] = (float)next[i].e[j];
+    });
+    if (r + step < a.rows) request_row<T, NT, NV, V>((const T*)a.x + (r + step) * a.ldx, a.cols, t, next);
+    if constexpr (!HELD) parameters();
+    const bool over = centre_row<NT, NV, V, TAIL>(v, a.cols, t, a.eps, red[turn], mean, rstd) && may_run_over<T>;
+    any_over |= over;
+    finish(r, v, mean, rstd, !over);   // (such a row is left: y may be x)
+  }
+  if (any_over) {
+    if constexpr (!HELD) parameters();
+    rows_that_ran_over<T, NT, NV, V, TAIL>((const T*)a.x, a.ldx, first, a.rows, step, a.cols, t, a.eps, red,
+                                           [&](long long row, float(&v)[NV][V], float mean, float rstd) { finish(row, v, mean, rstd, true); });
   }
 }
 
@@ -235,23 +248,12 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void quantize_rows(QuantizeArg
   __shared__ float red_max[2][NT > 64 ? NT / 64 : 1];
   const int t = TEAMS > 1 ? threadIdx.x % NT : threadIdx.x, team = TEAMS > 1 ? threadIdx.x / NT : 0;
   const int width = quantized_width(a);
-  int turn = 0;
-  for (long long r = (long long)blockIdx.x * TEAMS + team; r < a.rows; r += (long long)gridDim.x * TEAMS, turn ^= 1) {
-    LoosePack<T, V> k[NV];
-    request_row<T, NT, NV, V>((const T*)a.x + r * a.ldx, a.cols, t, k);
-    settle_row<T, NT, NV, V, TAIL>(a.cols, t, k);
-    float v[NV][V];
-    each_pack<NT, NV, V>(a.cols, t, [&](int i, int) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) v[i][j] = (float)k[i].e[j];
-    });
-    float m = 0.f;
+  // a row without its mean, or as it is, to its 8-bit form
+  auto finish = [&](long long r, float(&v)[NV][V], float rstd, float* red) {
     if (a.norm) {
       Parameter<float, NT, NV, V, TAIL> gamma, beta;
       gamma.load(a.gamma, a.cols, t);
       beta.load(a.beta, a.cols, t);
-      float mean, rstd;
-      centre_row<NT, NV, V, TAIL>(v, a.cols, t, a.eps, red[turn], mean, rstd);
       each_pack<NT, NV, V>(a.cols, t, [&](int i, int) {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -261,11 +263,12 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void quantize_rows(QuantizeArg
         }
       });
     }
+    float m = 0.f;
     each_pack<NT, NV, V>(a.cols, t, [&](int i, int) {
 #pragma unroll
       for (int j = 0; j < V; ++j) m = max_nan(m, fabsf(v[i][j]));
     });
-    m = team_max<NT>(m, red_max[turn]);
+    m = team_max<NT>(m, red);
     const double inv = quantize_factor(m);
     const bool fine = quantizable(m);
     unsigned char* q = (unsigned char*)a.q + r * a.ldq;
@@ -283,7 +286,25 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void quantize_rows(QuantizeArg
           if (c + j < width) q[c + j] = k.e[j];
     }
     if (t == 0) a.scale[r] = quantize_scale(m);
+  };
+  int turn = 0;
+  const long long step = (long long)gridDim.x * TEAMS, first = (long long)blockIdx.x * TEAMS + team;
+  bool any_over = false;
+  for (long long r = first; r < a.rows; r += step, turn ^= 1) {
+    LoosePack<T, V> k[NV];
+    request_row<T, NT, NV, V>((const T*)a.x + r * a.ldx, a.cols, t, k);
+    settle_row<T, NT, NV, V, TAIL>(a.cols, t, k);
+    float v[NV][V], mean, rstd = 1.f;
+    each_pack<NT, NV, V>(a.cols, t, [&](int i, int) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[i][j] = (float)k[i].e[j];
+    });
+    if (a.norm) any_over |= centre_row<NT, NV, V, TAIL>(v, a.cols, t, a.eps, red[turn], mean, rstd);
+    finish(r, v, rstd, red_max[turn]);
   }
+  if (may_run_over<T> && any_over)
+    rows_that_ran_over<T, NT, NV, V, TAIL>((const T*)a.x, a.ldx, first, a.rows, step, a.cols, t, a.eps, red,
+                                           [&](long long row, float(&v)[NV][V], float, float rstd) { finish(row, v, rstd, red_max[0]); });
 }
 
 // ---- rows of any length: three passes by 256 threads, element by element -------------------------------------------------------
@@ -300,7 +321,7 @@ __device__ __forceinline__ void row_statistics(const T* x, int cols, float eps, 
     s[0] += (double)u * u;
   }
   team_sum<kRowThreads>(s, red + kRowThreads / 64);
-  rstd = 1.f / sqrtf((float)(s[0] / cols) + eps);
+  rstd = row_rstd(s[0] / cols, eps);
 }
 
 template <typename T, typename W>
@@ -480,16 +501,6 @@ void launch_layer_norm_backward(const LayerNormGradArgs& given, int type, int wt
 // (from <k, P t> = C r (q - W b) and dr = -r^2 mean(xh dx), d xh = P dx).
 // f32 rows without gaps, in registers like the others; gamma and beta are there.
 template <int NT, int NV, int V, bool TAIL>
-__device__ __forceinline__ void load_row(const float* p, int cols, int t, float (&v)[NV][V]) {
-  LoosePack<float, V> k[NV];
-  request_row<float, NT, NV, V>(p, cols, t, k);
-  settle_row<float, NT, NV, V, TAIL>(cols, t, k);
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[i][j] = (i * NT + t) * V < cols ? k[i].e[j] : 0.f;
-}
-template <int NT, int NV, int V, bool TAIL>
 __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_tangent(LayerNormTangentArgs a) {
   constexpr int NB = NT > 256 ? NT : 256, TEAMS = NB / NT;
   __shared__ float red[2][NT > 64 ? 2 * NT / 64 : 1];
@@ -499,10 +510,10 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_tangent(LayerNormTange
   for (long long r = (long long)blockIdx.x * TEAMS + team; r < a.rows; r += (long long)gridDim.x * TEAMS, turn ^= 1) {
     const size_t o = (size_t)r * a.cols;
     float x[NV][V], v[NV][V], g[NV][V], b[NV][V];
-    load_row<NT, NV, V, TAIL>(a.x + o, a.cols, t, x);
-    load_row<NT, NV, V, TAIL>(a.tx + o, a.cols, t, v);
-    load_row<NT, NV, V, TAIL>(a.gamma, a.cols, t, g);
-    load_row<NT, NV, V, TAIL>(a.beta, a.cols, t, b);
+    load_row<float, NT, NV, V, TAIL>(a.x + o, a.cols, t, x);
+    load_row<float, NT, NV, V, TAIL>(a.tx + o, a.cols, t, v);
+    load_row<float, NT, NV, V, TAIL>(a.gamma, a.cols, t, g);
+    load_row<float, NT, NV, V, TAIL>(a.beta, a.cols, t, b);
     const float mean = a.mean[r], rstd = a.rstd[r];
     float s[2] = {0.f, 0.f};
 #pragma unroll
@@ -538,11 +549,11 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_tangent_bwd(LayerNormT
   for (long long r = (long long)blockIdx.x * TEAMS + team; r < a.rows; r += (long long)gridDim.x * TEAMS, turn ^= 1) {
     const size_t o = (size_t)r * a.cols;
     float x[NV][V], v[NV][V], k[NV][V], g[NV][V], b[NV][V];
-    load_row<NT, NV, V, TAIL>(a.x + o, a.cols, t, x);
-    load_row<NT, NV, V, TAIL>(a.tx + o, a.cols, t, v);
-    load_row<NT, NV, V, TAIL>(a.dty + o, a.cols, t, k);
-    load_row<NT, NV, V, TAIL>(a.gamma, a.cols, t, g);
-    load_row<NT, NV, V, TAIL>(a.beta, a.cols, t, b);
+    load_row<float, NT, NV, V, TAIL>(a.x + o, a.cols, t, x);
+    load_row<float, NT, NV, V, TAIL>(a.tx + o, a.cols, t, v);
+    load_row<float, NT, NV, V, TAIL>(a.dty + o, a.cols, t, k);
+    load_row<float, NT, NV, V, TAIL>(a.gamma, a.cols, t, g);
+    load_row<float, NT, NV, V, TAIL>(a.beta, a.cols, t, b);
     const float mean = a.mean[r], rstd = a.rstd[r];
     float s[5] = {0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll

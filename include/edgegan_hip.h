@@ -235,7 +235,8 @@ unsigned int eg_crc32c(unsigned int crc, const void* data, unsigned long long n)
 enum { EG_F32 = 0, EG_BF16 = 1, EG_F16 = 2 };                       /* element types */
 enum { EG_ACT_NONE = 0, EG_ACT_RELU = 1, EG_ACT_LRELU = 2 };        /* LeakyReLU's slope is 0.2, as the discriminators' */
 
-/* y = act((x - mean) rstd gamma + beta) for each row; rstd = (var + eps)^-1/2, var biased.  gamma / beta [cols] of type wtype, or
+/* y = act((x - mean) rstd gamma + beta) for each row; rstd = (var + eps)^-1/2, var biased.  Rows of any finite
+ * values whose differences from their mean are finite in f32; x - mean takes the mean as it is stored, rounded to f32.  gamma / beta [cols] of type wtype, or
  * NULL; mean / rstd [rows] (what the gradient needs), or NULL. */
 int eg_layer_norm(int device, void* stream, int dtype, const void* x, long long ldx, int wtype, const void* gamma, const void* beta,
                   long long rows, long long cols, float eps, int act, void* y, long long ldy, float* mean, float* rstd);

@@ -57,3 +57,78 @@ def test_gradient_of_activations_at_zero(ops, rows, cols, act, dtype):
         assert (y[:3] == 0).all()
     if act == 'relu':
         assert (dx[:3] == 0).all()
+
+
+def check_statistics(ops, x, w, b, eps=1e-5, act=None):
+    """y and the statistics against 64 bits.  A rstd below the normal numbers is a multiple of 2^-149: off by half of one, which y sees relative to rstd."""
+    y, mean, rstd = ops.layer_norm(x.cuda(), w.cuda(), b.cuda(), eps=eps, act=act, statistics=True)
+    m64, r64, xh, z = R.norm64(x, w, b, eps)
+    low = 2.0 ** -150 / r64
+    ex = R.xhat_error(x, m64, r64) + xh.abs() * low[:, None]
+    near(mean.cpu(), m64, 2 * U * m64.abs() + ex.amax(1) / r64, 'mean')
+    near(rstd.cpu(), r64, r64 * (R.chain(x.shape[1]) + 8 * U + 2 * ex.amax(1) ** 2 + low), 'rstd')
+    want = torch.where(z > 0, z, R.ACT_SLOPE[act] * z)
+    ez = ex * w.double().abs() + 3 * U * (z.abs() + b.double().abs() + (xh * w.double()).abs())
+    near(y.cpu(), want, ez * (1 + half(x.dtype)) + half(x.dtype) * want.abs() + tiny(x.dtype), 'y')
+    return z, ez
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+@pytest.mark.parametrize('cols', [2, 3, 17, 40, 128, 1000, 1024, 3001, 5000, 9000, 17000, 40001])
+def test_layer_norm_of_large_values(ops, cols, dtype):
+    """Rows of the type's lowest and highest value, masked in parts by the lowest one, and of numbers whose squares 32 bits do not hold: the
+    statistics are those of the definition, alone and in front of the quantisation."""
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    big = [1.0, 1e15, 1e19, 3e19, 1e25, 1e37] if dtype != F16 else [1.0, 1e3, 1e4]
+    rows = [torch.full((cols,), low), torch.full((cols,), high)]
+    for i, s in enumerate(big):
+        rows.append((rnd(cols, seed=i).clamp(-4, 4) * s))
+    masked = rnd(cols, seed=20)
+    masked[cols // 2:] = low
+    rows.append(masked)
+    masked = rnd(cols, seed=21)
+    masked[-1] = low
+    rows.append(masked)
+    rows.append(rnd(cols, seed=22))          # an ordinary row between them
+    x = torch.stack(rows).to(dtype)
+    w, b = rnd(cols, seed=30, scale=0.2, shift=1.0), rnd(cols, seed=31, scale=0.2)
+    z, ez = check_statistics(ops, x, w, b, act='lrelu')
+    z, ez = check_statistics(ops, x, w, b)
+    how = (w.cuda(), b.cuda(), 1e-5)
+    q, s = ops.quantize_rows(x.cuda(), norm=how)
+    amax = z.abs().amax(1)
+    near(s.cpu(), amax / 127, ez.amax(1) / 127 + U * amax / 127, 'scale')
+    off = (q.cpu().double() - 127 * z / amax[:, None]).abs()
+    assert (off <= 0.5 + 127 * (ez + ez.amax(1, keepdim=True)) / amax[:, None] + 1e-9).all()
+    # few rows and short ones in one launch are the two calls
+    qw, sw = ops.quantize_rows(rnd(33, cols, seed=32).cuda())
+    for part in (x[:1], x[2:6], x, x[[-1, 0]], x[[0, -1]], x[[-1, -1, 0, -1]], x[[0, -1, -1, -1]], x[[-1, 6, 1]]):
+        got = ops.int8_linear(part.cuda(), qw, sw, norm=how)
+        assert torch.equal(got, ops.int8_matmul(*ops.quantize_rows(part.cuda(), norm=how), qw, sw, out_dtype=dtype))
+    # a row's neighbours do not matter
+    y = ops.layer_norm(x.cuda(), w.cuda(), b.cuda())
+    for r in range(len(rows)):
+        assert torch.equal(ops.layer_norm(x[r:r + 1].cuda(), w.cuda(), b.cuda())[0], y[r]), r
+    # many of them in the hands of each team, in place
+    many, wd, bd = x.repeat(900, 1).cuda(), w.cuda(), b.cuda()
+    assert ops._library().eg_layer_norm(0, stream(), R_TYPES[dtype], many.data_ptr(), cols, 0, wd.data_ptr(), bd.data_ptr(), len(many), cols, 1e-5, 0, many.data_ptr(), cols, None,
+                                        None) == 0
+    assert torch.equal(many, y.repeat(900, 1))
+
+
+@pytest.mark.parametrize('dtype', [F32, BF16], ids=str)
+@pytest.mark.parametrize('rows,cols', [(6, 40), (300, 100), (5, 1001), (3, 9000), (3, 20003)])
+def test_gradient_of_large_values(ops, rows, cols, dtype):
+    """The gradient at rows of size 10^25 (rstd is a normal number and dx of size 10^-25)."""
+    x = (rnd(rows, cols, seed=1, scale=1e25)).to(dtype)
+    R.check_norm(ops, x, rnd(rows, cols, seed=2, dtype=dtype), rnd(cols, seed=3, shift=1.0, scale=0.2), rnd(cols, seed=4, scale=0.2), 1e-5, 'lrelu')
+
+
+@pytest.mark.parametrize('cols', [*range(1, 40), 127, 250, 1001, 1002, 1003, 1023, 3001, 5001, 5002, 5003, 8191, 16383, 20001])
+def test_rows_of_one_value(ops, cols):
+    """xh is exactly 0, whatever the value and the length: y is the shift."""
+    for dtype in TYPES:
+        x = torch.tensor([0.1, 1000.1, -3.3e-7, 65503.0, 1 / 3, -0.7, 2.0 ** -14 * 1.1], dtype=dtype)[:, None].expand(7, cols).contiguous()
+        b = rnd(cols, seed=1, dtype=dtype).cuda()
+        y, mean, _ = ops.layer_norm(x.cuda(), None, b, statistics=True)
+        assert torch.equal(mean.cpu(), x[:, 0].float()) and torch.equal(y, b.expand(7, cols)), dtype
