@@ -299,7 +299,7 @@ int eg_set_teacher(eg_ctx* ctx, const int* index, const float* logits, int top, 
   EG_CHECK(c.cfg.multiclasses(), "eg_set_teacher: there is no classifier without classes");
   EG_CHECK(top >= 0 && top <= 1024, "eg_set_teacher: top = %d (0 .. 1024)", top);
   EG_CHECK(top == 0 || (index && logits), "eg_set_teacher: null argument");
-  EG_CHECK(top == 0 || (temperature > 0.f && std::isfinite(temperature) && std::isfinite(1.f / temperature) && std::isfinite(weight)),
+  EG_CHECK(top == 0 || (distill_temperature(temperature) && std::isfinite(weight)),
            "eg_set_teacher: temperature %g, weight %g", temperature, weight);
   EG_HIP(hipDeviceSynchronize());   // (a classifier sub-step in flight on another lane may read the old ones)
   c.teacher_top = 0;

@@ -11,6 +11,7 @@
 // behind the store of the row by the threads that hold the teacher's entries, in the same block.  exp((z - m) / T) is 2^((z - m) c): the difference
 // first, so that rows of the type's lowest value stay finite.
 // Measured: 4,096 x 65,536 bf16 218 - 224 us (4.9 TB/s; a copy of 1 GB 4.8 - 5.3), 511 x 10,007 f16 12.5 us, 64 x 14 f32 4.7 us.
+#include <cmath>
 #include <tuple>
 
 #include "rowops_dev.h"
@@ -227,7 +228,7 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void distill_rows(DistillArgs 
   }
   const float log_sum = logf(s[0]);
   const float loss = teacher_loss<NT>(a, t, kept, red[2], it, log_norm, m, log_sum);
-  if (t == 0) a.loss[r] = f * a.temperature * loss;
+  if (t == 0) a.loss[r] = f * (a.temperature * loss);   // (T^2 may leave f32's range where T^2 KL does not)
   team_sync<NT>();
   if (g) write_named<T, NT>(a, g, t, kept, f, [&](float x) { return it * (x - m) - log_sum; }, 0, a.cols);
 }
@@ -318,7 +319,7 @@ __global__ __launch_bounds__(kChunkThreads) void distill_chunk_grad(DistillArgs 
     team_sum<kChunkThreads>(s, red[1]);
     const float log_sum = logf(s[0]);
     const float loss = teacher_loss<kChunkThreads>(a, t, kept, red[2], it, log_norm, m, log_sum);
-    if (t == 0 && chunk == 0) a.loss[r] = w * a.temperature * a.temperature * loss;
+    if (t == 0 && chunk == 0) a.loss[r] = w * a.temperature * (a.temperature * loss);
     if (g) {
       const float f = w * a.temperature, fi = f / s[0];
       walk<V>(lo, hi, [&](int at, auto n) {
@@ -338,6 +339,9 @@ __global__ __launch_bounds__(kChunkThreads) void distill_chunk_grad(DistillArgs 
 // A row a team while its registers hold the row, else chunks; chunks also for rows that fill those registers where they are few. us, team / chunks, bf16:
 //   32,768 columns: 9.2 / 10.7 for one row, 10.1 / 11.8 for 64, 13.3 / 18.0 for 256;  65,536: 12.6 / 10.9, 14.0 / 13.3, 20.0 / 29.5 (128 rows: 16.3 / 17.4)
 static bool distill_in_chunks(long long rows, int cols) { return cols > 65536 || (cols > 32768 && rows <= 64); }
+
+// (the kernels scale by its reciprocal and by log2 e times that)
+bool distill_temperature(float t) { return t > 0.f && std::isfinite(t) && std::isfinite(1.f / t * kLog2e); }
 
 size_t distill_partial_floats(long long rows, int cols, int top) {
   return distill_in_chunks(rows, cols) ? (size_t)rows * (2 * chunks_of(cols) + top) : 0;

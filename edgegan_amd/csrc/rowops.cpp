@@ -225,7 +225,7 @@ int eg_distill_loss(int device, void* stream, int dtype, const void* logits, lon
     EG_CHECK(top >= 0 && top <= 1024, "eg_distill_loss: %lld teacher logits a row (0 .. 1024)", top);
     check_matrix("eg_distill_loss index", index, ld_index, rows, top, index_bytes);
     check_matrix("eg_distill_loss teacher", teacher, ld_teacher, rows, top, 4);
-    EG_CHECK(temperature > 0.f && std::isfinite(temperature) && std::isfinite(1.f / temperature), "eg_distill_loss: the temperature must be positive and finite");
+    EG_CHECK(distill_temperature(temperature), "eg_distill_loss: the temperature must be positive and finite, and log2(e) / temperature finite");
     if (rows == 0) return;
     EG_CHECK(loss, "eg_distill_loss: null loss");
     check_floats("eg_distill_loss", {row_weight, loss});

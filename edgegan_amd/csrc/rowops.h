@@ -109,6 +109,7 @@ void launch_int8_matmul(const Int8Args& a, int out_type, hipStream_t s);
 size_t int8_linear_bytes(long long m, int k);
 bool int8_linear_in_one(const QuantizeArgs& q, const Int8Args& a, int type, int out_type);   // one launch, which needs no workspace
 void launch_int8_linear(const QuantizeArgs& q, const Int8Args& a, int type, int out_type, void* workspace, hipStream_t s);
+bool distill_temperature(float t);   // one that the kernels take
 size_t distill_partial_floats(long long rows, int cols, int top);
 void launch_distill(const DistillArgs& a, int type, hipStream_t s);
 // grad[i] += more[i] (n values), *total = the sum of loss[0 .. rows)

@@ -273,7 +273,8 @@ int eg_int8_linear(int device, void* stream, int dtype, const void* x, long long
 /* Distillation from a teacher's top logits: p = softmax(teacher / T) over the `top` (<= 1024) kept logits of a row, q = softmax(logits / T);
  * loss[r] = w_r T^2 sum_k p_k (log p_k - log q_index[k]); grad (or NULL) = d(sum of loss) / d(logits).  index: 4- or 8-byte integers;
  * one outside [0, cols) is padding, one given twice counts twice.  row_weight f32 [rows] or NULL (1): a row of weight 0 or without a kept
- * logit has loss 0 and gradient 0 whatever its logits hold. */
+ * logit has loss 0 and gradient 0 whatever its logits hold.  T from 5e-39 to the largest f32; the logarithms are formed in f32, so the loss is off by some
+ * w T^2 2^-22 (1 + |log q|) besides its own rounding: with T far above the logits' spread and every class kept that is all of it. */
 long long eg_distill_loss_workspace(long long rows, long long cols, long long top);
 int eg_distill_loss(int device, void* stream, int dtype, const void* logits, long long ld, int index_bytes, const void* index,
                     long long ld_index, const float* teacher, long long ld_teacher, const float* row_weight, long long rows,

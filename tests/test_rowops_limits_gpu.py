@@ -132,3 +132,36 @@ def test_rows_of_one_value(ops, cols):
         b = rnd(cols, seed=1, dtype=dtype).cuda()
         y, mean, _ = ops.layer_norm(x.cuda(), None, b, statistics=True)
         assert torch.equal(mean.cpu(), x[:, 0].float()) and torch.equal(y, b.expand(7, cols)), dtype
+
+
+@pytest.mark.parametrize('cols', [14, 300, 5000, 40000, 70001])
+@pytest.mark.parametrize('t', [1e-25, 1e-12, 1e-3])
+def test_distill_at_small_temperatures(ops, t, cols):
+    """T^2 may be below every 32-bit number where T^2 KL is not: both distributions are one class, and the loss is T times the student's distance to it."""
+    rows = 5
+    z = rnd(rows, cols, seed=cols, scale=2.0)
+    z[:, 3] = 20.0                                   # the student's choice, ahead by more than 1e-3 of anything
+    idx, u = torch.tensor([[0, 1, 2, 3, 4]] * rows), rnd(rows, 5, seed=2)
+    u[:, 1] = 9.0                                    # the teacher's
+    loss, grad = ops.distill_loss(z.cuda(), idx.cuda(), u.cuda(), temperature=t)
+    want = t * (z[:, 3] - z[:, 1]).double()
+    near(loss.cpu(), want, 16 * U * want, 'loss')    # (a difference, 1 / T, three products)
+    g = torch.zeros(rows, cols, dtype=torch.float64)
+    g[:, 3], g[:, 1] = t, -t
+    near(grad.cpu(), g, 4 * U * g.abs(), 'grad')
+
+
+@pytest.mark.parametrize('cols', [14, 300, 5000, 40000, 70001])
+@pytest.mark.parametrize('t', [1e12, 1e18, 1e25])
+def test_distill_at_large_temperatures(ops, t, cols):
+    """Both distributions are even: T^2 log(classes / kept) where f32 holds it, infinity where not, and a gradient of size T."""
+    z, idx, u = rnd(3, cols, seed=cols), torch.tensor([[0, 3], [5, 1], [2, 13]]), rnd(3, 2, seed=2)
+    loss, grad = ops.distill_loss(z.cuda(), idx.cuda(), u.cuda(), temperature=t)
+    want = torch.full((3,), t * t * math.log(cols / 2), dtype=torch.float64)
+    if t < 1e19:   # the log-sums of `cols` and two exponentials, each off by a sum and a rounding; three products
+        near(loss.cpu(), want, t * t * (R.chain(cols) + 40 * U + 4 * U * math.log(cols)) + 4 * U * want, 'loss')
+    else:
+        assert (loss == math.inf).all()
+    g = torch.full((3, cols), t / cols, dtype=torch.float64)
+    g.scatter_add_(1, idx, torch.full((3, 2), -t / 2, dtype=torch.float64))
+    near(grad.cpu(), g, t * (R.chain(cols) + 40 * U) * (1 / cols + 0.5 * (g < 0)) + 4 * U * g.abs(), 'grad')
