@@ -165,7 +165,9 @@ class EdgeGAN:
         if index is None:
             self._check(self._lib.eg_set_teacher(self._ctx, None, None, 0, 1.0, 0.0))
             return
-        index, logits = np.ascontiguousarray(index, dtype=np.int32), np.ascontiguousarray(logits, dtype=np.float32)
+        index = np.asarray(index)
+        index = np.ascontiguousarray(np.where((index >= 0) & (index < self.config.num_classes), index, -1), dtype=np.int32)   # (one past 32 bits must not wrap into a class)
+        logits = np.ascontiguousarray(logits, dtype=np.float32)
         if index.ndim != 2 or index.shape != logits.shape or index.shape[0] != self.config.batch_size:
             raise EdgeGANLibError(f'set_teacher: index and logits [{self.config.batch_size}, top], not {index.shape} and {logits.shape}')
         self._check(self._lib.eg_set_teacher(self._ctx, iptr(index), fptr(logits), index.shape[1], temperature, weight))

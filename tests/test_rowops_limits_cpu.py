@@ -1,4 +1,7 @@
 """Refusals and sizes of the row operators at the limits of what they take, on the host (the ordinary ones: test_rowops_cpu)."""
+import numpy as np
+import pytest
+
 import test_rowops_cpu as R
 
 
@@ -7,3 +10,27 @@ def test_temperatures_whose_scale_is_infinite_are_refused(built_lib):
     for t in (3e-39, 4.2e-39, 1e-45):
         assert R.distill(built_lib, t=t) == 1 and 'temperature' in built_lib.eg_last_error(None).decode(), t
     assert R.distill(built_lib, rows=0, t=5e-39) == 0 and R.distill(built_lib, rows=0, t=3e38) == 0
+
+
+@pytest.mark.parametrize('dtype', [np.int32, np.int64, np.uint32, np.uint64, np.float32])
+def test_teacher_indexes_of_any_width(dtype):
+    """An index outside the classes is padding whatever integer type holds it: 2^32 + 3 is not class 3."""
+    import edgegan_amd as ea
+
+    class Lib:
+        def eg_set_teacher(self, ctx, index, logits, top, temperature, weight):
+            self.index = [index[i] for i in range(2 * top)]
+            return 0
+    net = ea.EdgeGAN.__new__(ea.EdgeGAN)
+    net.config, net._ctx, net._lib = ea.Config(batch_size=2), None, Lib()
+    rows = [[0, 13, 14, 2 ** 31 - 1], [3, 100, 5, 1]] if dtype in (np.int32, np.float32) else [[0, 13, 14, 2 ** 32 - 1], [3, 100, 5, 1]]
+    index = np.array(rows, dtype=dtype)
+    want = [0, 13, None, None, 3, None, 5, 1]
+    if dtype in (np.int64, np.uint64):
+        index[0, 2], index[1, 1] = 2 ** 32 + 3, 2 ** 40 + 13
+    if dtype in (np.int32, np.int64):
+        index[1, 3], want[7] = -2, None
+    net.set_teacher(index, np.zeros((2, 4), np.float32))
+    got = net._lib.index
+    net._ctx = None
+    assert [i if 0 <= i < 14 else None for i in got] == want
