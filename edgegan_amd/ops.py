@@ -5,7 +5,8 @@ They are for training and inference code beside the engine (a head behind the en
 from); the engine runs the same kernels where ``E_norm`` / ``G_norm`` / ``D_norm`` is 'layernorm', in ``EdgeGAN.set_teacher`` and in 8-bit inference.
 A call works on the current stream of its tensors' device, allocates its results there with torch, waits for nothing, and may be
 captured into a graph.  The last dimension is the row; the dimensions before it have to be one stride apart as if they were a single one (a slice of columns is fine, a transposed
-view is not).  Every refusal raises EdgeGANLibError.  There is no autograd: the gradient calls are explicit, as everywhere in this package."""
+view is not).  Every refusal raises EdgeGANLibError.  There is no autograd: results have no gradient history, whatever their inputs require, and the gradient calls are
+explicit, as everywhere in this package.  A gradient that torch has expanded (of a sum: stride 0) has to be made contiguous first."""
 from __future__ import annotations
 
 import math
@@ -41,6 +42,12 @@ def _refuse(what: str):
     raise EdgeGANLibError(what)
 
 
+def _refuse_negated(x: torch.Tensor, name: str):
+    """A view that torch negates when it is read: the imaginary part of a conjugate (never consecutive with more than one element)."""
+    if x.is_neg():
+        _refuse(f'{name}: a view that torch negates when it is read (resolve_neg makes a tensor of it)')
+
+
 def _rows(x: torch.Tensor, name: str, types=_TYPES) -> Tuple[int, int, int]:
     """(rows, cols, elements between rows) of a GPU tensor of one of `types`."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
@@ -52,7 +59,13 @@ def _rows(x: torch.Tensor, name: str, types=_TYPES) -> Tuple[int, int, int]:
     if n == 0:
         _refuse(f'{name}: at least one dimension is required')
     cols = shape[-1]
-    if x.is_contiguous():
+    try:
+        consecutive = x.is_contiguous()
+    except RuntimeError:
+        _refuse(f'{name}: a strided tensor is required, not {x.layout}')
+    if cols == 1 or not consecutive:
+        _refuse_negated(x, name)
+    if consecutive:
         return (shape[0] if n == 2 else 1 if n == 1 else math.prod(shape[:-1])), cols, cols
     stride = x.stride()
     if cols > 1 and stride[-1] != 1:
@@ -79,7 +92,13 @@ def _vector(v: Optional[torch.Tensor], n: int, name: str, device: int, dtype: to
         _refuse(f'{name}: a tensor on GPU {device} is required')
     if v.dtype != dtype:
         _refuse(f'{name}: {dtype} is required, not {v.dtype}')
-    if v.numel() != n or not v.is_contiguous():
+    if n == 1:
+        _refuse_negated(v, name)
+    try:
+        consecutive = v.is_contiguous()
+    except RuntimeError:
+        _refuse(f'{name}: a strided tensor is required, not {v.layout}')
+    if v.numel() != n or not consecutive:
         _refuse(f'{name}: {n} consecutive elements are required, not {tuple(v.shape)} with strides {tuple(v.stride())}')
     return v.data_ptr()
 
@@ -108,7 +127,10 @@ def _number(v, name: str) -> float:
     if type(v) is float:
         return v
     if isinstance(v, (int, float)):
-        return float(v)
+        try:
+            return float(v)
+        except OverflowError:
+            _refuse(f'{name}: a number that a float holds is required')
     _refuse(f'{name}: a number is required, not {type(v).__name__}')
 
 

@@ -34,3 +34,11 @@ def test_teacher_indexes_of_any_width(dtype):
     got = net._lib.index
     net._ctx = None
     assert [i if 0 <= i < 14 else None for i in got] == want
+
+
+def test_numbers_past_every_float_are_refused():
+    from edgegan_amd import EdgeGANLibError, ops
+    assert ops._number(3, 'eps') == 3.0 and ops._number(np.float64(2.5), 'eps') == 2.5
+    for bad in (10 ** 400, -10 ** 4400, '1', None, np.zeros(1)):
+        with pytest.raises(EdgeGANLibError):
+            ops._number(bad, 'eps')

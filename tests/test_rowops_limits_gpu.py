@@ -165,3 +165,20 @@ def test_distill_at_large_temperatures(ops, t, cols):
     g = torch.full((3, cols), t / cols, dtype=torch.float64)
     g.scatter_add_(1, idx, torch.full((3, 2), -t / 2, dtype=torch.float64))
     near(grad.cpu(), g, t * (R.chain(cols) + 40 * U) * (1 / cols + 0.5 * (g < 0)) + 4 * U * g.abs(), 'grad')
+
+
+def test_tensors_without_plain_memory_are_refused(ops):
+    """Sparse tensors, and tensors whose sign torch applies when they are read."""
+    from edgegan_amd import EdgeGANLibError
+    x = torch.randn(4, 32, device='cuda')
+    column = torch.randn(4, 1, dtype=torch.complex64, device='cuda').conj().imag     # the values of minus its memory
+    one = torch.randn(1, dtype=torch.complex64, device='cuda').conj().imag
+    assert column.is_neg() and one.is_neg()
+    v = torch.ones(32, device='cuda')
+    for f in (lambda: ops.layer_norm(x.to_sparse()), lambda: ops.layer_norm(x.to_sparse_csr()), lambda: ops.layer_norm(column), lambda: ops.layer_norm(one),
+              lambda: ops.layer_norm(x, v.to_sparse()), lambda: ops.layer_norm(column.clone(), one), lambda: ops.layer_norm(x, eps=10 ** 400),
+              lambda: ops.quantize_rows(column), lambda: ops.distill_loss(column, torch.zeros(4, 1, dtype=torch.int64, device='cuda'), torch.zeros(4, 1, device='cuda')),
+              lambda: ops.distill_loss(x, torch.zeros(4, 1, dtype=torch.int64, device='cuda'), column)):
+        with pytest.raises(EdgeGANLibError):
+            f()
+    assert ops.layer_norm(column.resolve_neg()).shape == (4, 1)
