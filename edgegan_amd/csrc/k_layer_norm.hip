@@ -382,7 +382,7 @@ __global__ __launch_bounds__(kRowThreads) void ln_bwd_rows(LayerNormGradArgs a) 
   }
 }
 
-// The parameter gradients: a block takes 64 columns and every kPartRows-th group of rows; four row lanes a block.
+// The parameter gradients: a block takes 64 columns and a share of the rows, four of them at a time.
 constexpr int kPartBlocks = 64;   // row groups
 template <typename T, typename W>
 __global__ __launch_bounds__(256) void ln_bwd_columns(LayerNormGradArgs a) {
@@ -437,7 +437,22 @@ static dim3 team_block(int nt) { return dim3(nt > 256 ? nt : 256); }
 // Blocks of the gradient: each leaves one row of partial parameter gradients.  With a row ahead in flight, 16,384 x 4,096 bf16 (a row a block): 512
 // blocks 80 + 5 us (gradient + join), 256 83 + 5, 1,024 98 + 7; 65,536 x 128 f32 (8 rows a block): 1,024 blocks 19 + 5 us, 512 22 + 4, 256 31 + 4.
 constexpr int kGradBlocks = 1024;   // half of them where the block is one row's team
-size_t layer_norm_partial_floats(long long rows, int cols) { return (size_t)std::min<long long>(kGradBlocks, rows) * 2 * cols; }
+static dim3 gradient_grid(long long rows, int nt) { return team_grid(rows, nt, nt > 64 ? kGradBlocks / 2 : kGradBlocks); }
+// f(team) for the gradient's form of rows of type T in registers
+template <typename T, typename F>
+static bool gradient_team(int cols, F f) { return row_team<T, 16, sizeof(T) == 2 ? 32 : 16>(cols, f); }
+// Blocks that leave a row of partial sums
+template <typename T>
+static int gradient_groups(long long rows, int cols) {
+  int groups = 0;
+  if (!gradient_team<T>(cols, [&](auto nt, auto, auto, auto) { groups = (int)gradient_grid(rows, nt).x; })) groups = part_groups(rows);
+  return groups;
+}
+// (enough for rows of any type)
+size_t layer_norm_partial_floats(long long rows, int cols) {
+  if (rows == 0 || cols == 0) return 0;
+  return (size_t)std::max(gradient_groups<float>(rows, cols), gradient_groups<bf16_t>(rows, cols)) * 2 * cols;
+}
 
 // Few rows by one block, which then has the whole sums: no second launch, no workspace. 4 rows for each of its teams (as many teams as f32 rows have), 2 where
 // the block is one team.  us of a call / of its kernels, against two launches: 16 x 1000 bf16 11.6 / 6.7 (15.7 / 6.0), 32 x 128 11.3 / 5.1 (15.6 / 6.5), 2 x 4096 11.1 / 9.0
@@ -473,16 +488,13 @@ void launch_layer_norm_backward(const LayerNormGradArgs& given, int type, int wt
       using W = decltype(w);
       int groups = 0;
       if (a.rows) {
-        const bool held = row_team<T, 16, sizeof(T) == 2 ? 32 : 16>(a.cols, [&](auto nt, auto nv, auto v, auto tail) {
-          const dim3 grid = team_grid(a.rows, nt, params && one ? 1 : nt > 64 ? kGradBlocks / 2 : kGradBlocks);
-          groups = (int)grid.x;
+        groups = gradient_groups<T>(a.rows, a.cols);
+        const bool held = gradient_team<T>(a.cols, [&](auto nt, auto nv, auto v, auto tail) {
+          const dim3 grid = params && one ? dim3(1) : gradient_grid(a.rows, nt);
           row_launch(ln_bwd<T, W, nt, nv, v, tail>, grid, team_block(nt), s, a);
         });
         if (!held) {
-          if (params) {   // (first: dx may be dy)
-            groups = part_groups(a.rows);
-            row_launch(ln_bwd_columns<T, W>, dim3((a.cols + 63) / 64, groups), dim3(256), s, a);
-          }
+          if (params) row_launch(ln_bwd_columns<T, W>, dim3((a.cols + 63) / 64, groups), dim3(256), s, a);   // (first: dx may be dy)
           if (a.dx) row_launch(ln_bwd_rows<T, W>, row_grid(a.rows), dim3(kRowThreads), s, a);
         }
       }
@@ -595,15 +607,15 @@ __global__ __launch_bounds__(NT > 256 ? NT : 256) void ln_tangent_bwd(LayerNormT
 
 void launch_layer_norm_tangent(const LayerNormTangentArgs& a, hipStream_t s) {
   if (!a.rows || !a.cols) return;
-  const bool held = row_team<float, 16, 16>(a.cols, [&](auto nt, auto nv, auto v, auto tail) {
+  const bool held = gradient_team<float>(a.cols, [&](auto nt, auto nv, auto v, auto tail) {
     row_launch(ln_tangent<nt, nv, v, tail>, team_grid(a.rows, nt, 8192), team_block(nt), s, a);
   });
   EG_CHECK(held, "layer norm tangent: %d channels", a.cols);
 }
 void launch_layer_norm_tangent_backward(const LayerNormTangentArgs& a, hipStream_t s) {
   if (!a.rows || !a.cols) return;
-  const bool held = row_team<float, 16, 16>(a.cols, [&](auto nt, auto nv, auto v, auto tail) {
-    const dim3 grid = team_grid(a.rows, nt, nt > 64 ? kGradBlocks / 2 : kGradBlocks);
+  const bool held = gradient_team<float>(a.cols, [&](auto nt, auto nv, auto v, auto tail) {
+    const dim3 grid = gradient_grid(a.rows, nt);
     row_launch(ln_tangent_bwd<nt, nv, v, tail>, grid, team_block(nt), s, a);
     if (a.dgamma)
       row_launch(ln_bwd_finish<float>, dim3((2 * a.cols + 31) / 32), dim3(1024), s, a.partial, (int)grid.x, a.cols, a.dgamma, (float*)nullptr, a.acc_w);

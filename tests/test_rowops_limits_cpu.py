@@ -42,3 +42,14 @@ def test_numbers_past_every_float_are_refused():
     for bad in (10 ** 400, -10 ** 4400, '1', None, np.zeros(1)):
         with pytest.raises(EdgeGANLibError):
             ops._number(bad, 'eps')
+
+
+def test_gradient_workspace_is_what_the_kernels_write(built_lib):
+    """[blocks][2][cols] of f32: 512 blocks where a row has a block or four waves, 1,024 where a wave or less, 64 groups of rows where it is too long for registers; never more
+    blocks than the rows give work to."""
+    size = built_lib.eg_layer_norm_workspace
+    for rows, cols, blocks in ((65536, 128, 1024), (16384, 4096, 512), (8192, 32768, 64), (100, 32768, 25), (300, 4096, 300), (129, 32, 5), (1 << 40, 1000, 1024), (5000, 8, 157)):
+        assert size(rows, cols) == blocks * 2 * cols * 4, (rows, cols, size(rows, cols) / (8 * cols))
+    for rows in (3, 17, 129, 700, 5000, 100000):
+        for cols in (1, 7, 8, 33, 64, 65, 128, 200, 256, 500, 1000, 1024, 1025, 2048, 3000, 4096, 8192, 8193, 12000, 16384, 16385, 70000):
+            assert 0 <= size(rows, cols) <= min(rows, 1024) * 8 * cols, (rows, cols)

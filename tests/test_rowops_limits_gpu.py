@@ -182,3 +182,22 @@ def test_tensors_without_plain_memory_are_refused(ops):
         with pytest.raises(EdgeGANLibError):
             f()
     assert ops.layer_norm(column.resolve_neg()).shape == (4, 1)
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+@pytest.mark.parametrize('rows,cols', [(129, 32), (33, 100), (700, 100), (5000, 128), (17, 1000), (600, 1000), (1100, 1024), (3, 5001), (700, 4096), (600, 8193), (3, 20003), (300, 16500), (70, 33000)])
+def test_gradient_writes_inside_its_workspace(ops, rows, cols, dtype):
+    """The workspace of eg_layer_norm_workspace's size is enough for every type, and what lies behind it stays."""
+    lib = ops._library()
+    x, dy, w = rnd(rows, cols, seed=1, dtype=dtype).cuda(), rnd(rows, cols, seed=2, dtype=dtype).cuda(), rnd(cols, seed=3, dtype=dtype).cuda()
+    _, m, r = ops.layer_norm(x, w, w, statistics=True)
+    size = lib.eg_layer_norm_workspace(rows, cols)
+    assert size > 0
+    ws = torch.full((size + (8 << 20),), 77, dtype=torch.uint8, device='cuda')   # (room for twice the blocks and more)
+    out = torch.empty(2, cols, dtype=dtype, device='cuda')
+    e = R_TYPES[dtype]
+    assert lib.eg_layer_norm_backward(0, stream(), e, dy.data_ptr(), cols, x.data_ptr(), cols, m.data_ptr(), r.data_ptr(), e, w.data_ptr(), w.data_ptr(), rows, cols, 0,
+                                      None, 0, out[0].data_ptr(), out[1].data_ptr(), ws.data_ptr(), size) == 0
+    assert (ws[size:] == 77).all()
+    _, dw, db = ops.layer_norm_backward(dy, x, m, r, w, w)
+    assert torch.equal(out[0], dw) and torch.equal(out[1], db)
