@@ -24,7 +24,8 @@ __device__ __forceinline__ i32x4 load16(const signed char* row, int k, int k_end
 // the same operations in every kernel, so that a result does not depend on the variant
 __device__ __forceinline__ float int8_result(int sum, float sa, float sb, float bias) { return rounded_mul(rounded_mul((float)sum, sa), sb) + bias; }
 
-// Any sizes, strides and alignment: 64 x 64 outputs a block, a wave 32 x 32 of them, operands straight from memory.
+// Any sizes, strides and alignment: 64 x 64 outputs a block, a wave 32 x 32 of them, operands straight from memory, byte by byte where they are not aligned: 23 x 8190 x 2050 204 us
+// (rows at a pitch of 16 bytes take the tiles below: 6.4), 1024 x 1024 x 1001 95.
 template <typename T>
 __global__ __launch_bounds__(256) void int8_any(Int8Args a, int tiles_n, int aligned_a, int aligned_b) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;

@@ -13,8 +13,9 @@
 // last pack of three is off by less than what rounding the mean of seven or more takes back).  Where a pack's sum runs over in 32 bits, the row is
 // summed again in 64 (rows_that_ran_over).  The gradient's sums are in 32.  xh gamma + beta is formed by the same three rounded operations in the forward and the gradient (no
 // contraction into an fma), so the gradient's sign of it is the forward's.
-// Measured: forward 65,536 x 128 f32 12.8 us (5.2 TB/s; a copy of these bytes 6.5), 8,192 x 4,096 bf16 26 us; gradient 16,384 x 4,096 bf16 80 + 5 us
-// (4.7 TB/s with three tensors); quantisation 8,192 x 4,096 bf16 24 - 27 us (3.9 TB/s).
+// Measured: forward 65,536 x 128 f32 12.9 - 15.1 us (up to 5.2 TB/s; a copy of these bytes 6.5), 8,192 x 4,096 bf16 25 us; gradient 16,384 x 4,096 bf16 79 + 5 us
+// (4.8 TB/s with three tensors); quantisation 8,192 x 4,096 bf16 24 - 27 us (3.9 TB/s).  Rows that do not end with a pack: 1,023 x 5,001 f16 12.2 us, 5,000 8.6 (the cut
+// pack's shift takes registers, 208 a thread, and its tail goes element by element).
 #include <tuple>
 
 #include "rowops_dev.h"
@@ -412,7 +413,8 @@ static int part_groups(long long rows) { return (int)std::min<long long>(kPartBl
 // most 16 / 32 elements a thread, rows x columns: forward bf16 8192 x 2048 (256 threads or a wave) 21.4 / 16.6, 4096 x 8192 (1,024 or 256) 55 / 30.4, f32 4096 x 6000
 // 45 / 34.6, but 64 x 6000 4.0 / 4.6; quantisation of the same 16.0 / 12.8, 40.8 / 21.7, 37 / 28.7, 3.6 / 4.2.  Gradient: bf16 8192 x 2048 29.2 / 35.7, so 16 in a wave;
 // 4096 x 8192 124 / 59.5, so 32 in a block of 256; f32 4096 x 6000 64.0 / 64.6, 64 x 6000 10.4 / 11.0, so 16 there.  With at most 8, bf16 8192 x 4096
-// takes 97 (forward) and 148 (gradient), against 26 and 45.
+// takes 97 (forward) and 148 (gradient), against 26 and 45.  The gradient spills with 1,024 threads (40 to 100 registers a thread, in every type; its tangent's reverse 63
+// to 71): bf16 2,048 x 10,000 72 us, 2,048 x 16,384 104, for 123 and 201 MB.  512 threads lie between and have not been tried.
 template <typename T, int WAVE, int BLOCK, typename F>
 static bool row_team(int cols, F f) {
   constexpr int V = 16 / sizeof(T);

@@ -243,7 +243,8 @@ int eg_layer_norm(int device, void* stream, int dtype, const void* x, long long 
 /* The gradient: dx [rows x cols], dgamma and dbeta [cols] (type wtype); each may be NULL.  beta matters only to an activation's sign.
  * Where the pre-activation is exactly 0 (a row of one value with no shift or one of 0), LeakyReLU's derivative is its slope 0.2 and ReLU's 0; the engine's own
  * block norms take 1 for LeakyReLU there, as the gradient of max(z, 0.2 z).
- * The workspace (bytes: eg_layer_norm_workspace, 0 for few rows, -1 for bad sizes) is needed for dgamma / dbeta. */
+ * The workspace (bytes: eg_layer_norm_workspace, 0 for few rows, -1 for bad sizes) is needed for dgamma / dbeta; one that is given has to hold what the form for
+ * more rows would need. */
 long long eg_layer_norm_workspace(long long rows, long long cols);
 int eg_layer_norm_backward(int device, void* stream, int dtype, const void* dy, long long lddy, const void* x, long long ldx,
                            const float* mean, const float* rstd, int wtype, const void* gamma, const void* beta, long long rows,
@@ -256,7 +257,7 @@ int eg_layer_norm_backward(int device, void* stream, int dtype, const void* dy, 
 int eg_quantize_rows(int device, void* stream, int dtype, const void* x, long long ldx, int norm, const float* gamma, const float* beta,
                      float eps, long long rows, long long cols, signed char* q, long long ldq, float* scale);
 /* out[i][j] = (sum_k a[i][k] b[j][k]) a_scale[i] b_scale[j] + bias[j]: a [m x k] a scale for each row (token, position), b [n x k] one for
- * each output channel; 32-bit integer sums (k <= 131071).  bias f32 or NULL.  Where rows begin at multiples of 16 bytes, the
+ * each output channel; 32-bit integer sums (k <= 131071), the rest in f32 in this order.  bias f32 or NULL.  Where rows begin at multiples of 16 bytes, the
  * 16-byte group that k ends in is read whole (and what lies past k there ignored). */
 int eg_int8_matmul(int device, void* stream, const signed char* a, long long lda, const float* a_scale, const signed char* b,
                    long long ldb, const float* b_scale, const float* bias, long long m, long long n, long long k, int out_type,
